@@ -26,7 +26,9 @@ ABI_VERSION = 1
 EXPORTS = ('sbl_version', 'sbl_last_error', 'sbl_has_tensor_path', 'sbl_workspace_bytes', 'sbl_forward',
            'sbl_key_logscale', 'sbl_key_summary', 'sbl_band_forward', 'sbl_query_features',
            'sbl_key_features', 'sbl_attention_weights', 'sbl_check_status', 'sbl_selftest_wait_timeout',
-           'sbl_key_logscale_static', 'sbl_static_last_error', 'sbl_status_words')
+           'sbl_key_logscale_static', 'sbl_static_last_error', 'sbl_status_words', 'sbl_forward_train',
+           'sbl_backward_workspace_bytes', 'sbl_backward', 'sbl_norm_rotary_forward',
+           'sbl_norm_rotary_workspace_bytes', 'sbl_norm_rotary_backward')
 
 
 class SblParams(ctypes.Structure):
@@ -54,6 +56,50 @@ class SblParams(ctypes.Structure):
         ('sum_lo', ctypes.c_int32), ('sum_hi', ctypes.c_int32),
         ('flags', ctypes.c_int32),
         ('reserved', ctypes.c_int32 * 3),
+    ]
+
+
+class SblGrads(ctypes.Structure):
+    """Mirror of `struct SblGrads`."""
+    _fields_ = [
+        ('dout', ctypes.c_void_p), ('do_stride_b', ctypes.c_int64), ('do_stride_t', ctypes.c_int64),
+        ('do_stride_h', ctypes.c_int64),
+        ('row_stats', ctypes.c_void_p),
+        ('dq', ctypes.c_void_p), ('dq_stride_b', ctypes.c_int64), ('dq_stride_t', ctypes.c_int64),
+        ('dq_stride_h', ctypes.c_int64),
+        ('dk', ctypes.c_void_p), ('dk_stride_b', ctypes.c_int64), ('dk_stride_s', ctypes.c_int64),
+        ('dk_stride_h', ctypes.c_int64),
+        ('dv', ctypes.c_void_p), ('dv_stride_b', ctypes.c_int64), ('dv_stride_s', ctypes.c_int64),
+        ('dv_stride_h', ctypes.c_int64),
+        ('reserved', ctypes.c_int32 * 4),
+    ]
+
+
+class SblNormRotarySide(ctypes.Structure):
+    """Mirror of `struct SblNormRotarySide`."""
+    _fields_ = [
+        ('T', ctypes.c_int32), ('H', ctypes.c_int32),
+        ('x', ctypes.c_void_p), ('x_stride_b', ctypes.c_int64), ('x_stride_t', ctypes.c_int64),
+        ('x_stride_h', ctypes.c_int64),
+        ('y', ctypes.c_void_p), ('y_stride_b', ctypes.c_int64), ('y_stride_t', ctypes.c_int64),
+        ('y_stride_h', ctypes.c_int64),
+        ('dy', ctypes.c_void_p), ('dy_stride_b', ctypes.c_int64), ('dy_stride_t', ctypes.c_int64),
+        ('dy_stride_h', ctypes.c_int64),
+        ('weight', ctypes.c_void_p), ('dweight', ctypes.c_void_p),
+        ('positions', ctypes.c_void_p), ('pos_stride_b', ctypes.c_int64), ('pos_stride_t', ctypes.c_int64),
+        ('pos0', ctypes.c_int64),
+    ]
+
+
+class SblNormRotary(ctypes.Structure):
+    """Mirror of `struct SblNormRotary`."""
+    _fields_ = [
+        ('dtype', ctypes.c_int32), ('weight_dtype', ctypes.c_int32),
+        ('B', ctypes.c_int32), ('E', ctypes.c_int32),
+        ('rotary', ctypes.c_int32), ('interleaved', ctypes.c_int32),
+        ('eps', ctypes.c_double), ('theta', ctypes.c_double),
+        ('side', SblNormRotarySide * 2),
+        ('reserved', ctypes.c_int32 * 4),
     ]
 
 
@@ -121,6 +167,19 @@ def load():
         lib.sbl_key_logscale_static.argtypes = [P, vp, vp]
         lib.sbl_static_last_error.restype = ctypes.c_char_p
         lib.sbl_static_last_error.argtypes = []
+        G, R = ctypes.POINTER(SblGrads), ctypes.POINTER(SblNormRotary)
+        lib.sbl_forward_train.restype = ctypes.c_int
+        lib.sbl_forward_train.argtypes = [P, vp, sz, vp, vp]
+        lib.sbl_backward_workspace_bytes.restype = ctypes.c_int
+        lib.sbl_backward_workspace_bytes.argtypes = [P, ctypes.POINTER(sz)]
+        lib.sbl_backward.restype = ctypes.c_int
+        lib.sbl_backward.argtypes = [P, G, vp, sz, vp]
+        lib.sbl_norm_rotary_forward.restype = ctypes.c_int
+        lib.sbl_norm_rotary_forward.argtypes = [R, vp]
+        lib.sbl_norm_rotary_workspace_bytes.restype = ctypes.c_int
+        lib.sbl_norm_rotary_workspace_bytes.argtypes = [R, ctypes.POINTER(sz)]
+        lib.sbl_norm_rotary_backward.restype = ctypes.c_int
+        lib.sbl_norm_rotary_backward.argtypes = [R, vp, sz, vp]
         if lib.sbl_version() != ABI_VERSION:
             raise ImportError(f'{path} has ABI version {lib.sbl_version()}, expected {ABI_VERSION}: rebuild')
         _lib = lib

@@ -74,6 +74,40 @@ int check_workspace(const Workspace& ws, void* workspace, size_t bytes) {
   return SBL_OK;
 }
 
+// What the training entry points ask for on top of validate().
+int validate_training(const SblParams* p) {
+  int rc = validate(p);
+  if (rc != SBL_OK) return rc;
+  if (p->softmax_eps != 0.f) return fail(SBL_ERR_UNSUPPORTED, "gradients are built for softmax_eps = 0 only");
+  if (p->q_pos0 != 0 || p->k_pos0 != 0 || p->S_total != p->S || p->sum_lo != 0 || p->sum_hi != p->S)
+    return fail(SBL_ERR_UNSUPPORTED, "gradients are not built for sequence shards");
+  return SBL_OK;
+}
+
+int validate_norm_rotary(const SblNormRotary* p, bool backward) {
+  if (!p) return fail(SBL_ERR_INVALID_ARGUMENT, "params is null");
+  for (int dt : {p->dtype, p->weight_dtype})
+    if (dt != SBL_DTYPE_F32 && dt != SBL_DTYPE_BF16)
+      return fail(SBL_ERR_INVALID_ARGUMENT, "dtype %d is not SBL_DTYPE_F32 or SBL_DTYPE_BF16", dt);
+  if (p->B < 0 || p->E <= 0) return fail(SBL_ERR_INVALID_ARGUMENT, "B must be >= 0 and E positive (got %d, %d)", p->B, p->E);
+  if (p->E > SBL_NORM_ROTARY_MAX_E)
+    return fail(SBL_ERR_UNSUPPORTED, "head dim E=%d > %d has no kernel", p->E, SBL_NORM_ROTARY_MAX_E);
+  if (p->rotary < 0 || p->rotary > p->E || p->rotary % 2 != 0)
+    return fail(SBL_ERR_INVALID_ARGUMENT, "rotary=%d must be even and in 0..E=%d", p->rotary, p->E);
+  if (p->interleaved != 0 && p->interleaved != 1) return fail(SBL_ERR_INVALID_ARGUMENT, "interleaved must be 0 or 1");
+  if (!(p->eps >= 0.0)) return fail(SBL_ERR_INVALID_ARGUMENT, "eps must be >= 0");
+  if (!(p->theta > 0.0)) return fail(SBL_ERR_INVALID_ARGUMENT, "theta must be > 0");
+  for (int r : p->reserved)
+    if (r != 0) return fail(SBL_ERR_INVALID_ARGUMENT, "reserved fields must be 0");
+  for (const SblNormRotarySide& s : p->side) {
+    if (s.T < 0 || s.H <= 0) return fail(SBL_ERR_INVALID_ARGUMENT, "T must be >= 0 and H positive (got %d, %d)", s.T, s.H);
+    if (s.T == 0 || p->B == 0) continue;
+    if (!s.x || !s.y) return fail(SBL_ERR_INVALID_ARGUMENT, "x and y must be non-null device pointers");
+    if (backward && !s.dy) return fail(SBL_ERR_INVALID_ARGUMENT, "dy must be a non-null device pointer");
+  }
+  return SBL_OK;
+}
+
 int prepare(const SblParams* p, void* workspace, size_t bytes, Workspace* ws) {
   int rc = validate(p);
   if (rc != SBL_OK) return rc;
@@ -209,7 +243,7 @@ int sbl_band_forward(const SblParams* p, void* workspace, size_t workspace_bytes
   return SBL_OK;
 }
 
-int sbl_forward(const SblParams* p, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+static int forward(const SblParams* p, void* workspace, size_t workspace_bytes, float* row_stats, void* cuda_stream) {
   Workspace ws;
   int rc = prepare(p, workspace, workspace_bytes, &ws);
   if (rc != SBL_OK) return rc;
@@ -226,7 +260,7 @@ int sbl_forward(const SblParams* p, void* workspace, size_t workspace_bytes, voi
     if ((e = tc_key_logscale_bound(*p, ws, base, beta, st, true)) != cudaSuccess)
       return cuda_fail(e, "key logscale bound");
     if ((e = tc_key_summary(*p, ws, base, beta, kv, ksum, st, true)) != cudaSuccess) return cuda_fail(e, "key summary");
-    if ((e = tc_band(*p, ws, base, beta, kv, ksum, st, true)) != cudaSuccess) return cuda_fail(e, "band forward");
+    if ((e = tc_band(*p, ws, base, beta, kv, ksum, st, true, row_stats)) != cudaSuccess) return cuda_fail(e, "band forward");
     return SBL_OK;
   }
   float* phik = reinterpret_cast<float*>(base + ws.phik);
@@ -238,7 +272,79 @@ int sbl_forward(const SblParams* p, void* workspace, size_t workspace_bytes, voi
                               reinterpret_cast<float*>(base + ws.qls), st)) != cudaSuccess)
     return cuda_fail(e, "query features");
   if ((e = f32_band(*p, ws, base, beta, kv, ksum, st)) != cudaSuccess) return cuda_fail(e, "band forward");
+  if (row_stats && (e = f32_row_stats(*p, ws, base, row_stats, st)) != cudaSuccess) return cuda_fail(e, "row statistics");
   return SBL_OK;
+}
+
+int sbl_forward(const SblParams* p, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+  return forward(p, workspace, workspace_bytes, nullptr, cuda_stream);
+}
+
+int sbl_forward_train(const SblParams* p, void* workspace, size_t workspace_bytes, float* row_stats,
+                      void* cuda_stream) {
+  int rc = validate_training(p);
+  if (rc != SBL_OK) return rc;
+  if (!row_stats) return fail(SBL_ERR_INVALID_ARGUMENT, "row_stats is null");
+  return forward(p, workspace, workspace_bytes, row_stats, cuda_stream);
+}
+
+int sbl_backward_workspace_bytes(const SblParams* p, size_t* bytes) {
+  if (!bytes) return fail(SBL_ERR_INVALID_ARGUMENT, "bytes is null");
+  int rc = validate_training(p);
+  if (rc != SBL_OK) return rc;
+  BwdWorkspace ws;
+  f32_plan_backward(*p, &ws);
+  *bytes = ws.total;
+  return SBL_OK;
+}
+
+int sbl_backward(const SblParams* p, const SblGrads* g, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+  int rc = validate_training(p);
+  if (rc != SBL_OK) return rc;
+  if (!g) return fail(SBL_ERR_INVALID_ARGUMENT, "grads is null");
+  if (!g->dout || !g->row_stats || !g->dq || !g->dk || !g->dv)
+    return fail(SBL_ERR_INVALID_ARGUMENT, "dout, row_stats, dq, dk and dv must be non-null device pointers");
+  for (int r : g->reserved)
+    if (r != 0) return fail(SBL_ERR_INVALID_ARGUMENT, "reserved fields must be 0");
+  cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+  BwdWorkspace ws;
+  f32_plan_backward(*p, &ws);
+  if ((rc = check_workspace(ws.fwd, workspace, workspace_bytes)) != SBL_OK) return rc;
+  cudaError_t e = f32_backward(*p, *g, ws, static_cast<char*>(workspace), st);
+  return e == cudaSuccess ? SBL_OK : cuda_fail(e, "backward");
+}
+
+int sbl_norm_rotary_forward(const SblNormRotary* p, void* cuda_stream) {
+  int rc = validate_norm_rotary(p, false);
+  if (rc != SBL_OK) return rc;
+  if (p->B == 0 || (p->side[0].T == 0 && p->side[1].T == 0)) return SBL_OK;
+  cudaError_t e = norm_rotary(*p, false, nullptr, static_cast<cudaStream_t>(cuda_stream));
+  return e == cudaSuccess ? SBL_OK : cuda_fail(e, "norm and rotation");
+}
+
+int sbl_norm_rotary_workspace_bytes(const SblNormRotary* p, size_t* bytes) {
+  if (!bytes) return fail(SBL_ERR_INVALID_ARGUMENT, "bytes is null");
+  int rc = validate_norm_rotary(p, true);
+  if (rc != SBL_OK) return rc;
+  *bytes = norm_rotary_partial_bytes(*p);
+  return SBL_OK;
+}
+
+int sbl_norm_rotary_backward(const SblNormRotary* p, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+  int rc = validate_norm_rotary(p, true);
+  if (rc != SBL_OK) return rc;
+  const bool weights = p->side[0].dweight || p->side[1].dweight;
+  if (weights) {
+    const size_t need = norm_rotary_partial_bytes(*p);
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < need)
+      return fail(SBL_ERR_WORKSPACE, "workspace must be 16-byte aligned and hold %zu bytes (has %zu)", need,
+                  workspace ? workspace_bytes : (size_t)0);
+  }
+  // (a batch without rows still gets its weight gradients: zeros)
+  if (!weights && (p->B == 0 || (p->side[0].T == 0 && p->side[1].T == 0))) return SBL_OK;
+  cudaError_t e = norm_rotary(*p, true, weights ? static_cast<float*>(workspace) : nullptr,
+                              static_cast<cudaStream_t>(cuda_stream));
+  return e == cudaSuccess ? SBL_OK : cuda_fail(e, "norm and rotation gradients");
 }
 
 int sbl_attention_weights(const SblParams* p, void* workspace, size_t workspace_bytes, float* attn,

@@ -50,8 +50,37 @@ cudaError_t f32_query_features(const SblParams& p, const Workspace& ws, char* ba
 cudaError_t f32_band(const SblParams& p, const Workspace& ws, char* base, const float* beta,
                      const float* kv, const float* ksum, cudaStream_t st);
 
+// psi(q_t) = exp(+-u - tau|q|^2/2 - ln(m)/2 - row_scale[t]): query features over a scale per row
+cudaError_t f32_query_features_over(const SblParams& p, const Workspace& ws, char* base, const float* row_scale,
+                                    float* psi, cudaStream_t st);
+cudaError_t f32_query_summary(const SblParams& p, const SblGrads& g, const float* psi, const float* delta,
+                              int split_rows, int nsplit, float* partial, float* qg, float* qd, cudaStream_t st);
 cudaError_t f32_attention_weights(const SblParams& p, const Workspace& ws, char* base, const float* beta,
                                   float* attn, float* attn_un, float* attn_lr, cudaStream_t st);
+
+// ---- gradients, generic path (any E, D, r, w; fp32 math), sbl_bwd_f32.cu ----
+// One buffer for the whole backward pass.  `fwd` is the view the forward's feature and summary kernels take; its
+// sections lie inside the same buffer.
+struct BwdWorkspace {
+  Workspace fwd;
+  size_t lognorm;   // (BH,T) log-normaliser of a query row
+  size_t scale;     // (BH,T) the same minus beta: what psi is divided by
+  size_t delta;     // (BH,T) dout . out
+  size_t psi;       // (BH,T,m)
+  size_t qg, qd;    // (BH,m,D), (BH,m): query-side summary
+  size_t h;         // (BH,max(T,S),m): feature times its gradient
+  size_t partial;   // split partials of the query-side summary
+  size_t total;
+  int nsplit, split_rows;
+};
+void f32_plan_backward(const SblParams& p, BwdWorkspace* ws);
+cudaError_t f32_backward(const SblParams& p, const SblGrads& g, const BwdWorkspace& ws, char* base, cudaStream_t st);
+// row_stats (2,BH,T) of a generic forward: its log-normalisers, and ones
+cudaError_t f32_row_stats(const SblParams& p, const Workspace& ws, char* base, float* row_stats, cudaStream_t st);
+
+// ---- norm and rotation of heads, sbl_rotary.cu ----
+size_t norm_rotary_partial_bytes(const SblNormRotary& p);
+cudaError_t norm_rotary(const SblNormRotary& p, bool backward, float* partial, cudaStream_t st);
 
 // ---- tensor-core path (bf16 storage, tcgen05 + TMA), sbl_tc.cu ----
 bool tc_supported(const SblParams& p);
@@ -67,7 +96,8 @@ cudaError_t tc_key_logscale_bound(const SblParams& p, const Workspace& ws, char*
 cudaError_t tc_key_summary(const SblParams& p, const Workspace& ws, char* base, const float* beta,
                            float* kv, float* ksum, cudaStream_t st, bool also_bf16 = false);
 cudaError_t tc_band(const SblParams& p, const Workspace& ws, char* base, const float* beta,
-                    const float* kv, const float* ksum, cudaStream_t st, bool kv16_ready = false);
+                    const float* kv, const float* ksum, cudaStream_t st, bool kv16_ready = false,
+                    float* row_stats = nullptr);
 // runs a kernel whose only wait can never be satisfied; *host_status receives the recorded wait site (99)
 cudaError_t tc_wait_selftest(int* device_status, int* host_status, cudaStream_t st);
 // copies the three device status words (host_status[0]: wait site that ran out, host_status[1]: 1 if an

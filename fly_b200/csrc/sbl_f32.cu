@@ -7,97 +7,10 @@
 // All matrix products are register-tiled 64x64 block tiles (4x4 per thread,
 // 256 threads) fed from shared memory in K-slices of 16 with the next slice
 // prefetched into registers.
-#include "sbl_common.cuh"
+#include "sbl_f32_tile.cuh"
 
 namespace sbl {
 namespace {
-
-constexpr int TILE = 64;       // block tile edge
-constexpr int KS = 16;         // K slice
-constexpr int LDT = TILE + 4;  // shared leading dimension (keeps float4 rows 16-byte aligned)
-constexpr int NTHR = 256;
-constexpr int PER_THR = TILE * KS / NTHR;  // slice elements per thread = 4
-
-__device__ __forceinline__ float ldf(const float* p) { return *p; }
-__device__ __forceinline__ float ldf(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void stf(float* p, float x) { *p = x; }
-__device__ __forceinline__ void stf(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
-
-// atomic max on a float through its ordered integer image
-__device__ __forceinline__ void atomic_max_float(float* addr, float v) {
-  if (v >= 0.f) atomicMax(reinterpret_cast<int*>(addr), __float_as_int(v));
-  else atomicMin(reinterpret_cast<unsigned int*>(addr), __float_as_uint(v));
-}
-
-// Fetches this thread's share of a TILE x KS slice (rows of a row-major
-// matrix, K-contiguous) into registers; out-of-range elements read as 0.
-template <typename T>
-__device__ __forceinline__ void fetch_slice(float (&reg)[PER_THR], const T* base, int64_t ld, int nrows,
-                                            int k0, int K) {
-#pragma unroll
-  for (int i = 0; i < PER_THR; ++i) {
-    const int idx = threadIdx.x + i * NTHR;
-    const int row = idx / KS, kk = idx % KS;
-    reg[i] = (row < nrows && k0 + kk < K) ? ldf(base + (int64_t)row * ld + k0 + kk) : 0.f;
-  }
-}
-__device__ __forceinline__ void stash_slice(float (*s)[LDT], const float (&reg)[PER_THR]) {
-#pragma unroll
-  for (int i = 0; i < PER_THR; ++i) {
-    const int idx = threadIdx.x + i * NTHR;
-    s[idx % KS][idx / KS] = reg[i];
-  }
-}
-
-// acc(64x64) += A(64 x K) * B(64 x K)^T, both operands K-contiguous in global
-// memory.  Thread (ty,tx) owns rows ty*4.., cols tx*4...
-template <typename TA, typename TB>
-__device__ __forceinline__ void tile_nt(float (&acc)[4][4], const TA* A, int64_t lda, int na, const TB* B,
-                                        int64_t ldb, int nb, int K, float (*sA)[LDT], float (*sB)[LDT]) {
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  float ra[PER_THR], rb[PER_THR];
-  fetch_slice(ra, A, lda, na, 0, K);
-  fetch_slice(rb, B, ldb, nb, 0, K);
-  for (int k0 = 0; k0 < K; k0 += KS) {
-    __syncthreads();
-    stash_slice(sA, ra);
-    stash_slice(sB, rb);
-    __syncthreads();
-    if (k0 + KS < K) {
-      fetch_slice(ra, A, lda, na, k0 + KS, K);
-      fetch_slice(rb, B, ldb, nb, k0 + KS, K);
-    }
-    // two-level sum: one partial per K slice, so the rounding error grows with K/16, not K
-    // (the feature dimension can be tens of thousands)
-    float part[4][4] = {};
-#pragma unroll
-    for (int kk = 0; kk < KS; ++kk) {
-      const float4 a = *reinterpret_cast<const float4*>(&sA[kk][ty * 4]);
-      const float4 b = *reinterpret_cast<const float4*>(&sB[kk][tx * 4]);
-      const float av[4] = {a.x, a.y, a.z, a.w};
-      const float bv[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) part[i][j] = fmaf(av[i], bv[j], part[i][j]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] += part[i][j];
-  }
-}
-
-__device__ __forceinline__ float group16_max(float v) {
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-__device__ __forceinline__ float group16_sum(float v) {
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
 
 // ---------------------------------------------------------------------------
 // sqrt(tau) * W  (feature_maps_sb.py:62-64: the projection is scaled before
@@ -114,7 +27,7 @@ __global__ void fill_kernel(float* p, float v, int n) {
 
 // ---------------------------------------------------------------------------
 // Feature map (feature_maps_sb.py:51-82).  One block = 64 rows of one (b,h).
-enum { MODE_QUERY = 0, MODE_KEYMAX = 1, MODE_KEY = 2 };
+enum { MODE_QUERY = 0, MODE_KEYMAX = 1, MODE_KEY = 2, MODE_ROW = 3 };
 
 struct FeatArgs {
   const void* x;
@@ -123,7 +36,8 @@ struct FeatArgs {
   const float* Wt;
   float tau, half_log_m, eps_m;
   float* phi;             // (BH, rows, m): QUERY and KEY
-  float* ls;              // QUERY: (BH, rows) log-scales; KEYMAX: beta out (BH); KEY: beta in (BH)
+  float* ls;              // QUERY: (BH, rows) log-scales; KEYMAX: beta out (BH); KEY: beta in (BH);
+                          // ROW: (BH, rows) log-scale in, one per row (gradients: features over the row's normaliser)
   const int64_t* lengths; // KEY
   int64_t pos0, S_total;  // KEY: global position of row 0, global key count
   int row_lo, row_hi;     // rows processed
@@ -163,6 +77,7 @@ __global__ void __launch_bounds__(NTHR) feat_kernel(FeatArgs a) {
     beta = a.ls[bh];
     len_b = a.lengths ? a.lengths[b] : a.S_total;
   }
+  const float* row_ls = MODE == MODE_ROW ? a.ls + (int64_t)bh * a.rows + row0 : nullptr;
   float* phi_rows = (MODE == MODE_KEYMAX) ? nullptr : a.phi + ((int64_t)bh * a.rows + row0) * m;
 
   for (int c0 = 0; c0 < a.r; c0 += TILE) {
@@ -185,7 +100,8 @@ __global__ void __launch_bounds__(NTHR) feat_kernel(FeatArgs a) {
           run_max[i] = fmaxf(run_max[i], (fabsf(u) - g) - a.half_log_m);
         } else {
           float e1 = 0.f, e2 = 0.f;
-          if (a.pos0 + row0 + row < len_b) {
+          if (MODE == MODE_ROW) beta = row_ls[row];
+          if (MODE == MODE_ROW || a.pos0 + row0 + row < len_b) {
             e1 = expf(((u - g) - a.half_log_m) - beta) + a.eps_m;
             e2 = expf(((-u - g) - a.half_log_m) - beta) + a.eps_m;
           }
@@ -229,11 +145,13 @@ __global__ void __launch_bounds__(NTHR) feat_kernel(FeatArgs a) {
 
 // ---------------------------------------------------------------------------
 // Summary: partial[bh][split] (m x (D+1)) = phi(K)[rows]^T [V | 1]
-// (scatterbrain_utils.py:20,49).  The extra column carries sum_s phi(k_s).
+// (scatterbrain_utils.py:20,49).  The extra column carries sum_s phi(k_s), or,
+// with `last` (BH, S), sum_s last_s phi(k_s).
 template <typename T>
 __global__ void __launch_bounds__(NTHR)
 summary_partial_kernel(const float* phik, const void* vptr, int64_t sb, int64_t ss, int64_t sh, int S, int m,
-                       int D, int H, int row_lo, int row_hi, int split_rows, int dtiles, float* partial) {
+                       int D, int H, int row_lo, int row_hi, int split_rows, int dtiles, float* partial,
+                       const float* last) {
   __shared__ __align__(16) float sA[KS][LDT];
   __shared__ __align__(16) float sB[KS][LDT];
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
@@ -255,7 +173,7 @@ summary_partial_kernel(const float* phik, const void* vptr, int64_t sb, int64_t 
       const bool in = s < s_end;
       sA[kk][c] = (in && f0 + c < m) ? pk[(int64_t)s * m + f0 + c] : 0.f;
       const int d = d0 + c;
-      sB[kk][c] = !in ? 0.f : (d < D ? ldf(v + (int64_t)s * ss + d) : (d == D ? 1.f : 0.f));
+      sB[kk][c] = !in ? 0.f : (d < D ? ldf(v + (int64_t)s * ss + d) : (d == D ? (last ? last[(int64_t)bh * S + s] : 1.f) : 0.f));
     }
     __syncthreads();
     float part[4][4] = {};   // two-level sum over the keys
@@ -626,14 +544,34 @@ cudaError_t f32_key_summary(const SblParams& p, const Workspace& ws, char* base,
   if (p.dtype == SBL_DTYPE_F32)
     summary_partial_kernel<float><<<grid, NTHR, 0, st>>>(phik, p.v, p.v_stride_b, p.v_stride_s, p.v_stride_h, p.S,
                                                          m, p.D, p.H, p.sum_lo, p.sum_hi, ws.split_rows, dtiles,
-                                                         partial);
+                                                         partial, nullptr);
   else
     summary_partial_kernel<__nv_bfloat16><<<grid, NTHR, 0, st>>>(phik, p.v, p.v_stride_b, p.v_stride_s,
                                                                  p.v_stride_h, p.S, m, p.D, p.H, p.sum_lo, p.sum_hi,
-                                                                 ws.split_rows, dtiles, partial);
+                                                                 ws.split_rows, dtiles, partial, nullptr);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return f32_combine_partials(p, ws, base, kv, ksum, st);
+}
+
+// The summary of the gradients, over the query rows: qg (BH,m,D) = psi^T dout, qd (BH,m) = sum_t delta_t psi_t.
+cudaError_t f32_query_summary(const SblParams& p, const SblGrads& g, const float* psi, const float* delta,
+                              int split_rows, int nsplit, float* partial, float* qg, float* qd, cudaStream_t st) {
+  const int m = 2 * p.r, bh = p.B * p.H;
+  const int dtiles = (int)div_up(p.D + 1, TILE), mtiles = (int)div_up(m, TILE);
+  dim3 grid((unsigned)(mtiles * dtiles), (unsigned)nsplit, (unsigned)bh);
+  if (p.dtype == SBL_DTYPE_F32)
+    summary_partial_kernel<float><<<grid, NTHR, 0, st>>>(psi, g.dout, g.do_stride_b, g.do_stride_t, g.do_stride_h, p.T,
+                                                         m, p.D, p.H, 0, p.T, split_rows, dtiles, partial, delta);
+  else
+    summary_partial_kernel<__nv_bfloat16><<<grid, NTHR, 0, st>>>(psi, g.dout, g.do_stride_b, g.do_stride_t,
+                                                                 g.do_stride_h, p.T, m, p.D, p.H, 0, p.T, split_rows,
+                                                                 dtiles, partial, delta);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const int64_t n = (int64_t)bh * m * (p.D + 1);
+  summary_combine_kernel<<<(unsigned)div_up(n, 256), 256, 0, st>>>(partial, nsplit, m, p.D, bh, qg, qd);
+  return cudaGetLastError();
 }
 
 cudaError_t f32_combine_partials(const SblParams& p, const Workspace& ws, char* base, float* kv, float* ksum,
@@ -651,6 +589,15 @@ cudaError_t f32_query_features(const SblParams& p, const Workspace& ws, char* ba
   a.phi = phiq_out;
   a.ls = qls_out;
   return launch_feat<MODE_QUERY>(p, a, st);
+}
+
+cudaError_t f32_query_features_over(const SblParams& p, const Workspace& ws, char* base, const float* row_scale,
+                                    float* psi, cudaStream_t st) {
+  FeatArgs a = feat_args(p, ws, base, true);
+  a.ls = const_cast<float*>(row_scale);
+  a.phi = psi;
+  a.eps_m = 0.f;
+  return launch_feat<MODE_ROW>(p, a, st);
 }
 
 cudaError_t f32_attention_weights(const SblParams& p, const Workspace& ws, char* base, const float* beta,

@@ -625,6 +625,7 @@ struct BandArgs {
   const float* ksum;     // (BH, 256) fp32, reference feature order
   const float* wmax;     // [1]: max_f |sqrt(tau) w_f| of the bf16 projection
   int* status;
+  float* row_stats;      // (2,BH,T): query + key log-scale and normaliser of every row, for the gradients; or null
   int ntq;               // query tiles per (b,h)
   int ntiles;            // ntq * B * H
 };
@@ -744,6 +745,8 @@ struct PkTrack {
 // query tile `it` uses slot (2 it + h) % 3, use number (2 it + h) / 3 of that slot.  Both halves of
 // tile it + 1 are formed while tile it is processed: half 0 in the slot tile it does not use, half 1
 // in the slot of tile it's half 0 as soon as the last P product has read that.
+// STATS: also leave a.row_stats (its own instance: two more live values cost the forward registers)
+template <bool STATS>
 __global__ void __launch_bounds__(band::NTHREADS, 1) tc_band_kernel(const __grid_constant__ BandArgs a) {
   using namespace band;
   extern __shared__ uint8_t smem_raw[];
@@ -1308,6 +1311,7 @@ __global__ void __launch_bounds__(band::NTHREADS, 1) tc_band_kernel(const __grid
           if (it >= 2) mbar_wait(bars + B_XFREE + (it & 1), ((it >> 1) - 1) & 1, a.status, 47);
           s_lz[(it & 1) * 512 + cq * 128 + row] = L;
           s_lz[(it & 1) * 512 + 256 + cq * 128 + row] = z_c;
+          if (STATS && cq == 0 && row < T.nq) a.row_stats[(int64_t)T.bh * p.T + T.i0 + row] = pls;
           warp_arrive(bars + B_LZFULL + (it & 1), lane);
           gk += nt;
         }
@@ -1374,7 +1378,10 @@ __global__ void __launch_bounds__(band::NTHREADS, 1) tc_band_kernel(const __grid
         tc_fence_after_sync();
         // The reference clamps Z - dps at 1e-24 in ITS feature units; ours are smaller by the slack of the bound
         // stabilisers (e^-5 ... e^-50), so the constant here is the smallest that still keeps the division finite.
-        const float inv = 1.f / fmaxf(ZD, L + 1e-37f);
+        const float norm = fmaxf(ZD, L + 1e-37f);
+        const float inv = 1.f / norm;
+        if (STATS && cq == 0 && row < T.nq)
+          a.row_stats[(int64_t)(p.B * p.H + T.bh) * p.T + T.i0 + row] = norm;
         // Nothing here is ever rescaled, so for inputs far above unit-variance logits the exponentials leave the
         // fp32 range (queries and keys ~15 times the unit scale), or every feature of a row falls under it (the
         // bound stabilisers' slack grows with the norms): record either instead of returning it silently.
@@ -1556,8 +1563,8 @@ cudaError_t tc_key_summary(const SblParams& p, const Workspace& ws, char* base, 
 }
 
 cudaError_t tc_band(const SblParams& p, const Workspace& ws, char* base, const float* beta, const float* kv,
-                    const float* ksum, cudaStream_t st, bool kv16_ready) {
-  if (tc128_shape(p)) return tc128_band(p, ws, base, beta, kv, ksum, st, kv16_ready);
+                    const float* ksum, cudaStream_t st, bool kv16_ready, float* row_stats) {
+  if (tc128_shape(p)) return tc128_band(p, ws, base, beta, kv, ksum, st, kv16_ready, row_stats);
   const TcLayout l = tc_layout(ws, base);
   cudaError_t e = cudaSuccess;
   if (!kv16_ready) {
@@ -1589,18 +1596,21 @@ cudaError_t tc_band(const SblParams& p, const Workspace& ws, char* base, const f
   a.ksum = ksum;
   a.wmax = l.wmax;
   a.status = l.status;
+  a.row_stats = row_stats;
   a.ntq = (int)div_up(p.T, band::BQ);
   a.ntiles = a.ntq * p.B * p.H;
   DeviceInfo* dev = nullptr;
   if ((e = device_info(&dev)) != cudaSuccess) return e;
-  if (!dev->attr_band) {
-    e = cudaFuncSetAttribute(tc_band_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)band::SMEM_BYTES);
+  const bool stats = row_stats != nullptr;
+  const auto kernel = stats ? tc_band_kernel<true> : tc_band_kernel<false>;
+  if (!dev->attr_band[stats]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)band::SMEM_BYTES);
     if (e != cudaSuccess) return e;
-    dev->attr_band = true;
+    dev->attr_band[stats] = true;
   }
   // persistent: one CTA per SM (shared and tensor memory allow no more), each walking its share of the query tiles
   const unsigned grid = (unsigned)(a.ntiles < dev->sms ? a.ntiles : dev->sms);
-  tc_band_kernel<<<grid, band::NTHREADS, band::SMEM_BYTES, st>>>(a);
+  kernel<<<grid, band::NTHREADS, band::SMEM_BYTES, st>>>(a);
   return cudaGetLastError();
 }
 

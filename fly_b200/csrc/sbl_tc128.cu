@@ -437,6 +437,7 @@ struct Band128Args {
   const float* ksum;     // (BH, 512) fp32, internal feature order
   const float* wmax;     // [1]: max_f |sqrt(tau) w_f| of the bf16 projection
   int* status;
+  float* row_stats;      // (2,BH,T): query + key log-scale and normaliser of every row, for the gradients; or null
   int ntq;               // query tiles per (b,h)
   int ntiles;            // ntq * B * H
 };
@@ -542,6 +543,8 @@ struct RingPos {
 //   t = 1..nt:  Wt half 0 of the next tile [t = nt] | V(t-1) | K(t+1) [t+1 < nt] |   the output staging slot
 // and the phi(K) ring 4 nt pieces:  t = 0..nt-1:  phi(K)_0(t) (2), phi(K)_1(t) (2).
 // Key tile t of a query tile uses buffer (G + t) & 1, G = key tiles of the earlier query tiles of this CTA.
+// STATS: also leave a.row_stats (its own instance: two more live values cost the forward registers)
+template <bool STATS>
 __global__ void __launch_bounds__(band128::NTHREADS, 1) tc128_band_kernel(const __grid_constant__ Band128Args a) {
   using namespace band128;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -1003,6 +1006,7 @@ __global__ void __launch_bounds__(band128::NTHREADS, 1) tc128_band_kernel(const 
         if (it >= 1) ph.wait(bars, B_LZFREE, a.status, 173);
         s_lz[cq * 128 + row] = L;
         s_lz[256 + cq * 128 + row] = z;
+        if (STATS && cq == 0 && row < T.nq) a.row_stats[(int64_t)T.bh * p.T + T.i0 + row] = pls;
         warp_arrive(bars + B_LZFULL, lane);
       }
     } else {
@@ -1071,7 +1075,10 @@ __global__ void __launch_bounds__(band128::NTHREADS, 1) tc128_band_kernel(const 
         tc_fence_after_sync();
         // The reference clamps Z - dps at 1e-24 in ITS feature units; ours are smaller by the slack of the bound
         // stabilisers, so the constant here is the smallest that still keeps the division finite.
-        const float inv = 1.f / fmaxf(ZD, L + 1e-37f);
+        const float norm = fmaxf(ZD, L + 1e-37f);
+        const float inv = 1.f / norm;
+        if (STATS && cq == 0 && row < T.nq)
+          a.row_stats[(int64_t)(p.B * p.H + T.bh) * p.T + T.i0 + row] = norm;
         // Nothing is ever rescaled: for inputs far above unit-variance logits the exponentials leave the fp32
         // range, or every feature of a row falls under it.  Record either instead of returning it silently.
         if (!(L < 1e30f) || !(fabsf(ZD) < 1e30f) || (Zrow == 0.f && T.len_b > 0)) a.status[1] = 1;
@@ -1185,7 +1192,7 @@ cudaError_t tc128_key_summary(const SblParams& p, const Workspace& ws, char* bas
 }
 
 cudaError_t tc128_band(const SblParams& p, const Workspace& ws, char* base, const float* beta, const float* kv,
-                       const float* ksum, cudaStream_t st, bool kv16_ready) {
+                       const float* ksum, cudaStream_t st, bool kv16_ready, float* row_stats) {
   const TcLayout l = tc_layout(ws, base);
   cudaError_t e = cudaSuccess;
   if (!kv16_ready) {
@@ -1217,18 +1224,21 @@ cudaError_t tc128_band(const SblParams& p, const Workspace& ws, char* base, cons
   a.ksum = ksum_slots(ws, base);
   a.wmax = l.wmax;
   a.status = l.status;
+  a.row_stats = row_stats;
   a.ntq = (int)div_up(p.T, band128::BQ);
   a.ntiles = a.ntq * p.B * p.H;
   DeviceInfo* dev = nullptr;
   if ((e = device_info(&dev)) != cudaSuccess) return e;
-  if (!dev->attr_band128) {
-    e = cudaFuncSetAttribute(tc128_band_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)band128::SMEM_BYTES);
+  const bool stats = row_stats != nullptr;
+  const auto kernel = stats ? tc128_band_kernel<true> : tc128_band_kernel<false>;
+  if (!dev->attr_band128[stats]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)band128::SMEM_BYTES);
     if (e != cudaSuccess) return e;
-    dev->attr_band128 = true;
+    dev->attr_band128[stats] = true;
   }
   // persistent: one CTA per SM (shared and tensor memory allow no more), each walking its share of the query tiles
   const unsigned grid = (unsigned)(a.ntiles < dev->sms ? a.ntiles : dev->sms);
-  tc128_band_kernel<<<grid, band128::NTHREADS, band128::SMEM_BYTES, st>>>(a);
+  kernel<<<grid, band128::NTHREADS, band128::SMEM_BYTES, st>>>(a);
   return cudaGetLastError();
 }
 

@@ -25,9 +25,9 @@ bool map_bthe(CUtensorMap* m, const void* base, int B, int rows, int H, int E, i
 struct DeviceInfo {
   int sms = 0;
   bool attr_keys[2] = {false, false};
-  bool attr_band = false;
+  bool attr_band[2] = {false, false};   // without, with row statistics
   bool attr_keys128 = false;
-  bool attr_band128 = false;
+  bool attr_band128[2] = {false, false};
 };
 cudaError_t device_info(DeviceInfo** out);
 
@@ -49,6 +49,6 @@ bool tc128_shape(const SblParams& p);
 cudaError_t tc128_key_summary(const SblParams& p, const Workspace& ws, char* base, const float* beta, float* kv,
                               float* ksum, cudaStream_t st, bool also_bf16);
 cudaError_t tc128_band(const SblParams& p, const Workspace& ws, char* base, const float* beta, const float* kv,
-                       const float* ksum, cudaStream_t st, bool kv16_ready);
+                       const float* ksum, cudaStream_t st, bool kv16_ready, float* row_stats);
 
 }  // namespace sbl

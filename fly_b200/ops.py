@@ -163,6 +163,42 @@ class Problem:
                 status_watch.post(ws, self.status_offset, self.device)
         return self.out
 
+    def forward_train(self, workspace):
+        """Forward that also returns what `backward` needs of it: row statistics (2,B,H,T) fp32."""
+        B, H, T = self.shape[:3]
+        stats = torch.empty(2, B, H, T, device=self.device, dtype=torch.float32)
+        self._call(_cabi.load().sbl_forward_train, stats.data_ptr(), workspace=workspace)
+        return self.out, stats
+
+    def backward_workspace_bytes(self):
+        n = ctypes.c_size_t(0)
+        _cabi.check(_cabi.load().sbl_backward_workspace_bytes(ctypes.byref(self.params), ctypes.byref(n)))
+        return n.value
+
+    def backward(self, grad_out, row_stats):
+        """(dq, dk, dv) of sum(grad_out * out); the problem's `out` must hold the output of `forward_train`."""
+        query, key, value = self._keep[:3]
+        B, H, T, S, E, D = self.shape
+        if grad_out.shape != (B, T, H, D) or grad_out.dtype != query.dtype or grad_out.device != self.device:
+            raise ValueError('grad_out must be (B,T,H,D) in the input dtype on the problem device')
+        if grad_out.stride(-1) != 1:
+            grad_out = grad_out.contiguous()
+        nbytes = self.backward_workspace_bytes()
+        dq, dk, dv = (torch.empty(x.shape, device=self.device, dtype=x.dtype) for x in (query, key, value))
+        # of this call alone: a backward pass may run on another stream or be captured while another one is alive
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        g = _cabi.SblGrads()
+        g.dout, g.do_stride_b, g.do_stride_t, g.do_stride_h = grad_out.data_ptr(), *grad_out.stride()[:3]
+        g.row_stats = row_stats.data_ptr()
+        g.dq, g.dq_stride_b, g.dq_stride_t, g.dq_stride_h = dq.data_ptr(), *dq.stride()[:3]
+        g.dk, g.dk_stride_b, g.dk_stride_s, g.dk_stride_h = dk.data_ptr(), *dk.stride()[:3]
+        g.dv, g.dv_stride_b, g.dv_stride_s, g.dv_stride_h = dv.data_ptr(), *dv.stride()[:3]
+        with torch.cuda.device(self.device):
+            stream = torch.cuda.current_stream(self.device).cuda_stream
+            rc = _cabi.load().sbl_backward(ctypes.byref(self.params), ctypes.byref(g), ws.data_ptr(), nbytes, stream)
+        _cabi.check(rc)
+        return dq, dk, dv
+
     def check_status(self, workspace=None):
         """Synchronises the stream; raises if a kernel gave up on a bounded wait."""
         self._call(_cabi.load().sbl_check_status, workspace=workspace)
@@ -230,3 +266,178 @@ def sblocal_forward(query, key, value, W, local_context, softmax_temp=None, soft
     value (B,S,H,D) with projection W (r,E); one call of `sbl_forward`."""
     return Problem(query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths,
                    out).forward(watch=watch)
+
+
+class _SBLocal(torch.autograd.Function):
+    """Differentiable SBLocal attention: saves the inputs, the output and two floats per query row; the gradients
+    recompute the weights (sbl_backward)."""
+
+    @staticmethod
+    def forward(ctx, query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths, watch):
+        prob = Problem(query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths)
+        ctx.args = (local_context, softmax_temp, softmax_eps)
+        if softmax_eps != 0:
+            # the forward is built for eps != 0, its gradients are not
+            ctx.stats = None
+            return prob.forward(watch=watch)
+        # a workspace of this call alone, for the reason given in Problem.backward
+        ws = torch.empty(prob.workspace_bytes, dtype=torch.uint8, device=prob.device)
+        out, stats = prob.forward_train(ws)
+        if watch and prob.status_offset is not None and not torch.cuda.is_current_stream_capturing():
+            with torch.cuda.device(prob.device):
+                status_watch.post(ws, prob.status_offset, prob.device)
+        ctx.stats = True
+        ctx.save_for_backward(query, key, value, W, key_lengths, out, stats)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        if ctx.stats is None:
+            raise NotImplementedError('sblocal_b200: gradients are built for softmax_eps = 0 only')
+        query, key, value, W, key_lengths, out, stats = ctx.saved_tensors
+        prob = Problem(query, key, value, W, *ctx.args, key_lengths, out=out)
+        dq, dk, dv = prob.backward(grad_out, stats)
+        return dq, dk, dv, None, None, None, None, None, None
+
+
+def sblocal_attention(query, key, value, W, local_context, softmax_temp=None, softmax_eps=0.0, key_lengths=None,
+                      watch=False):
+    """`sblocal_forward` that autograd can differentiate in query, key and value (softmax_eps = 0; the projection W
+    and the lengths are constants).  Rows of a batch without any real key give an output and gradients of zero, and
+    padded keys gradients of zero.  Padded keys and values must hold finite numbers."""
+    if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
+        return _SBLocal.apply(query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths, watch)
+    return sblocal_forward(query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths, watch=watch)
+
+
+# ---- norm and rotation of query and key heads -------------------------------------------------------------------
+
+def _norm_rotary_params(xs, weights, positions, pos0, rotary_dim, theta, interleaved, eps):
+    """SblNormRotary of the inputs; the tensors it points to must stay alive."""
+    p = _cabi.SblNormRotary()
+    B, _, _, E = xs[0].shape
+    p.dtype = _DTYPES[xs[0].dtype]
+    w = weights[0] if weights[0] is not None else weights[1]
+    p.weight_dtype = _DTYPES[w.dtype] if w is not None else _cabi.SBL_DTYPE_F32
+    p.B, p.E, p.rotary, p.interleaved = B, E, rotary_dim, 1 if interleaved else 0
+    p.eps, p.theta = eps, theta
+    for i in range(2):
+        s, x = p.side[i], xs[i]
+        s.T, s.H = x.shape[1], x.shape[2]
+        s.x, s.x_stride_b, s.x_stride_t, s.x_stride_h = x.data_ptr(), *x.stride()[:3]
+        if weights[i] is not None:
+            s.weight = weights[i].data_ptr()
+        if positions[i] is not None:
+            s.positions = positions[i].data_ptr()
+            s.pos_stride_t = positions[i].stride(-1)
+            s.pos_stride_b = positions[i].stride(0) if positions[i].dim() == 2 else 0
+        s.pos0 = pos0
+    return p
+
+
+def _norm_rotary_forward(xs, weights, *args):
+    p = _norm_rotary_params(xs, weights, *args)
+    dev = xs[0].device
+    ys = tuple(torch.empty(x.shape, dtype=x.dtype, device=dev) for x in xs)
+    for s, y in zip(p.side, ys):
+        s.y, s.y_stride_b, s.y_stride_t, s.y_stride_h = y.data_ptr(), *y.stride()[:3]
+    with torch.cuda.device(dev):
+        rc = _cabi.load().sbl_norm_rotary_forward(ctypes.byref(p), torch.cuda.current_stream(dev).cuda_stream)
+    _cabi.check(rc)
+    return ys
+
+
+class _NormRotary(torch.autograd.Function):
+    """Saves the inputs only: the norms are recomputed with the gradients."""
+
+    @staticmethod
+    def forward(ctx, query, key, query_weight, key_weight, positions, key_positions, *args):
+        ctx.save_for_backward(query, key, query_weight, key_weight, positions, key_positions)
+        ctx.args = args
+        return _norm_rotary_forward((query, key), (query_weight, key_weight), (positions, key_positions), *args)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        query, key, query_weight, key_weight, positions, key_positions = ctx.saved_tensors
+        weights = (query_weight, key_weight)
+        p = _norm_rotary_params((query, key), weights, (positions, key_positions), *ctx.args)
+        dev = query.device
+        dys = [dy if dy.stride(-1) == 1 else dy.contiguous() for dy in (dq_out, dk_out)]
+        dxs = [torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (query, key)]
+        dws = [torch.empty_like(w) if w is not None and ctx.needs_input_grad[2 + i] else None
+               for i, w in enumerate(weights)]
+        for s, dy, dx, dw in zip(p.side, dys, dxs, dws):
+            s.dy, s.dy_stride_b, s.dy_stride_t, s.dy_stride_h = dy.data_ptr(), *dy.stride()[:3]
+            s.y, s.y_stride_b, s.y_stride_t, s.y_stride_h = dx.data_ptr(), *dx.stride()[:3]
+            if dw is not None:
+                s.dweight = dw.data_ptr()
+        lib = _cabi.load()
+        ws, nbytes = None, 0
+        if dws[0] is not None or dws[1] is not None:
+            n = ctypes.c_size_t(0)
+            _cabi.check(lib.sbl_norm_rotary_workspace_bytes(ctypes.byref(p), ctypes.byref(n)))
+            nbytes = n.value
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev):
+            rc = lib.sbl_norm_rotary_backward(ctypes.byref(p), ws.data_ptr() if ws is not None else None, nbytes,
+                                              torch.cuda.current_stream(dev).cuda_stream)
+        _cabi.check(rc)
+        return (*dxs, *dws, *([None] * (2 + len(ctx.args))))
+
+
+def qk_norm_rotary(query, key, query_weight=None, key_weight=None, positions=None, key_positions=None, pos0=0,
+                   rotary_dim=None, theta=10000.0, interleaved=False, eps=1e-6):
+    """Root-mean-square norm of every query and key head, times a weight over the head dim, then the rotation of
+    its first `rotary_dim` entries by the row's position, in one kernel for both tensors; autograd differentiates it
+    in the inputs and the weights.
+
+    query (B,T,Hq,E), key (B,S,Hk,E), float32 or bfloat16, any strides over the first three axes; weights (E,)
+    float32 or bfloat16, or None for ones.  positions: int64 (T,) or (B,T), negative ones too; key_positions the
+    same over S, by default `positions` (which then has to fit both).  Without positions row t has position
+    pos0 + t.  rotary_dim: even, by default all of an even E; pair i turns by position * theta^(-2i / rotary_dim); pairs are
+    (i, i + rotary_dim / 2), or (2i, 2i + 1) with `interleaved`.  Returns new contiguous (query, key)."""
+    if not (query.is_cuda and key.is_cuda):
+        raise ValueError('sblocal_b200 runs on CUDA tensors only (there is no CPU path)')
+    if query.dim() != 4 or key.dim() != 4 or query.shape[0] != key.shape[0] or query.shape[3] != key.shape[3]:
+        raise ValueError(f'query/key must be (B,T,Hq,E), (B,S,Hk,E): got {tuple(query.shape)}, {tuple(key.shape)}')
+    if query.dtype not in _DTYPES:
+        raise TypeError(f'dtype {query.dtype} is not supported (float32 and bfloat16 are)')
+    if key.dtype != query.dtype:
+        raise TypeError('query and key must share one dtype')
+    dev, E = query.device, query.shape[3]
+    if key.device != dev:
+        raise ValueError('query and key must be on one device')
+    if query.shape[2] == 0 or key.shape[2] == 0 or E == 0:
+        raise ValueError('query and key need at least one head and one entry')
+    for w in (query_weight, key_weight):
+        if w is not None and (w.shape != (E,) or w.device != dev):
+            raise ValueError(f'weights must have shape ({E},) on the device of the query')
+        if w is not None and w.dtype not in _DTYPES:
+            raise TypeError(f'weight dtype {w.dtype} is not supported (float32 and bfloat16 are)')
+    if query_weight is not None and key_weight is not None and query_weight.dtype != key_weight.dtype:
+        raise TypeError('the two weights must share one dtype')
+    if key_positions is None:
+        key_positions = positions
+    places = []
+    for pos, x, name in ((positions, query, 'positions'), (key_positions, key, 'key_positions')):
+        if pos is not None:
+            if tuple(pos.shape) not in ((x.shape[1],), (x.shape[0], x.shape[1])):
+                raise ValueError(f'{name} must be ({x.shape[1]},) or ({x.shape[0]}, {x.shape[1]}), got '
+                                 f'{tuple(pos.shape)}')
+            if pos.dtype != torch.int64 or pos.device != dev:
+                raise ValueError(f'{name} must be int64 on the device of the query')
+        places.append(pos)
+    rotary_dim = E - E % 2 if rotary_dim is None else int(rotary_dim)
+    if rotary_dim < 0 or rotary_dim > E or rotary_dim % 2:
+        raise ValueError(f'rotary_dim must be even and in 0..{E}, got {rotary_dim}')
+    query = query if query.stride(-1) == 1 else query.contiguous()
+    key = key if key.stride(-1) == 1 else key.contiguous()
+    query_weight, key_weight = (w if w is None or w.is_contiguous() else w.contiguous()
+                                for w in (query_weight, key_weight))
+    args = (int(pos0), rotary_dim, float(theta), bool(interleaved), float(eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (query, key, query_weight, key_weight)):
+        return _NormRotary.apply(query, key, query_weight, key_weight, *places, *args)
+    return _norm_rotary_forward((query, key), (query_weight, key_weight), places, *args)

@@ -4,27 +4,18 @@ attention plus a Performer low-rank estimate outside the band, jointly
 normalised.  Same constructor and `forward` signature; the forward runs as
 hand-written sm_100a CUDA kernels behind the C ABI of include/sblocal_b200.h.
 
-Forward only.  There is no CPU path: CPU tensors raise.  Not built (raise
-NotImplementedError): causal=True (the reference marks it unchecked, :61),
-an attn_mask that masks anything (the reference's own assert at :106 rejects
-it), dropout in training mode.
+Differentiable in query, key and value (softmax_eps = 0): the backward pass
+recomputes the weights from two saved floats per row.  There is no CPU path:
+CPU tensors raise.  Not built (raise NotImplementedError): causal=True (the
+reference marks it unchecked, :61), an attn_mask that masks anything (the
+reference's own assert at :106 rejects it), dropout in training mode,
+gradients with softmax_eps != 0 or through need_weights.
 """
 import torch
 import torch.nn as nn
 
 from . import ops
 from .feature_maps_sb import SBPerformerFeatures
-
-
-class _ForwardOnly(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths):
-        return ops.sblocal_forward(query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths,
-                                   watch=True)
-
-    @staticmethod
-    def backward(ctx, *grads):
-        raise NotImplementedError('sblocal_b200 implements the forward pass only')
 
 
 class SBLocalAttention(nn.Module):
@@ -51,6 +42,8 @@ class SBLocalAttention(nn.Module):
         # (E = D = 64, 256 features, eps = 0) are rounded to bf16, run there, and the output is returned in fp32
         # (2e-2 of the reference, several times faster).  Set it on the module; the constructor is unchanged.
         self.compute_dtype = None
+        # Not in the reference.  A `QKNormRotary` (or any module with its call) set here runs on query and key first.
+        self.qk_norm = None
 
     def forward(self, query, key, value, attn_mask=None, key_padding_mask=None, need_weights=False,
                 return_attn_unnormalized=False):
@@ -69,6 +62,8 @@ class SBLocalAttention(nn.Module):
         key_lengths = None
         if key_padding_mask is not None and not bool(key_padding_mask.all_ones):
             key_lengths = key_padding_mask.lengths
+        if self.qk_norm is not None:
+            query, key = self.qk_norm(query, key)
         self.feature_map.new_feature_map(query.device)
         W = self.feature_map.projection_matrix
         out_dtype = None
@@ -86,10 +81,7 @@ class SBLocalAttention(nn.Module):
             out = prob.forward(workspace=ws)
             attn = prob.attention_weights(unnormalized=return_attn_unnormalized, workspace=ws)
             return out, attn
-        if torch.is_grad_enabled() and any(t.requires_grad for t in (query, key, value)):
-            out = _ForwardOnly.apply(*args)
-        else:
-            out = ops.sblocal_forward(*args, watch=True)
+        out = ops.sblocal_attention(*args, watch=True)
         if out_dtype is not None:
             out = out.to(out_dtype)
         return out, None

@@ -223,6 +223,87 @@ int sbl_key_features(const SblParams* p, void* workspace, size_t workspace_bytes
 int sbl_key_logscale_static(const SblParams* p, float* beta, void* cuda_stream);
 const char* sbl_static_last_error(void);
 
+/* ------------------------------------------------------------------ training */
+
+/*
+ * sbl_forward that also leaves what the gradients need: row_stats (2,B,H,T) fp32
+ * device, [0] a log-scale and [1] a positive normaliser per query row, so that
+ * row_stats[0] + ln(row_stats[1]) is the row's log_normalization
+ * (sblocal_attention.py:115): inside the window a key weighs
+ * exp(tau q.k - log_normalization).  `out` is the same as sbl_forward's.  Rows
+ * without any real key get an output of zero.  Sequence shards and
+ * softmax_eps != 0: SBL_ERR_UNSUPPORTED.
+ */
+int sbl_forward_train(const SblParams* p, void* workspace, size_t workspace_bytes, float* row_stats,
+                      void* cuda_stream);
+
+/*
+ * Gradients of sbl_forward_train.  Layouts as in SblParams: dout like out, dq
+ * like q, dk like k, dv like v, same dtype, last axis contiguous, element
+ * strides for the others (a stride of 0 is allowed in dout only).
+ */
+typedef struct SblGrads {
+  const void* dout; int64_t do_stride_b, do_stride_t, do_stride_h;
+  const float* row_stats;     /* (2,B,H,T) from sbl_forward_train                          */
+  void* dq; int64_t dq_stride_b, dq_stride_t, dq_stride_h;
+  void* dk; int64_t dk_stride_b, dk_stride_s, dk_stride_h;
+  void* dv; int64_t dv_stride_b, dv_stride_s, dv_stride_h;
+  int32_t reserved[4];        /* must be 0                                                 */
+} SblGrads;
+
+/* Bytes of workspace sbl_backward needs (256-byte aligned base); nothing of a forward's workspace is reused. */
+int sbl_backward_workspace_bytes(const SblParams* p, size_t* bytes);
+
+/*
+ * dq, dk, dv of sum(dout * out), with p->out holding the forward's output.  The
+ * weights are recomputed from q, k and row_stats; no (T,S) or (T,w) matrix is
+ * stored.  In the reference autograd differentiates sblocal_attention.py:77-122;
+ * there the stabilising maxima cancel, and so they do here (softmax_eps = 0).
+ * Padded keys and rows without a real key get zeros.  Deterministic.
+ */
+int sbl_backward(const SblParams* p, const SblGrads* g, void* workspace, size_t workspace_bytes, void* cuda_stream);
+
+/*
+ * Norm and rotation of query and key heads in one pass.  For every head row x of
+ * E entries:  z = x / sqrt(mean(x^2) + eps) * weight, then the pairs (2i, 2i+1)
+ * (interleaved) or (i, i + rotary/2) of the first `rotary` entries are turned by
+ * position * theta^(-2i/rotary); the entries behind them stay.  side[0] is the
+ * query, side[1] the key; they may differ in length and heads.  Angles are
+ * reduced in fp64, so far positions keep their accuracy; sums are fp32.  y must
+ * not overlap x or dy.  No counterpart in the reference.
+ */
+typedef struct SblNormRotarySide {
+  int32_t T, H;               /* rows and heads; a side without rows may have null pointers */
+  const void* x; int64_t x_stride_b, x_stride_t, x_stride_h;   /* (B,T,H,E) input            */
+  void* y; int64_t y_stride_b, y_stride_t, y_stride_h;         /* forward: output; backward: dx */
+  const void* dy; int64_t dy_stride_b, dy_stride_t, dy_stride_h; /* backward only            */
+  const void* weight;         /* (E) in weight_dtype, or null = all ones                   */
+  void* dweight;              /* backward: (E) in weight_dtype, or null                    */
+  const int64_t* positions;   /* device int64, or null: row t has position pos0 + t        */
+  int64_t pos_stride_b, pos_stride_t;
+  int64_t pos0;
+} SblNormRotarySide;
+
+typedef struct SblNormRotary {
+  int32_t dtype, weight_dtype;  /* SblDType of x, y, dy and of the weights                 */
+  int32_t B, E;                 /* E <= SBL_NORM_ROTARY_MAX_E                              */
+  int32_t rotary;               /* even, 0..E                                              */
+  int32_t interleaved;          /* 1: neighbours are a pair, 0: halves                     */
+  double eps, theta;
+  SblNormRotarySide side[2];
+  int32_t reserved[4];          /* must be 0                                               */
+} SblNormRotary;
+
+#define SBL_NORM_ROTARY_MAX_E 512
+
+int sbl_norm_rotary_forward(const SblNormRotary* p, void* cuda_stream);
+
+/* Workspace (16-byte aligned) of the backward pass: the blocks' partial weight gradients. */
+int sbl_norm_rotary_workspace_bytes(const SblNormRotary* p, size_t* bytes);
+
+/* y <- dx and dweight (fixed order of summation) from x and dy; the norms are recomputed. */
+int sbl_norm_rotary_backward(const SblNormRotary* p, void* workspace, size_t workspace_bytes, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif
