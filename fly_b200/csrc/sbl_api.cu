@@ -66,6 +66,8 @@ int validate(const SblParams* p) {
   return SBL_OK;
 }
 
+bool tensor_path(const SblParams& p) { return tc_supported(p) && !(p.flags & SBL_FLAG_GENERIC_PATH); }
+
 int check_workspace(const Workspace& ws, void* workspace, size_t bytes) {
   if (!workspace) return fail(SBL_ERR_WORKSPACE, "workspace is null (need %zu bytes)", ws.total);
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0)
@@ -292,9 +294,15 @@ int sbl_backward_workspace_bytes(const SblParams* p, size_t* bytes) {
   if (!bytes) return fail(SBL_ERR_INVALID_ARGUMENT, "bytes is null");
   int rc = validate_training(p);
   if (rc != SBL_OK) return rc;
-  BwdWorkspace ws;
-  f32_plan_backward(*p, &ws);
-  *bytes = ws.total;
+  if (tensor_path(*p)) {
+    TcBwdWorkspace ws;
+    tc_plan_backward(*p, &ws);
+    *bytes = ws.fwd.total;
+  } else {
+    BwdWorkspace ws;
+    f32_plan_backward(*p, &ws);
+    *bytes = ws.total;
+  }
   return SBL_OK;
 }
 
@@ -307,6 +315,16 @@ int sbl_backward(const SblParams* p, const SblGrads* g, void* workspace, size_t 
   for (int r : g->reserved)
     if (r != 0) return fail(SBL_ERR_INVALID_ARGUMENT, "reserved fields must be 0");
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+  if (tensor_path(*p)) {
+    if (const char* name = tc_backward_strides(*g, *p))
+      return fail(SBL_ERR_INVALID_ARGUMENT, "%s must be 16-byte aligned with positive strides that are multiples of 8 "
+                  "(or set SBL_FLAG_GENERIC_PATH)", name);
+    TcBwdWorkspace ws;
+    tc_plan_backward(*p, &ws);
+    if ((rc = check_workspace(ws.fwd, workspace, workspace_bytes)) != SBL_OK) return rc;
+    cudaError_t e = tc_backward(*p, *g, ws, static_cast<char*>(workspace), st);
+    return e == cudaSuccess ? SBL_OK : cuda_fail(e, "backward");
+  }
   BwdWorkspace ws;
   f32_plan_backward(*p, &ws);
   if ((rc = check_workspace(ws.fwd, workspace, workspace_bytes)) != SBL_OK) return rc;

@@ -86,8 +86,9 @@ cudaError_t norm_rotary(const SblNormRotary& p, bool backward, float* partial, c
 bool tc_supported(const SblParams& p);
 // reset_status: clear the device status words (first stage of a call sequence)
 // beta_fill: when given, the B*H key log-scales there are reset to -inf by the same launch
+// wt_lo: when given, receives what the bf16 rounding of the projection leaves, in bf16
 cudaError_t tc_prepare_projection(const SblParams& p, const Workspace& ws, char* base, cudaStream_t st,
-                                  bool reset_status, float* beta_fill = nullptr);
+                                  bool reset_status, float* beta_fill = nullptr, __nv_bfloat16* wt_lo = nullptr);
 cudaError_t tc_key_logscale(const SblParams& p, const Workspace& ws, char* base, float* beta, cudaStream_t st);
 // one-pass upper bound on the key log-scale (valid stabiliser when eps = 0); used by the fused forward
 cudaError_t tc_key_logscale_bound(const SblParams& p, const Workspace& ws, char* base, float* beta, cudaStream_t st,
@@ -98,6 +99,22 @@ cudaError_t tc_key_summary(const SblParams& p, const Workspace& ws, char* base, 
 cudaError_t tc_band(const SblParams& p, const Workspace& ws, char* base, const float* beta,
                     const float* kv, const float* ksum, cudaStream_t st, bool kv16_ready = false,
                     float* row_stats = nullptr);
+// ---- gradients on the tensor cores (same shapes), sbl_tc_bwd.cu ----
+// [0]: queries, [1]: keys.  `fwd` is the view the projection and log-scale kernels of the forward take.
+struct TcBwdWorkspace {
+  Workspace fwd;            // status (offset 0), wt, phiq = Wt in bf16, beta; total
+  size_t wlo;               // what is left of Wt, in bf16
+  size_t n2, delta;         // (BH,Tp)
+  size_t feat[2];           // psi (BH,T,m), phi (BH,S,m) bf16
+  size_t sum[2], sum1[2];   // (BH,m,D) bf16, (BH,m) fp32
+  size_t partial;           // split partials of one side's summary
+  size_t part;              // (BH,max(T,S),D) fp32: exact part of dq or dk
+  int Tp, nsplit[2];
+};
+void tc_plan_backward(const SblParams& p, TcBwdWorkspace* ws);
+// name of the first gradient tensor whose alignment or strides these kernels cannot take, or null
+const char* tc_backward_strides(const SblGrads& g, const SblParams& p);
+cudaError_t tc_backward(const SblParams& p, const SblGrads& g, const TcBwdWorkspace& ws, char* base, cudaStream_t st);
 // runs a kernel whose only wait can never be satisfied; *host_status receives the recorded wait site (99)
 cudaError_t tc_wait_selftest(int* device_status, int* host_status, cudaStream_t st);
 // copies the three device status words (host_status[0]: wait site that ran out, host_status[1]: 1 if an

@@ -157,7 +157,7 @@ constexpr int kPartialLd = 80;   // row pitch (floats) of a split-partial summar
 // norm of the bf16 copy (bound on |u_f| / |x| used as the query feature stabiliser), status reset.
 __global__ void __launch_bounds__(1024) tc_prep_kernel(const float* W, float c, float* wt32, __nv_bfloat16* wt16,
                                                        int r, int E, int* status, float* wmax, int reset_status,
-                                                       float* beta_fill, int n_beta) {
+                                                       float* beta_fill, int n_beta, __nv_bfloat16* wt_lo) {
   __shared__ float red[32];
   // the fused forward lets this launch also reset the key log-scales (they are formed by atomic max)
   for (int i = threadIdx.x; i < n_beta; i += blockDim.x) beta_fill[i] = -INFINITY;
@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(1024) tc_prep_kernel(const float* W, float c, 
         wt32[f * E + e] = v;
         wt16[f * E + e] = b;
         const float vb = __bfloat162float(b);
+        if (wt_lo) wt_lo[f * E + e] = __float2bfloat16_rn(v - vb);
         s = fmaf(vb, vb, s);
       }
     s += __shfl_xor_sync(0xffffffffu, s, 1);
@@ -1506,10 +1507,10 @@ bool tc_supported(const SblParams& p) {
 }
 
 cudaError_t tc_prepare_projection(const SblParams& p, const Workspace& ws, char* base, cudaStream_t st,
-                                  bool reset_status, float* beta_fill) {
+                                  bool reset_status, float* beta_fill, __nv_bfloat16* wt_lo) {
   const TcLayout l = tc_layout(ws, base);
   tc_prep_kernel<<<1, 1024, 0, st>>>(p.W, (float)sqrt((double)p.softmax_temp), l.wt32, l.wt16, p.r, p.E, l.status,
-                                    l.wmax, reset_status ? 1 : 0, beta_fill, beta_fill ? p.B * p.H : 0);
+                                    l.wmax, reset_status ? 1 : 0, beta_fill, beta_fill ? p.B * p.H : 0, wt_lo);
   return cudaGetLastError();
 }
 

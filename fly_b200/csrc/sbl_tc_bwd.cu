@@ -1,0 +1,1636 @@
+// bf16 tensor-core path of the SBLocal gradients for sm_100a: E = D = 64,
+// r = 128 (m = 256) and E = D = 128, r = 256 (m = 512), eps = 0, any T, S, w and
+// key lengths.  The formulas are those at the top of sbl_bwd_f32.cu.
+//
+// Kernels (rows = the side a CTA's 128-row tiles belong to, columns = the other)
+//   rows      delta = dout . out and the log-normaliser (base 2) of every query
+//   feat      per (split, block of 128 features, b*h): U = X Wt^T, the features
+//             phi (keys) or psi (queries, over the row's normaliser) -> bf16 to the
+//             workspace, and the summary phi^T [V | 1] or psi^T [dout | delta]
+//   combine   sums the splits -> summary in bf16, its extra column in fp32
+//   window    exact part of dq or dk: S = X X'^T, G = Y Y'^T, p (G - delta) -> bf16,
+//             dx += (p g) X', over the 64-column steps of the window -> fp32
+//   dvalue    S = K Q^T -> p, minus phi psi^T (same buffer, A operand negated),
+//             packed, dv += (p - a) dout; dv += phi QG
+//   lowrank   G = Y Y'^T - delta -> bf16, df -= G f' over the window (256 features at
+//             a time in tensor memory), df += Y summary^T; du = (f df)_+ - (f df)_-,
+//             dx += du Wt; adds the exact part, writes dq or dk
+//
+// Numerics.  Products take bf16 operands and accumulate in fp32.  Rounded to bf16
+// (half a step, 2^-9 on average): features, summaries, g, p g, p - a, du.  The
+// projection is carried as two bf16 terms (16 bits of mantissa): rounded to one,
+// it alone was half of the error of dq and dk (U enters an exponential, and the
+// same rounding comes back with du Wt).
+//
+// Where a tile's columns are few (`complement`), df is summed over the columns
+// OUTSIDE the window directly instead of all - inside: a short sequence lies
+// inside its windows almost entirely, and the difference of two sums of bf16
+// products would leave their rounding where the exact value is next to nothing.
+//
+// Feature order: block of 128 = "+" features of 64 projections, then their "-".
+// All waits are bounded (mbar_wait): a wait that runs out sets the first word of
+// the workspace and the kernel runs to its end.
+#include "sbl_common.cuh"
+#include "sbl_tc_dev.cuh"
+#include "sbl_tc_host.cuh"
+
+namespace sbl {
+namespace {
+
+using namespace ptx;
+using namespace tcdev;
+using namespace tch;
+
+enum { QUERIES = 0, KEYS = 1 };
+constexpr int TR = 128;        // rows of a tile
+
+struct Geom {
+  const int64_t* lengths;
+  int H, T, S, w, ntr, ntiles;   // ntr: row tiles per (b,h)
+};
+struct RowTile {
+  int bh, b, h, r0, nr, len, c0, n;   // n column steps from c0 on
+};
+
+// The column steps of width STEP (a power of two) that a row tile meets; all real columns with `whole`.
+template <int SIDE, int STEP>
+__device__ __noinline__ RowTile row_tile(const Geom& g, int tile, bool whole) {
+  RowTile t;
+  t.bh = tile / g.ntr;
+  t.r0 = (tile - t.bh * g.ntr) * TR;
+  t.b = t.bh / g.H;
+  t.h = t.bh - t.b * g.H;
+  t.len = g.S;
+  if (g.lengths) {
+    const int64_t l = g.lengths[t.b];
+    t.len = l < 0 ? 0 : (l < g.S ? (int)l : g.S);
+  }
+  const int hw = g.w / 2;
+  int lo, hi;
+  if (SIDE == QUERIES) {
+    t.nr = min(TR, g.T - t.r0);
+    lo = t.r0 - hw;
+    hi = t.r0 + t.nr - 1 - hw + g.w - 1;
+    if (whole) { lo = 0; hi = t.len; }
+    hi = min(hi, t.len - 1);
+  } else {
+    t.nr = min(TR, g.S - t.r0);
+    lo = t.r0 + hw - g.w + 1;
+    hi = t.r0 + t.nr - 1 + hw;
+    if (whole) { lo = 0; hi = g.T; }
+    hi = t.r0 < t.len ? min(hi, g.T - 1) : -1;
+  }
+  lo = max(lo, 0);
+  t.c0 = lo & ~(STEP - 1);
+  t.n = hi >= lo ? (hi - t.c0) / STEP + 1 : 0;
+  return t;
+}
+
+__device__ __forceinline__ uint32_t bits(int lo, int hi) {   // bits lo..hi of a word, clipped
+  lo = max(lo, 0);
+  hi = min(hi, 31);
+  return hi >= lo ? (0xFFFFFFFFu >> (31 - (hi - lo))) << lo : 0u;
+}
+// Which of the 32 columns from c on row `row` has in its window; with `whole`, the real ones outside it.
+template <int SIDE>
+__device__ __forceinline__ uint32_t seen(const Geom& g, const RowTile& t, int row, int c, bool whole) {
+  const int hw = g.w / 2;
+  if (SIDE == QUERIES) {
+    const uint32_t real = bits(0, t.len - 1 - c);
+    const uint32_t in = bits(row - hw - c, row - hw + g.w - 1 - c) & real;
+    return whole ? real & ~in : in;
+  }
+  const uint32_t real = row < t.len ? bits(0, g.T - 1 - c) : 0u;
+  const uint32_t in = bits(row + hw - g.w + 1 - c, row + hw - c) & real;
+  return whole ? real & ~in : in;
+}
+
+__device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
+  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~(uintptr_t)1023);
+}
+// start-address steps (in 16-byte units) of K step k inside a K-major operand of [rows][64] pieces
+__device__ __forceinline__ uint64_t kmajor(int k, uint32_t piece_bytes) {
+  return (uint64_t)((uint32_t)(k >> 2) * (piece_bytes >> 4) + (uint32_t)(k & 3) * 2);
+}
+// tensor-memory column of K step k of a packed operand that lies over the first half of every 32 columns
+__device__ __forceinline__ uint32_t packed(int k) { return 32u * (uint32_t)(k >> 1) + 8u * (uint32_t)(k & 1); }
+
+// ---------------------------------------------------------------------------
+// Per query row: n2 = log-normaliser * log2(e), delta = dout . out; both (BH, Tp), zero in the padding rows.
+template <int D>
+__global__ void __launch_bounds__(256) bwd_rows_kernel(const __nv_bfloat16* out, int64_t ob, int64_t ot, int64_t oh,
+                                                       const __nv_bfloat16* dout, int64_t db, int64_t dt, int64_t dh,
+                                                       const float* stats, int B, int H, int T, int Tp, float* n2,
+                                                       float* delta) {
+  constexpr int LPR = D / 8;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;   // (b, t, h), heads innermost
+  const int sub = threadIdx.x % LPR;
+  const int h = (int)(i % H), t = (int)((i / H) % Tp), b = (int)(i / ((int64_t)H * Tp));
+  float s = 0.f;
+  if (b < B && t < T) {
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(out + b * ob + t * ot + h * oh) + sub);
+    const uint4 y = __ldg(reinterpret_cast<const uint4*>(dout + b * db + t * dt + h * dh) + sub);
+    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s = fmaf(bf16_lo(xw[j]), bf16_lo(yw[j]), s);
+      s = fmaf(bf16_hi(xw[j]), bf16_hi(yw[j]), s);
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (b < B && sub == 0) {
+    const int64_t bh = (int64_t)b * H + h, rows = (int64_t)B * H * T;
+    float n = 0.f;
+    if (t < T) n = stats[bh * T + t] * kLog2e + log2f(stats[rows + bh * T + t]);
+    n2[bh * Tp + t] = n;
+    delta[bh * Tp + t] = s;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Features and summary of one side.
+struct FeatArgs {
+  CUtensorMap tm_x, tm_y, tm_hi, tm_lo, tm_f;
+  const int64_t* lengths;
+  const float *beta, *n2, *delta;   // (BH); (BH, Tp)
+  float* partial;                   // (BH, nsplit, m, D + 4)
+  int* status;
+  int H, rows, Tp, nsplit;
+  float tau, half_log_m;
+};
+
+template <int D>
+struct FeatCfg {
+  static constexpr int NB = D / 64, M = 4 * D, XD = D == 64 ? 2 : 1;
+  static constexpr uint32_t WB = NB * 8192;              // one bf16 term of 64 projections
+  static constexpr uint32_t XB = NB * 16384, YB = (NB + 1) * 16384;
+  static constexpr uint32_t OFF_W = 0, OFF_X = 2 * WB, OFF_Y = OFF_X + XD * XB, OFF_A = OFF_Y + 2 * YB;
+  static constexpr uint32_t OFF_BAR = OFF_A + 2 * 32768;
+  static constexpr uint32_t SMEM = OFF_BAR + 256 + 1024;
+  static constexpr int NFEAT = 256, NTHR = NFEAT + 64;
+  static constexpr uint32_t T_U = 0, T_SUM = 128;        // 2 x 64 | D + 16
+  static_assert(SMEM <= 232448, "dynamic shared memory of one CTA");
+};
+
+template <int SIDE, int D>
+__global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant__ FeatArgs a) {
+  using C = FeatCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t *bar_w = bars, *bar_done = bars + 1, *x_full = bars + 2, *x_free = bars + 4, *y_full = bars + 6,
+           *y_free = bars + 8, *u_full = bars + 10, *u_free = bars + 12, *a_full = bars + 14, *a_free = bars + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int fb = blockIdx.x % (C::M / 128), split = blockIdx.x / (C::M / 128);
+  const int bh = blockIdx.y, b = bh / a.H, h = bh % a.H;
+  const int ntiles = (a.rows + TR - 1) / TR;
+  const int t_lo = (int)((int64_t)ntiles * split / a.nsplit), t_hi = (int)((int64_t)ntiles * (split + 1) / a.nsplit);
+  const int nt = t_hi - t_lo;
+
+  if (tid == 0) {
+    mbar_init(bar_w, 1);
+    mbar_init(bar_done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(x_full + i, 1);
+      mbar_init(x_free + i, 8);
+      mbar_init(y_full + i, 1);
+      mbar_init(y_free + i, 1);
+      mbar_init(u_full + i, 1);
+      mbar_init(u_free + i, 8);
+      mbar_init(a_full + i, 8);
+      mbar_init(a_free + i, 2);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  // the extra summary column's operand behind each Y slot: ones (keys), or delta per row, written with the features
+  for (int i = tid; i < 2 * 8192; i += C::NTHR)
+    reinterpret_cast<__nv_bfloat16*>(smem + C::OFF_Y + (i / 8192) * C::YB + C::NB * 16384)[i % 8192] =
+        __float2bfloat16(SIDE == KEYS ? 1.f : 0.f);
+  fence_async_smem();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  constexpr uint32_t tb = 0;   // the CTA owns all 512 tensor-memory columns of its SM
+  if (tid == 0 && *tmem_slot != 0) atomicCAS(a.status, 0, 241);
+
+  if (warp == 8) {
+    const bool leader = elect_one();
+    if (leader) {
+      mbar_expect_tx(bar_w, 2 * C::WB);
+      for (int j = 0; j < C::NB; ++j) {
+        tma_load_2d(smem + C::OFF_W + j * 8192, &a.tm_hi, bar_w, 64 * j, 64 * fb);
+        tma_load_2d(smem + C::OFF_W + C::WB + j * 8192, &a.tm_lo, bar_w, 64 * j, 64 * fb);
+      }
+    }
+    for (int i = 0; i < nt; ++i) {
+      const int r0 = (t_lo + i) * TR, xs = i % C::XD, s = i & 1;
+      if (i >= C::XD) mbar_wait(x_free + xs, ((i / C::XD) - 1) & 1, a.status, 201);
+      if (leader) {
+        mbar_expect_tx(x_full + xs, C::XB);
+        for (int j = 0; j < C::NB; ++j)
+          tma_load_4d(smem + C::OFF_X + xs * C::XB + j * 16384, &a.tm_x, x_full + xs, 64 * j, r0, h, b);
+      }
+      if (i >= 2) mbar_wait(y_free + s, ((i >> 1) - 1) & 1, a.status, 202);
+      if (leader) {
+        mbar_expect_tx(y_full + s, C::XB);
+        for (int j = 0; j < C::NB; ++j)
+          tma_load_4d(smem + C::OFF_Y + s * C::YB + j * 16384, &a.tm_y, y_full + s, 64 * j, r0, h, b);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    const bool leader = elect_one();
+    constexpr uint32_t id_u = idesc_bf16(128, 64, false, false);
+    constexpr uint32_t id_s = idesc_bf16(128, D + 16, true, true);
+    const uint64_t dW = smem_desc_sw128(smem_u32(smem + C::OFF_W), 16, 1024);
+    const uint64_t dX = smem_desc_sw128(smem_u32(smem + C::OFF_X), 16, 1024);
+    const uint64_t dY = smem_desc_sw128(smem_u32(smem + C::OFF_Y), 16384, 1024);
+    const uint64_t dA = smem_desc_sw128(smem_u32(smem + C::OFF_A), 16384, 1024);
+    auto summary = [&](int u) {
+      const int s = u & 1;
+      mbar_wait(a_full + s, (u >> 1) & 1, a.status, 203);
+      mbar_wait(y_full + s, (u >> 1) & 1, a.status, 204);
+      tc_fence_after_sync();
+      if (leader) {
+        tma_store_3d(&a.tm_f, smem + C::OFF_A + s * 32768, 128 * fb, (t_lo + u) * TR, bh);
+        tma_store_3d(&a.tm_f, smem + C::OFF_A + s * 32768 + 16384, 128 * fb + 64, (t_lo + u) * TR, bh);
+        tma_store_commit();
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          mma_ss(tb + C::T_SUM, dA + (uint64_t)(s * (32768 >> 4) + k * 128), dY + (uint64_t)(s * (C::YB >> 4) + k * 128),
+                 id_s, u > 0 || k > 0);
+        mma_commit(a_free + s);
+        mma_commit(y_free + s);
+        // the previous tile's bulk store has read its buffer once at most one group is pending
+        if (u >= 1) {
+          tma_store_wait_read1();
+          mbar_arrive(a_free + (s ^ 1));
+        }
+      }
+      __syncwarp();
+    };
+    mbar_wait(bar_w, 0, a.status, 205);
+    for (int i = 0; i < nt; ++i) {
+      const int s = i & 1, xs = i % C::XD;
+      mbar_wait(x_full + xs, (i / C::XD) & 1, a.status, 206);
+      if (i >= 2) mbar_wait(u_free + s, ((i >> 1) - 1) & 1, a.status, 207);
+      tc_fence_after_sync();
+      if (leader) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_ss(tb + C::T_U + 64 * s, dX + (uint64_t)(xs * (C::XB >> 4)) + kmajor(k, 16384),
+                   dW + (uint64_t)(t * (C::WB >> 4)) + kmajor(k, 8192), id_u, t > 0 || k > 0);
+        mma_commit(u_full + s);
+      }
+      __syncwarp();
+      if (i >= 1) summary(i - 1);
+    }
+    if (nt > 0) summary(nt - 1);
+    if (leader) {
+      mma_commit(bar_done);
+      tma_store_wait_all();
+    }
+    __syncwarp();
+  } else {
+    const int qd = warp & 3, cq = warp >> 2;
+    const int row = qd * 32 + lane;
+    const uint32_t lane_base = tb + ((uint32_t)(qd * 32) << 16);
+    const float beta = a.beta[bh];
+    int len = a.rows;
+    if (SIDE == KEYS && a.lengths) {
+      const int64_t l = a.lengths[b];
+      len = l < 0 ? 0 : (l < a.rows ? (int)l : a.rows);
+    }
+    for (int i = 0; i < nt; ++i) {
+      const int s = i & 1, xs = i % C::XD;
+      const int r = (t_lo + i) * TR + row;
+      mbar_wait(x_full + xs, (i / C::XD) & 1, a.status, 208);
+      float sq = 0.f;
+#pragma unroll
+      for (int j = 0; j < C::NB; ++j) sq += row_sumsq_sw128(smem + C::OFF_X + xs * C::XB + j * 16384, row);
+      const float g = 0.5f * a.tau * sq;
+      const bool live = r < len;
+      float off, dl = 0.f;
+      if (SIDE == KEYS) {
+        off = (-g - a.half_log_m - beta) * kLog2e;
+      } else {
+        // r < Tp: the row arrays are padded to whole tiles
+        off = (-g - a.half_log_m + beta) * kLog2e - __ldg(a.n2 + (int64_t)bh * a.Tp + r);
+        dl = __ldg(a.delta + (int64_t)bh * a.Tp + r);
+      }
+      mbar_wait(u_full + s, (i >> 1) & 1, a.status, 209);   // U computed: the X tile has been read too
+      tc_fence_after_sync();
+      warp_arrive(x_free + xs, lane);
+      uint32_t u[32];
+      tmem_ld32(lane_base + C::T_U + 64 * s + 32 * cq, u);
+      tmem_ld_wait();
+      tc_fence_before_sync();
+      warp_arrive(u_free + s, lane);
+      uint32_t p1[16], p2[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float x = __uint_as_float(u[2 * j]), y = __uint_as_float(u[2 * j + 1]);
+        const uint32_t e = pack_bf16(ex2(fmaf(x, kLog2e, off)), ex2(fmaf(y, kLog2e, off)));
+        const uint32_t f = pack_bf16(ex2(fmaf(x, -kLog2e, off)), ex2(fmaf(y, -kLog2e, off)));
+        p1[j] = live ? e : 0u;
+        p2[j] = live ? f : 0u;
+      }
+      // the MMAs and the bulk store two tiles back are done with this buffer (and with the Y slot's extra column)
+      if (i >= 2) mbar_wait(a_free + s, ((i >> 1) - 1) & 1, a.status, 210);
+      uint8_t* line = smem + C::OFF_A + s * 32768 + row * 128;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t at = (uint32_t)(((4 * cq + c) ^ (row & 7)) << 4);
+        *reinterpret_cast<uint4*>(line + at) = make_uint4(p1[4 * c], p1[4 * c + 1], p1[4 * c + 2], p1[4 * c + 3]);
+        *reinterpret_cast<uint4*>(line + 16384 + at) = make_uint4(p2[4 * c], p2[4 * c + 1], p2[4 * c + 2], p2[4 * c + 3]);
+      }
+      if (SIDE == QUERIES) {
+        // delta in two bf16 terms: columns 0, 2, .. the high one, 1, 3, .. the low one
+        const float hi = __bfloat162float(__float2bfloat16_rn(dl));
+        const uint32_t w = pack_bf16(hi, dl - hi);
+        *reinterpret_cast<uint4*>(smem + C::OFF_Y + s * C::YB + C::NB * 16384 + row * 128 + ((cq ^ (row & 7)) << 4)) =
+            make_uint4(w, w, w, w);
+      }
+      fence_async_smem();
+      warp_arrive(a_full + s, lane);
+    }
+    mbar_wait(bar_done, 0, a.status, 211);
+    tc_fence_after_sync();
+    float* prow = a.partial + (((int64_t)bh * a.nsplit + split) * C::M + 128 * fb + row) * (D + 4);
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      uint32_t r[16];
+      const int c = (D / 2) * cq + 16 * j;
+      tmem_ld16(lane_base + C::T_SUM + c, r);
+      tmem_ld_wait();
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<uint4*>(prow + c + 4 * q) = nt ? make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3])
+                                                         : make_uint4(0, 0, 0, 0);
+    }
+    uint32_t r[16];
+    tmem_ld16(lane_base + C::T_SUM + D, r);
+    tmem_ld_wait();
+    if (cq == 0) prow[D] = nt == 0 ? 0.f : __uint_as_float(r[0]) + (SIDE == QUERIES ? __uint_as_float(r[1]) : 0.f);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 8) {
+    __syncwarp();
+    tmem_dealloc(tb, 512);
+  }
+}
+
+// summary (BH, m, D) bf16 and its extra column (BH, m) fp32 = sums over the splits
+template <int D>
+__global__ void __launch_bounds__(256) bwd_combine_kernel(const float* partial, int nsplit, int64_t rows, int m,
+                                                          __nv_bfloat16* sum, float* sum1) {
+  constexpr int G = D / 4 + 1;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * G) return;
+  const int64_t row = i / G, bh = row / m;
+  const int g = (int)(i % G);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < nsplit; ++k) {
+    const float* p = partial + ((bh * nsplit + k) * m + row % m) * (D + 4) + 4 * g;
+    if (g < D / 4) {
+      const float4 x = *reinterpret_cast<const float4*>(p);
+      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+    } else {
+      v.x += *p;
+    }
+  }
+  if (g < D / 4) *reinterpret_cast<uint2*>(sum + row * D + 4 * g) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+  else sum1[row] = v.x;
+}
+
+// ---------------------------------------------------------------------------
+// Exact part of dq or dk.
+struct WinArgs {
+  CUtensorMap tm_x, tm_y, tm_xo, tm_yo;   // own side (128 rows), other side (64 rows)
+  Geom g;
+  const float *n2, *delta;                // (BH, Tp)
+  float* part;                            // (BH, rows, D)
+  int* status;
+  int Tp;
+  float tau;
+};
+
+template <int D>
+struct WinCfg {
+  static constexpr int NB = D / 64, NS = D == 64 ? 6 : 3;
+  static constexpr uint32_t TB = NB * 16384, SLOT = 2 * NB * 8192;
+  static constexpr uint32_t OFF_X = 0, OFF_Y = 2 * TB, OFF_RING = 4 * TB, OFF_BAR = OFF_RING + NS * SLOT;
+  static constexpr uint32_t SMEM = OFF_BAR + 512 + 1024;
+  static constexpr int NTHR = 576, W_LOAD = 16, W_MMA = 17;
+  static constexpr uint32_t T_DX = 256;   // buffers: S at 128 b, G at 128 b + 64; dx at 256 + D b
+  enum { XY_FULL = 0, XY_FREE = 2, R_FULL = 4, R_FREE = R_FULL + NS, ST_FULL = R_FREE + NS, DS_DONE = ST_FULL + 2,
+         DX_FULL = DS_DONE + 2, DX_FREE = DX_FULL + 2, COUNT = DX_FREE + 2 };
+  static_assert(SMEM <= 232448 && COUNT <= 60, "shared memory of one CTA");
+};
+
+template <int SIDE, int D>
+__global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constant__ WinArgs a) {
+  using C = WinCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::COUNT);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  if (tid == 0) {
+    for (int i = 0; i < C::COUNT; ++i)
+      mbar_init(bars + i, i >= C::DX_FREE ? 16 : (i >= C::DS_DONE && i < C::DX_FULL ? 8 : 1));
+    fence_mbar_init();
+  }
+  if (warp == C::W_LOAD) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  constexpr uint32_t tb = 0;
+  if (tid == 0 && *tmem_slot != 0) atomicCAS(a.status, 0, 241);
+  const int step = gridDim.x;
+
+  if (warp == C::W_LOAD) {
+    const bool leader = elect_one();
+    int n = 0, ne = 0;
+    for (int tile = blockIdx.x; tile < a.g.ntiles; tile += step) {
+      const RowTile t = row_tile<SIDE, 64>(a.g, tile, false);
+      if (t.n == 0) continue;
+      const int buf = ne & 1;
+      if (ne >= 2) mbar_wait(bars + C::XY_FREE + buf, ((ne >> 1) - 1) & 1, a.status, 221);
+      if (leader) {
+        mbar_expect_tx(bars + C::XY_FULL + buf, 2 * C::TB);
+        for (int j = 0; j < C::NB; ++j) {
+          tma_load_4d(smem + C::OFF_X + buf * C::TB + j * 16384, &a.tm_x, bars + C::XY_FULL + buf, 64 * j, t.r0, t.h, t.b);
+          tma_load_4d(smem + C::OFF_Y + buf * C::TB + j * 16384, &a.tm_y, bars + C::XY_FULL + buf, 64 * j, t.r0, t.h, t.b);
+        }
+      }
+      ++ne;
+      for (int s = 0; s < t.n; ++s, ++n) {
+        const int slot = n % C::NS;
+        if (n >= C::NS) mbar_wait(bars + C::R_FREE + slot, ((n / C::NS) - 1) & 1, a.status, 222);
+        if (leader) {
+          uint8_t* dst = smem + C::OFF_RING + slot * C::SLOT;
+          mbar_expect_tx(bars + C::R_FULL + slot, C::SLOT);
+          for (int j = 0; j < C::NB; ++j) {
+            tma_load_4d(dst + j * 8192, &a.tm_xo, bars + C::R_FULL + slot, 64 * j, t.c0 + 64 * s, t.h, t.b);
+            tma_load_4d(dst + (C::NB + j) * 8192, &a.tm_yo, bars + C::R_FULL + slot, 64 * j, t.c0 + 64 * s, t.h, t.b);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == C::W_MMA) {
+    const bool leader = elect_one();
+    constexpr uint32_t id_st = idesc_bf16(128, 64, false, false);
+    constexpr uint32_t id_dx = idesc_bf16(128, D, false, true);
+    const uint64_t dX = smem_desc_sw128(smem_u32(smem + C::OFF_X), 16, 1024);
+    const uint64_t dY = smem_desc_sw128(smem_u32(smem + C::OFF_Y), 16, 1024);
+    const uint64_t dR = smem_desc_sw128(smem_u32(smem + C::OFF_RING), 16, 1024);
+    const uint64_t dRt = smem_desc_sw128(smem_u32(smem + C::OFF_RING), 8192, 1024);
+    // Two cursors over the same stream of steps: `st` runs two steps ahead of `dx`.
+    struct Cursor {
+      int tile, s, n, ne;
+    };
+    auto seek = [&](Cursor& c) {   // to the first step of the next tile that has one
+      while (c.tile < a.g.ntiles && (c.n = row_tile<SIDE, 64>(a.g, c.tile, false).n) == 0) c.tile += step;
+      c.s = 0;
+      ++c.ne;
+    };
+    auto next = [&](Cursor& c) {
+      if (++c.s == c.n) {
+        c.tile += step;
+        seek(c);
+      }
+    };
+    Cursor st{(int)blockIdx.x, 0, 0, -1};
+    seek(st);
+    Cursor dx = st;
+    int gs = 0;
+    auto issue_st = [&]() {
+      if (st.tile >= a.g.ntiles) return;
+      const int buf = gs & 1, xb = st.ne & 1, slot = gs % C::NS;
+      if (st.s == 0) mbar_wait(bars + C::XY_FULL + xb, (st.ne >> 1) & 1, a.status, 223);
+      mbar_wait(bars + C::R_FULL + slot, (gs / C::NS) & 1, a.status, 224);
+      tc_fence_after_sync();
+      if (leader) {
+        const uint64_t x = dX + (uint64_t)(xb * (C::TB >> 4)), y = dY + (uint64_t)(xb * (C::TB >> 4));
+        const uint64_t o = dR + (uint64_t)(slot * (C::SLOT >> 4));
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_ss(tb + 128 * buf, x + kmajor(k, 16384), o + kmajor(k, 8192), id_st, k > 0);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_ss(tb + 128 * buf + 64, y + kmajor(k, 16384), o + (uint64_t)(C::NB * (8192 >> 4)) + kmajor(k, 8192), id_st,
+                 k > 0);
+        mma_commit(bars + C::ST_FULL + buf);
+        if (st.s == st.n - 1) mma_commit(bars + C::XY_FREE + xb);
+      }
+      __syncwarp();
+      ++gs;
+      next(st);
+    };
+    issue_st();
+    issue_st();
+    for (int g = 0; dx.tile < a.g.ntiles; ++g, next(dx)) {
+      const int buf = g & 1, db = dx.ne & 1, slot = g % C::NS;
+      mbar_wait(bars + C::DS_DONE + buf, (g >> 1) & 1, a.status, 225);
+      if (dx.s == 0 && dx.ne >= 2) mbar_wait(bars + C::DX_FREE + db, ((dx.ne >> 1) - 1) & 1, a.status, 226);
+      tc_fence_after_sync();
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_ts(tb + C::T_DX + D * db, tb + 128 * buf + packed(k),
+                 dRt + (uint64_t)(slot * (C::SLOT >> 4) + k * 128), id_dx, dx.s > 0 || k > 0);
+        mma_commit(bars + C::R_FREE + slot);
+        if (dx.s == dx.n - 1) mma_commit(bars + C::DX_FULL + db);
+      }
+      __syncwarp();
+      issue_st();
+    }
+  } else {
+    // two groups of eight warps, one per buffer; a thread owns a row and 32 of the step's 64 columns
+    const int grp = warp >> 3, qd = warp & 3, cq = (warp >> 2) & 1;
+    const int row = qd * 32 + lane;
+    const uint32_t lane_base = tb + ((uint32_t)(qd * 32) << 16);
+    const float sc = a.tau * kLog2e;
+    int g = 0, ne = 0;
+    for (int tile = blockIdx.x; tile < a.g.ntiles; tile += step) {
+      const RowTile t = row_tile<SIDE, 64>(a.g, tile, false);
+      const int r = t.r0 + row;
+      const float* n2 = a.n2 + (int64_t)t.bh * a.Tp;
+      const float* dl = a.delta + (int64_t)t.bh * a.Tp;
+      float rn = 0.f, rd = 0.f;
+      if (SIDE == QUERIES) {
+        rn = __ldg(n2 + r);
+        rd = __ldg(dl + r);
+      }
+      for (int s = 0; s < t.n; ++s, ++g) {
+        if ((g & 1) != grp) continue;
+        const int c = t.c0 + 64 * s + 32 * cq;
+        const uint32_t vis = seen<SIDE>(a.g, t, r, c, false);
+        const uint32_t ts = lane_base + 128 * grp + 32 * cq;
+        uint32_t o[16];
+        mbar_wait(bars + C::ST_FULL + grp, (g >> 1) & 1, a.status, 227);
+        tc_fence_after_sync();
+        if (__any_sync(0xffffffffu, vis != 0u)) {
+          uint32_t x[32], y[32];
+          tmem_ld32(ts, x);
+          tmem_ld32(ts + 64, y);
+          tmem_ld_wait();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            float4 cn = make_float4(rn, rn, rn, rn), cd = make_float4(rd, rd, rd, rd);
+            if (SIDE == KEYS) {
+              // c < Tp: the row arrays are padded to whole tiles
+              cn = __ldg(reinterpret_cast<const float4*>(n2 + c) + q);
+              cd = __ldg(reinterpret_cast<const float4*>(dl + c) + q);
+            }
+            const float nn[4] = {cn.x, cn.y, cn.z, cn.w}, dd[4] = {cd.x, cd.y, cd.z, cd.w};
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float p = ex2(fmaf(__uint_as_float(x[4 * q + j]), sc, -nn[j]));
+              v[j] = keep_if_bit(p * (__uint_as_float(y[4 * q + j]) - dd[j]), vis, 4 * q + j);
+            }
+            o[2 * q] = pack_bf16(v[0], v[1]);
+            o[2 * q + 1] = pack_bf16(v[2], v[3]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = 0u;
+        }
+        tmem_st16(ts, o);
+        tmem_st_wait();
+        tc_fence_before_sync();
+        warp_arrive(bars + C::DS_DONE + grp, lane);
+      }
+      // this thread's quarter of the row's D sums
+      constexpr int NC = D / 4;
+      const int c = NC * (2 * grp + cq);
+      uint32_t v[32];
+      if (t.n > 0) {
+        const int db = ne & 1;
+        mbar_wait(bars + C::DX_FULL + db, (ne >> 1) & 1, a.status, 228);
+        tc_fence_after_sync();
+        if constexpr (NC == 32) {
+          tmem_ld32(lane_base + C::T_DX + D * db + c, v);
+        } else {
+          uint32_t w[16];
+          tmem_ld16(lane_base + C::T_DX + D * db + c, w);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = w[j];
+        }
+        tmem_ld_wait();
+        tc_fence_before_sync();
+        warp_arrive(bars + C::DX_FREE + db, lane);
+        ++ne;
+      } else {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) v[j] = 0u;
+      }
+      if (row < t.nr) {
+        const int rows = SIDE == QUERIES ? a.g.T : a.g.S;
+        float4* dst = reinterpret_cast<float4*>(a.part + ((int64_t)t.bh * rows + r) * D + c);
+#pragma unroll
+        for (int j = 0; j < NC / 4; ++j)
+          dst[j] = make_float4(a.tau * __uint_as_float(v[4 * j]), a.tau * __uint_as_float(v[4 * j + 1]),
+                               a.tau * __uint_as_float(v[4 * j + 2]), a.tau * __uint_as_float(v[4 * j + 3]));
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == C::W_LOAD) {
+    __syncwarp();
+    tmem_dealloc(tb, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Low-rank part of dq or dk, and the sum of both.
+struct LowArgs {
+  CUtensorMap tm_y, tm_yo, tm_fo, tm_sum, tm_hi, tm_lo;
+  Geom g;
+  const __nv_bfloat16* f;                  // own features (BH, rows, m)
+  const float* sum1;                       // (BH, m): extra column of the other side's summary
+  const float* delta;                      // (BH, Tp)
+  const float* part;                       // (BH, rows, D): exact part
+  const __nv_bfloat16* x; int64_t xb, xr, xh;
+  __nv_bfloat16* dx; int64_t ob, orow, oh;
+  int* status;
+  int Tp, whole;
+  float tau;
+};
+
+template <int D>
+struct LowCfg {
+  static constexpr int NB = D / 64, M = 4 * D, PASS = M / 256, NS = D == 64 ? 3 : 2;
+  static constexpr uint32_t TB = NB * 16384;             // own Y tile
+  static constexpr uint32_t AUX = 512 * D;               // 256 features x D of the summary; 2 terms x 128 x D of Wt
+  static constexpr uint32_t SLOT = 32768 + NB * 8192;    // 64 columns: 256 features, then Y'
+  static constexpr uint32_t OFF_Y = 0, OFF_SUM = 2 * TB;
+  static constexpr uint32_t OFF_W = D == 64 ? OFF_SUM + AUX : OFF_SUM;   // head dim 128: one buffer for both, in turn
+  static constexpr uint32_t OFF_RING = OFF_W + AUX, OFF_H = OFF_RING + NS * SLOT, OFF_BAR = OFF_H + 1024;
+  static constexpr uint32_t SMEM = OFF_BAR + 256 + 1024;
+  static constexpr int NTHR = 320, W_LOAD = 8, W_MMA = 9;
+  static constexpr uint32_t T_DF = 0, T_DX = 256, T_G = 384;   // 256 | D | 2 x 64
+  enum { Y_FULL = 0, Y_FREE = 2, R_FULL = 4, R_FREE = R_FULL + NS, SUM_FULL = R_FREE + NS, SUM_FREE, W_FULL, W_FREE,
+         T_FULL, G_DONE = T_FULL + 2, DF_FULL = G_DONE + 2, DU_DONE, DX_FULL, DX_FREE, COUNT };
+  static_assert(SMEM <= 232448 && COUNT <= 30, "shared memory of one CTA");
+};
+
+template <int SIDE, int D>
+__global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_constant__ LowArgs a) {
+  using C = LowCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::COUNT);
+  float* s_h = reinterpret_cast<float*>(smem + C::OFF_H);   // [2 column halves][128 rows]
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  if (tid == 0) {
+    for (int i = 0; i < C::COUNT; ++i)
+      mbar_init(bars + i, (i >= C::G_DONE && i < C::DF_FULL) || i == C::DU_DONE || i == C::DX_FREE ? 8 : 1);
+    fence_mbar_init();
+  }
+  if (warp == C::W_LOAD) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  constexpr uint32_t tb = 0;
+  if (tid == 0 && *tmem_slot != 0) atomicCAS(a.status, 0, 241);
+  const int step = gridDim.x;
+  const bool whole = a.whole != 0;
+  // number of tiles of this CTA; a unit is a (tile, pass of 256 features)
+  const int n_it = (a.g.ntiles - (int)blockIdx.x + step - 1) / step, n_u = n_it * C::PASS;
+
+  if (warp == C::W_LOAD) {
+    const bool leader = elect_one();
+    int n = 0;
+    for (int u = 0; u < n_u; ++u) {
+      const int it = u / C::PASS, pass = u % C::PASS;
+      const RowTile t = row_tile<SIDE, 64>(a.g, blockIdx.x + it * step, whole);
+      if (pass == 0) {
+        const int buf = it & 1;
+        if (it >= 2) mbar_wait(bars + C::Y_FREE + buf, ((it >> 1) - 1) & 1, a.status, 261);
+        if (leader) {
+          mbar_expect_tx(bars + C::Y_FULL + buf, C::TB);
+          for (int j = 0; j < C::NB; ++j)
+            tma_load_4d(smem + C::OFF_Y + buf * C::TB + j * 16384, &a.tm_y, bars + C::Y_FULL + buf, 64 * j, t.r0, t.h, t.b);
+        }
+      }
+      for (int s = 0; s < t.n; ++s, ++n) {
+        const int slot = n % C::NS;
+        if (n >= C::NS) mbar_wait(bars + C::R_FREE + slot, ((n / C::NS) - 1) & 1, a.status, 262);
+        if (leader) {
+          uint8_t* dst = smem + C::OFF_RING + slot * C::SLOT;
+          mbar_expect_tx(bars + C::R_FULL + slot, C::SLOT);
+          for (int j = 0; j < C::NB; ++j)
+            tma_load_4d(dst + 32768 + j * 8192, &a.tm_yo, bars + C::R_FULL + slot, 64 * j, t.c0 + 64 * s, t.h, t.b);
+          for (int j = 0; j < 4; ++j)
+            tma_load_3d(dst + j * 8192, &a.tm_fo, bars + C::R_FULL + slot, 256 * pass + 64 * j, t.c0 + 64 * s, t.bh);
+        }
+      }
+      // Head dim 64: the summary has a buffer of its own and Wt stays.  Head dim 128: summary and Wt of the pass
+      // take turns in one buffer (summary -> its product -> Wt -> its product -> next summary).
+      if (!whole) {
+        if (u >= 1) {
+          if (D == 64) mbar_wait(bars + C::SUM_FREE, (u - 1) & 1, a.status, 263);
+          else mbar_wait(bars + C::W_FREE, (u - 1) & 1, a.status, 264);
+        }
+        if (leader) {
+          mbar_expect_tx(bars + C::SUM_FULL, C::AUX);
+          for (int j = 0; j < C::NB; ++j)
+            for (int f = 0; f < 2; ++f)
+              tma_load_3d(smem + C::OFF_SUM + j * 32768 + f * 16384, &a.tm_sum, bars + C::SUM_FULL, 64 * j,
+                          256 * pass + 128 * f, t.bh);
+        }
+      }
+      if (D != 64 || u == 0) {
+        if (D != 64) {
+          if (!whole) mbar_wait(bars + C::SUM_FREE, u & 1, a.status, 265);
+          else if (u >= 1) mbar_wait(bars + C::W_FREE, (u - 1) & 1, a.status, 266);
+        }
+        if (leader) {
+          mbar_expect_tx(bars + C::W_FULL, C::AUX);
+          for (int j = 0; j < C::NB; ++j) {
+            tma_load_2d(smem + C::OFF_W + j * 16384, &a.tm_hi, bars + C::W_FULL, 64 * j, 128 * pass);
+            tma_load_2d(smem + C::OFF_W + C::AUX / 2 + j * 16384, &a.tm_lo, bars + C::W_FULL, 64 * j, 128 * pass);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == C::W_MMA) {
+    const bool leader = elect_one();
+    constexpr uint32_t id_t = idesc_bf16(128, 64, false, false);
+    constexpr uint32_t id_df = idesc_bf16(128, 256, false, true);
+    constexpr uint32_t id_sum = idesc_bf16(128, 256, false, false);
+    constexpr uint32_t id_dx = idesc_bf16(128, D, false, true);
+    const uint64_t dY = smem_desc_sw128(smem_u32(smem + C::OFF_Y), 16, 1024);
+    const uint64_t dYo = smem_desc_sw128(smem_u32(smem + C::OFF_RING + 32768), 16, 1024);
+    const uint64_t dFo = smem_desc_sw128(smem_u32(smem + C::OFF_RING), 8192, 1024);
+    const uint64_t dSum = smem_desc_sw128(smem_u32(smem + C::OFF_SUM), 16, 1024);
+    const uint64_t dW = smem_desc_sw128(smem_u32(smem + C::OFF_W), 16384, 1024);
+    // G of step s of unit u; gg: its number in the CTA's stream of steps
+    auto issue_t = [&](int u, int s, int gg) {
+      const int it = u / C::PASS, slot = gg % C::NS;
+      if (u % C::PASS == 0 && s == 0) mbar_wait(bars + C::Y_FULL + (it & 1), (it >> 1) & 1, a.status, 267);
+      mbar_wait(bars + C::R_FULL + slot, (gg / C::NS) & 1, a.status, 268);
+      tc_fence_after_sync();
+      if (leader) {
+        const uint64_t y = dY + (uint64_t)((it & 1) * (C::TB >> 4)), o = dYo + (uint64_t)(slot * (C::SLOT >> 4));
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_ss(tb + C::T_G + 64 * (gg & 1), y + kmajor(k, 16384), o + kmajor(k, 8192), id_t, k > 0);
+        mma_commit(bars + C::T_FULL + (gg & 1));
+      }
+      __syncwarp();
+    };
+    int g0 = 0, n = 0, n_next = 0;
+    if (n_u > 0) {
+      n_next = row_tile<SIDE, 64>(a.g, blockIdx.x, whole).n;
+      for (int s = 0; s < 2 && s < n_next; ++s) issue_t(0, s, s);
+    }
+    for (int u = 0; u < n_u; ++u) {
+      const int it = u / C::PASS, pass = u % C::PASS;
+      n = n_next;
+      for (int s = 0; s < n; ++s) {
+        const int gg = g0 + s, slot = gg % C::NS;
+        mbar_wait(bars + C::G_DONE + (gg & 1), (gg >> 1) & 1, a.status, 269);
+        tc_fence_after_sync();
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_ts(tb + C::T_DF, tb + C::T_G + 64 * (gg & 1) + packed(k),
+                   dFo + (uint64_t)(slot * (C::SLOT >> 4) + k * 128), id_df, s > 0 || k > 0);
+          mma_commit(bars + C::R_FREE + slot);
+        }
+        __syncwarp();
+        if (s + 2 < n) issue_t(u, s + 2, gg + 2);
+      }
+      // without steps nobody has waited for the Y tile yet
+      if (n == 0 && pass == 0) mbar_wait(bars + C::Y_FULL + (it & 1), (it >> 1) & 1, a.status, 270);
+      if (!whole) {
+        mbar_wait(bars + C::SUM_FULL, u & 1, a.status, 271);
+        tc_fence_after_sync();
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_ss(tb + C::T_DF, dY + (uint64_t)((it & 1) * (C::TB >> 4)) + kmajor(k, 16384), dSum + kmajor(k, 32768),
+                   id_sum, n > 0 || k > 0);
+          mma_commit(bars + C::SUM_FREE);
+        }
+        __syncwarp();
+      }
+      if (leader) {
+        if (pass == C::PASS - 1) mma_commit(bars + C::Y_FREE + (it & 1));
+        mma_commit(bars + C::DF_FULL);
+      }
+      __syncwarp();
+      // the next unit's first two G run while this unit's df turns into du
+      g0 += n;
+      if (u + 1 < n_u) {
+        if (pass == C::PASS - 1) n_next = row_tile<SIDE, 64>(a.g, blockIdx.x + (it + 1) * step, whole).n;
+        for (int s = 0; s < 2 && s < n_next; ++s) issue_t(u + 1, s, g0 + s);
+      }
+      mbar_wait(bars + C::DU_DONE, u & 1, a.status, 272);
+      if (pass == 0 && it >= 1) mbar_wait(bars + C::DX_FREE, (it - 1) & 1, a.status, 273);
+      if (D != 64) mbar_wait(bars + C::W_FULL, u & 1, a.status, 274);
+      else if (u == 0) mbar_wait(bars + C::W_FULL, 0, a.status, 275);
+      tc_fence_after_sync();
+      if (leader) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)        // the two terms of Wt
+#pragma unroll
+          for (int k = 0; k < 8; ++k)      // 128 projections
+            mma_ts(tb + C::T_DX, tb + C::T_DF + 128 * (k >> 2) + packed(k & 3),
+                   dW + (uint64_t)(x * (C::AUX >> 5) + k * 128), id_dx, pass > 0 || x > 0 || k > 0);
+        mma_commit(bars + C::W_FREE);
+        if (pass == C::PASS - 1) mma_commit(bars + C::DX_FULL);
+      }
+      __syncwarp();
+    }
+  } else {
+    const int qd = warp & 3, cq = warp >> 2;
+    const int row = qd * 32 + lane;
+    const uint32_t lane_base = tb + ((uint32_t)(qd * 32) << 16);
+    const int rows = SIDE == QUERIES ? a.g.T : a.g.S;
+    const float sign = whole ? 1.f : -1.f;   // the window's G enters with a minus
+    int gg = 0;
+    float hs = 0.f;
+    for (int u = 0; u < n_u; ++u) {
+      const int it = u / C::PASS, pass = u % C::PASS;
+      const RowTile t = row_tile<SIDE, 64>(a.g, blockIdx.x + it * step, whole);
+      const int r = t.r0 + row;
+      const bool mine = row < t.nr;
+      const float* dl = a.delta + (int64_t)t.bh * a.Tp;
+      const float rd = SIDE == QUERIES ? __ldg(dl + r) : 0.f;
+      for (int s = 0; s < t.n; ++s, ++gg) {
+        const int c = t.c0 + 64 * s + 32 * cq;
+        const uint32_t vis = seen<SIDE>(a.g, t, r, c, whole);
+        const uint32_t tg = lane_base + C::T_G + 64 * (gg & 1) + 32 * cq;
+        uint32_t o[16];
+        mbar_wait(bars + C::T_FULL + (gg & 1), (gg >> 1) & 1, a.status, 276);
+        tc_fence_after_sync();
+        if (__any_sync(0xffffffffu, vis != 0u)) {
+          uint32_t y[32];
+          tmem_ld32(tg, y);
+          tmem_ld_wait();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            float4 cd = make_float4(rd, rd, rd, rd);
+            if (SIDE == KEYS) cd = __ldg(reinterpret_cast<const float4*>(dl + c) + q);
+            const float dd[4] = {cd.x, cd.y, cd.z, cd.w};
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              v[j] = keep_if_bit(sign * (__uint_as_float(y[4 * q + j]) - dd[j]), vis, 4 * q + j);
+            o[2 * q] = pack_bf16(v[0], v[1]);
+            o[2 * q + 1] = pack_bf16(v[2], v[3]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = 0u;
+        }
+        tmem_st16(tg, o);
+        tmem_st_wait();
+        tc_fence_before_sync();
+        warp_arrive(bars + C::G_DONE + (gg & 1), lane);
+      }
+      // df -> du of this thread's 2 x 32 projections
+      const bool none = whole && t.n == 0;
+      const float d1 = whole ? 0.f : (SIDE == QUERIES ? rd : 1.f);
+      if (pass == 0) hs = 0.f;
+      const __nv_bfloat16* frow = a.f + ((int64_t)t.bh * rows + (mine ? r : t.r0)) * C::M + 256 * pass + 32 * cq;
+      const float* s1 = a.sum1 + (int64_t)t.bh * C::M + 256 * pass + 32 * cq;
+      mbar_wait(bars + C::DF_FULL, u & 1, a.status, 277);
+      tc_fence_after_sync();
+#pragma unroll 1
+      for (int blk = 0; blk < 2; ++blk) {
+        const uint32_t td = lane_base + C::T_DF + 128 * blk + 32 * cq;
+        uint32_t o[16];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t p[16], m[16];
+          tmem_ld16(td + 16 * hf, p);
+          tmem_ld16(td + 64 + 16 * hf, m);
+          uint4 fp[2], fm[2];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            fp[q] = __ldg(reinterpret_cast<const uint4*>(frow + 128 * blk + 16 * hf) + q);
+            fm[q] = __ldg(reinterpret_cast<const uint4*>(frow + 128 * blk + 64 + 16 * hf) + q);
+          }
+          tmem_ld_wait();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const uint32_t wp = (&fp[q >> 2].x)[q & 3], wm = (&fm[q >> 2].x)[q & 3];
+            const float2 sp = __ldg(reinterpret_cast<const float2*>(s1 + 128 * blk + 16 * hf) + q);
+            const float2 sm = __ldg(reinterpret_cast<const float2*>(s1 + 128 * blk + 64 + 16 * hf) + q);
+            const float p0 = none ? 0.f : __uint_as_float(p[2 * q]), p1 = none ? 0.f : __uint_as_float(p[2 * q + 1]);
+            const float m0 = none ? 0.f : __uint_as_float(m[2 * q]), m1 = none ? 0.f : __uint_as_float(m[2 * q + 1]);
+            const float hp0 = bf16_lo(wp) * fmaf(-d1, sp.x, p0), hp1 = bf16_hi(wp) * fmaf(-d1, sp.y, p1);
+            const float hm0 = bf16_lo(wm) * fmaf(-d1, sm.x, m0), hm1 = bf16_hi(wm) * fmaf(-d1, sm.y, m1);
+            hs += (hp0 + hm0) + (hp1 + hm1);
+            o[8 * hf + q] = pack_bf16(hp0 - hm0, hp1 - hm1);
+          }
+        }
+        // (both threads of a row write over their own "+" columns, which only they read)
+        tmem_st16(td, o);
+      }
+      tmem_st_wait();
+      tc_fence_before_sync();
+      warp_arrive(bars + C::DU_DONE, lane);
+      if (pass == C::PASS - 1) {
+        s_h[cq * 128 + row] = hs;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float hsum = a.tau * (s_h[row] + s_h[128 + row]);
+        mbar_wait(bars + C::DX_FULL, it & 1, a.status, 278);
+        tc_fence_after_sync();
+        const __nv_bfloat16* x = a.x + t.b * a.xb + t.h * a.xh + (int64_t)r * a.xr;
+        __nv_bfloat16* dx = a.dx + t.b * a.ob + t.h * a.oh + (int64_t)r * a.orow;
+        const float* part = a.part + ((int64_t)t.bh * rows + r) * D;
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) {
+          const int c = (D / 2) * cq + 16 * q;
+          uint32_t v[16];
+          tmem_ld16(lane_base + C::T_DX + c, v);
+          tmem_ld_wait();
+          if (mine) {
+            uint4 xv[2];
+            xv[0] = __ldg(reinterpret_cast<const uint4*>(x + c));
+            xv[1] = __ldg(reinterpret_cast<const uint4*>(x + c) + 1);
+            uint32_t o[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const uint32_t w = (&xv[j >> 2].x)[j & 3];
+              const float2 e = __ldg(reinterpret_cast<const float2*>(part + c) + j);
+              o[j] = pack_bf16(fmaf(-hsum, bf16_lo(w), __uint_as_float(v[2 * j]) + e.x),
+                               fmaf(-hsum, bf16_hi(w), __uint_as_float(v[2 * j + 1]) + e.y));
+            }
+            reinterpret_cast<uint4*>(dx + c)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            reinterpret_cast<uint4*>(dx + c)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        }
+        tc_fence_before_sync();
+        warp_arrive(bars + C::DX_FREE, lane);
+        // s_h may be written again once everyone has read it: the next write is behind another barrier of this kind
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == C::W_LOAD) {
+    __syncwarp();
+    tmem_dealloc(tb, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dv.
+struct ValArgs {
+  CUtensorMap tm_k, tm_q, tm_do, tm_phi, tm_psi, tm_sum;
+  Geom g;
+  const float* n2;                         // (BH, Tp)
+  __nv_bfloat16* dv; int64_t vb, vs, vh;
+  int* status;
+  int Tp;
+  float tau;
+};
+
+template <int D>
+struct ValCfg {
+  static constexpr int NB = D / 64, M = 4 * D, KBUF = D == 64 ? 2 : 1, NS = 4;
+  static constexpr uint32_t KB = NB * 16384, FB = (M / 64) * 16384;
+  static constexpr uint32_t OFF_K = 0, OFF_F = KBUF * KB, OFF_RING = OFF_F + KBUF * FB, OFF_BAR = OFF_RING + NS * 16384;
+  static constexpr uint32_t SMEM = OFF_BAR + 512 + 1024;
+  static constexpr int NTHR = 576, W_LOAD = 16, W_MMA = 17;
+  static constexpr uint32_t T_DV = 384;    // buffers at 128 b, b < 3
+  enum { K_FULL = 0, K_FREE = 2, F_FULL = 4, F_FREE = 6, R_FULL = 8, R_FREE = R_FULL + NS, S_FULL = R_FREE + NS,
+         E_DONE = S_FULL + 3, P_FULL = E_DONE + 3, D_DONE = P_FULL + 3, DV_FULL = D_DONE + 3, DV_FREE, COUNT };
+  static_assert(SMEM <= 232448 && COUNT <= 60, "shared memory of one CTA");
+};
+
+// The order in which the tensor core consumes what the producer loads; both walk it.  Column steps (128 queries) are
+// numbered g = 0, 1, .. over the CTA's tiles and use buffer g % 3.  The visitor's calls:
+//   score(tile t, first, ke, g)   S of step g; t is where it belongs, ke the number of that tile among those with steps
+//   begin(it), minus(t, s, g), value(t, s, g, first, last), rank(t, it, first, alone)
+template <typename V>
+__device__ __forceinline__ void walk_values(const Geom& g, V& v) {
+  const int stride = gridDim.x;
+  int sc_tile = blockIdx.x, sc_s = 0, sc_g = 0, sc_ke = 0;
+  RowTile sc{};
+  auto seek = [&]() {
+    sc.n = 0;
+    while (sc_tile < g.ntiles) {
+      sc = row_tile<KEYS, 128>(g, sc_tile, false);
+      if (sc.n > 0) break;
+      sc_tile += stride;
+    }
+    sc_s = 0;
+  };
+  auto score = [&]() {
+    if (sc_tile >= g.ntiles) return;
+    v.score(sc, sc_s, sc_ke, sc_g);
+    ++sc_g;
+    if (++sc_s == sc.n) {
+      sc_tile += stride;
+      ++sc_ke;
+      seek();
+    }
+  };
+  seek();
+  score();
+  score();
+  int n = 0;                        // steps so far
+  RowTile pend{};                   // tile and step of the value product that is still to come
+  int pend_s = -1;
+  int it = 0;
+  for (int tile = blockIdx.x; tile < g.ntiles; tile += stride, ++it) {
+    const RowTile t = row_tile<KEYS, 128>(g, tile, false);
+    v.begin(t, it);
+    bool fresh = true;              // nothing of this tile is in dv yet
+    for (int s = 0; s < t.n; ++s, ++n) {
+      v.minus(t, it, s, n);
+      if (pend_s >= 0) {
+        const bool own = s > 0;
+        v.value(pend, own ? it : it - 1, pend_s, n - 1, own && fresh, pend_s == pend.n - 1);
+        if (own) fresh = false;
+      }
+      score();
+      pend = t;
+      pend_s = s;
+    }
+    if (t.n == 0 && pend_s >= 0) {
+      v.value(pend, it - 1, pend_s, n - 1, false, true);
+      pend_s = -1;
+    }
+    v.rank(t, it, fresh, t.n == 0);
+    if (t.n == 0) pend_s = -1;
+  }
+  if (pend_s >= 0) v.value(pend, it - 1, pend_s, n - 1, false, true);
+}
+
+template <int D>
+struct ValLoader {
+  using C = ValCfg<D>;
+  const ValArgs& a;
+  uint8_t* smem;
+  uint64_t* bars;
+  bool leader;
+  int n = 0, loaded = 0;           // ring pieces, phi tiles
+
+  __device__ uint8_t* piece() {
+    const int slot = n % C::NS;
+    if (n >= C::NS) mbar_wait(bars + C::R_FREE + slot, ((n / C::NS) - 1) & 1, a.status, 281);
+    if (leader) mbar_expect_tx(bars + C::R_FULL + slot, 16384);
+    return smem + C::OFF_RING + slot * 16384;
+  }
+  __device__ uint64_t* full() { return bars + C::R_FULL + (n++ % C::NS); }
+  __device__ void phi(const RowTile& t, int it) {
+    const int buf = it % C::KBUF;
+    if (it >= C::KBUF) mbar_wait(bars + C::F_FREE + buf, ((it / C::KBUF) - 1) & 1, a.status, 282);
+    if (leader) {
+      mbar_expect_tx(bars + C::F_FULL + buf, C::FB);
+      for (int j = 0; j < C::M / 64; ++j)
+        tma_load_3d(smem + C::OFF_F + buf * C::FB + j * 16384, &a.tm_phi, bars + C::F_FULL + buf, 64 * j, t.r0, t.bh);
+    }
+    loaded = it + 1;
+  }
+  __device__ void score(const RowTile& t, int s, int ke, int) {
+    if (s == 0) {
+      const int buf = ke % C::KBUF;
+      if (ke >= C::KBUF) mbar_wait(bars + C::K_FREE + buf, ((ke / C::KBUF) - 1) & 1, a.status, 283);
+      if (leader) {
+        mbar_expect_tx(bars + C::K_FULL + buf, C::KB);
+        for (int j = 0; j < C::NB; ++j)
+          tma_load_4d(smem + C::OFF_K + buf * C::KB + j * 16384, &a.tm_k, bars + C::K_FULL + buf, 64 * j, t.r0, t.h, t.b);
+      }
+    }
+    for (int j = 0; j < C::NB; ++j) {
+      uint8_t* dst = piece();
+      uint64_t* bar = full();
+      if (leader) tma_load_4d(dst, &a.tm_q, bar, 64 * j, t.c0 + 128 * s, t.h, t.b);
+    }
+  }
+  __device__ void begin(const RowTile& t, int it) {
+    if (loaded <= it) phi(t, it);
+  }
+  __device__ void minus(const RowTile& t, int it, int s, int) {
+    for (int j = 0; j < C::M / 64; ++j) {
+      uint8_t* dst = piece();
+      uint64_t* bar = full();
+      if (leader) tma_load_3d(dst, &a.tm_psi, bar, 64 * j, t.c0 + 128 * s, t.bh);
+    }
+    // two phi buffers: the next tile's features come in behind this tile's first step (the previous tile's last
+    // product with its buffer was issued before this tile began)
+    if (C::KBUF == 2 && s == 0) {
+      const int tile = blockIdx.x + (it + 1) * (int)gridDim.x;
+      if (tile < a.g.ntiles) phi(row_tile<KEYS, 128>(a.g, tile, false), it + 1);
+    }
+  }
+  __device__ void value(const RowTile& t, int, int s, int, bool, bool) {
+    for (int j = 0; j < C::NB; ++j) {
+      uint8_t* dst = piece();
+      uint64_t* bar = full();
+      if (leader) tma_load_4d(dst, &a.tm_do, bar, 64 * j, t.c0 + 128 * s, t.h, t.b);
+    }
+  }
+  __device__ void rank(const RowTile& t, int, bool, bool) {
+    for (int f = 0; f < C::M / 128; ++f)
+      for (int j = 0; j < C::NB; ++j) {
+        uint8_t* dst = piece();
+        uint64_t* bar = full();
+        if (leader) tma_load_3d(dst, &a.tm_sum, bar, 64 * j, 128 * f, t.bh);
+      }
+  }
+};
+
+template <int D>
+struct ValIssuer {
+  using C = ValCfg<D>;
+  const ValArgs& a;
+  uint64_t* bars;
+  bool leader;
+  uint64_t dK, dF, dR, dRt;
+  int n = 0;
+
+  __device__ int take() {          // the next ring piece, landed
+    const int slot = n % C::NS;
+    mbar_wait(bars + C::R_FULL + slot, (n / C::NS) & 1, a.status, 284);
+    ++n;
+    tc_fence_after_sync();
+    return slot;
+  }
+  __device__ void score(const RowTile& t, int s, int ke, int g) {
+    const int kb = ke % C::KBUF;
+    if (s == 0) mbar_wait(bars + C::K_FULL + kb, (ke / C::KBUF) & 1, a.status, 285);
+    constexpr uint32_t id = idesc_bf16(128, 128, false, false);
+    for (int j = 0; j < C::NB; ++j) {
+      const int slot = take();
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_ss(128 * (g % 3), dK + (uint64_t)(kb * (C::KB >> 4) + j * 1024 + 2 * k), dR + (uint64_t)(slot * 1024 + 2 * k), id,
+                 j > 0 || k > 0);
+        mma_commit(bars + C::R_FREE + slot);
+      }
+      __syncwarp();
+    }
+    if (leader) {
+      mma_commit(bars + C::S_FULL + g % 3);
+      if (s == t.n - 1) mma_commit(bars + C::K_FREE + kb);
+    }
+    __syncwarp();
+  }
+  __device__ void begin(const RowTile&, int it) {
+    mbar_wait(bars + C::F_FULL + it % C::KBUF, (it / C::KBUF) & 1, a.status, 286);
+  }
+  __device__ void minus(const RowTile&, int it, int, int g) {
+    mbar_wait(bars + C::E_DONE + g % 3, (g / 3) & 1, a.status, 287);
+    constexpr uint32_t id = idesc_bf16(128, 128, false, false) | (1u << 13);   // bit 13 negates A
+    const int fb = it % C::KBUF;
+    for (int j = 0; j < C::M / 64; ++j) {
+      const int slot = take();
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_ss(128 * (g % 3), dF + (uint64_t)(fb * (C::FB >> 4) + j * 1024 + 2 * k), dR + (uint64_t)(slot * 1024 + 2 * k), id,
+                 true);
+        mma_commit(bars + C::R_FREE + slot);
+      }
+      __syncwarp();
+    }
+    if (leader) mma_commit(bars + C::P_FULL + g % 3);
+    __syncwarp();
+  }
+  __device__ void value(const RowTile&, int it, int, int g, bool first, bool last) {
+    mbar_wait(bars + C::D_DONE + g % 3, (g / 3) & 1, a.status, 288);
+    if (first && it >= 1) mbar_wait(bars + C::DV_FREE, (it - 1) & 1, a.status, 289);
+    constexpr uint32_t id = idesc_bf16(128, 64, false, true);
+    for (int j = 0; j < C::NB; ++j) {
+      const int slot = take();
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          mma_ts(C::T_DV + 64 * j, 128 * (g % 3) + packed(k), dRt + (uint64_t)(slot * 1024 + k * 128), id, !first || k > 0);
+        mma_commit(bars + C::R_FREE + slot);
+      }
+      __syncwarp();
+    }
+    if (leader && last) mma_commit(bars + C::DV_FULL);
+    __syncwarp();
+  }
+  __device__ void rank(const RowTile&, int it, bool first, bool alone) {
+    if (first && it >= 1) mbar_wait(bars + C::DV_FREE, (it - 1) & 1, a.status, 290);
+    constexpr uint32_t id = idesc_bf16(128, 64, false, true);
+    const int fb = it % C::KBUF;
+    for (int f = 0; f < C::M / 128; ++f)
+      for (int j = 0; j < C::NB; ++j) {
+        const int slot = take();
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_ss(C::T_DV + 64 * j, dF + (uint64_t)(fb * (C::FB >> 4) + 2 * f * 1024) + kmajor(k, 16384),
+                   dRt + (uint64_t)(slot * 1024 + k * 128), id, !first || f > 0 || k > 0);
+          mma_commit(bars + C::R_FREE + slot);
+        }
+        __syncwarp();
+      }
+    if (leader) {
+      mma_commit(bars + C::F_FREE + fb);
+      if (alone) mma_commit(bars + C::DV_FULL);
+    }
+    __syncwarp();
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(576, 1) bwd_value_kernel(const __grid_constant__ ValArgs a) {
+  using C = ValCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::COUNT);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  if (tid == 0) {
+    for (int i = 0; i < C::COUNT; ++i)
+      mbar_init(bars + i, (i >= C::E_DONE && i < C::P_FULL) || (i >= C::D_DONE && i < C::DV_FULL) || i == C::DV_FREE ? 8 : 1);
+    fence_mbar_init();
+  }
+  if (warp == C::W_LOAD) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  constexpr uint32_t tb = 0;
+  if (tid == 0 && *tmem_slot != 0) atomicCAS(a.status, 0, 241);
+  const int step = gridDim.x;
+
+  if (warp == C::W_LOAD) {
+    ValLoader<D> v{a, smem, bars, elect_one()};
+    walk_values(a.g, v);
+    __syncwarp();
+  } else if (warp == C::W_MMA) {
+    ValIssuer<D> v{a, bars, elect_one(), smem_desc_sw128(smem_u32(smem + C::OFF_K), 16, 1024),
+                   smem_desc_sw128(smem_u32(smem + C::OFF_F), 16, 1024),
+                   smem_desc_sw128(smem_u32(smem + C::OFF_RING), 16, 1024),
+                   smem_desc_sw128(smem_u32(smem + C::OFF_RING), 16384, 1024)};
+    walk_values(a.g, v);
+    __syncwarp();
+  } else {
+    // exponential group (warps 0-7): S -> p in place; packing group (warps 8-15): p - a -> bf16, epilogue.
+    // A thread owns a row and 64 columns, in two chunks of 32.
+    const bool exp_group = warp < 8;
+    const int qd = warp & 3, cq = (warp >> 2) & 1;
+    const int row = qd * 32 + lane;
+    const uint32_t lane_base = tb + ((uint32_t)(qd * 32) << 16);
+    const float sc = a.tau * kLog2e;
+    int g = 0, it = 0;
+    for (int tile = blockIdx.x; tile < a.g.ntiles; tile += step, ++it) {
+      const RowTile t = row_tile<KEYS, 128>(a.g, tile, false);
+      const int r = t.r0 + row;
+      const float* n2 = a.n2 + (int64_t)t.bh * a.Tp;
+      for (int s = 0; s < t.n; ++s, ++g) {
+        const int buf = g % 3;
+        mbar_wait(bars + (exp_group ? C::S_FULL : C::P_FULL) + buf, (g / 3) & 1, a.status, exp_group ? 291 : 292);
+        tc_fence_after_sync();
+#pragma unroll 1
+        for (int ch = 0; ch < 2; ++ch) {
+          const int c = t.c0 + 128 * s + 64 * cq + 32 * ch;
+          const uint32_t vis = seen<KEYS>(a.g, t, r, c, false);
+          const bool any = __any_sync(0xffffffffu, vis != 0u);
+          const uint32_t tc = lane_base + 128 * buf + 64 * cq + 32 * ch;
+          if (exp_group) {
+            if (!any) continue;   // hidden columns keep what they hold: the packing group writes zeros for them
+            uint32_t x[32];
+            tmem_ld32(tc, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const float4 n = __ldg(reinterpret_cast<const float4*>(n2 + c) + q);
+              x[4 * q] = __float_as_uint(ex2(fmaf(__uint_as_float(x[4 * q]), sc, -n.x)));
+              x[4 * q + 1] = __float_as_uint(ex2(fmaf(__uint_as_float(x[4 * q + 1]), sc, -n.y)));
+              x[4 * q + 2] = __float_as_uint(ex2(fmaf(__uint_as_float(x[4 * q + 2]), sc, -n.z)));
+              x[4 * q + 3] = __float_as_uint(ex2(fmaf(__uint_as_float(x[4 * q + 3]), sc, -n.w)));
+            }
+            tmem_st32(tc, x);
+          } else {
+            uint32_t o[16];
+            if (any) {
+              uint32_t x[32];
+              tmem_ld32(tc, x);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                o[j] = pack_bf16(keep_if_bit(__uint_as_float(x[2 * j]), vis, 2 * j),
+                                 keep_if_bit(__uint_as_float(x[2 * j + 1]), vis, 2 * j + 1));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = 0u;
+            }
+            tmem_st16(tc, o);
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before_sync();
+        warp_arrive(bars + (exp_group ? C::E_DONE : C::D_DONE) + buf, lane);
+      }
+      if (!exp_group) {
+        mbar_wait(bars + C::DV_FULL, it & 1, a.status, 293);
+        tc_fence_after_sync();
+        __nv_bfloat16* dst = a.dv + t.b * a.vb + t.h * a.vh + (int64_t)r * a.vs;
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) {
+          const int c = (D / 2) * cq + 16 * q;
+          uint32_t v[16];
+          tmem_ld16(lane_base + C::T_DV + c, v);
+          tmem_ld_wait();
+          uint32_t o[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = pack_bf16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+          if (row < t.nr) {
+            reinterpret_cast<uint4*>(dst + c)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            reinterpret_cast<uint4*>(dst + c)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        }
+        tc_fence_before_sync();
+        warp_arrive(bars + C::DV_FREE, lane);
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == C::W_LOAD) {
+    __syncwarp();
+    tmem_dealloc(tb, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+bool map_rows(CUtensorMap* m, const void* base, int64_t width, int64_t rows, int BH, uint32_t box_rows) {
+  const uint64_t dims[3] = {(uint64_t)width, (uint64_t)rows, (uint64_t)BH};
+  const uint64_t str[2] = {(uint64_t)width * 2, (uint64_t)(rows * width) * 2};
+  const uint32_t box[3] = {64, box_rows, 1};
+  return cached_tmap(m, base, 3, dims, str, box);
+}
+bool map_w(CUtensorMap* m, const void* base, int D, uint32_t box_rows) {
+  const uint64_t dims[2] = {(uint64_t)D, (uint64_t)(2 * D)};
+  const uint64_t str[1] = {(uint64_t)D * 2};
+  const uint32_t box[2] = {64, box_rows};
+  return cached_tmap(m, base, 2, dims, str, box);
+}
+
+// Raises the kernel's shared-memory limit once per device.
+template <typename K>
+cudaError_t allow_smem(K kernel, uint32_t bytes, bool* done) {
+  if (*done) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) *done = true;
+  return e;
+}
+
+struct Side {
+  const void *x, *y;
+  int64_t xb, xr, xh, yb, yr, yh;
+  int rows;
+};
+struct Host {
+  const SblParams& p;
+  const SblGrads& g;
+  const TcBwdWorkspace& ws;
+  char* base;
+  cudaStream_t st;
+  DeviceInfo* dev;
+  Side side[2];
+  template <typename T>
+  T* at(size_t off) const { return reinterpret_cast<T*>(base + off); }
+  bool map_x(CUtensorMap* m, int s, uint32_t box) const {
+    const Side& d = side[s];
+    return map_bthe(m, d.x, p.B, d.rows, p.H, p.E, d.xb, d.xr, d.xh, box);
+  }
+  bool map_y(CUtensorMap* m, int s, uint32_t box) const {
+    const Side& d = side[s];
+    return map_bthe(m, d.y, p.B, d.rows, p.H, p.E, d.yb, d.yr, d.yh, box);
+  }
+  Geom geom(int s) const {
+    Geom gm;
+    gm.lengths = p.key_lengths;
+    gm.H = p.H;
+    gm.T = p.T;
+    gm.S = p.S;
+    // a window wider than both sequences sees everything: keeps the index arithmetic far from 2^31
+    const int64_t most = 2 * (int64_t)(p.T > p.S ? p.T : p.S) + 2;
+    gm.w = (int)(p.w < most ? p.w : most);
+    gm.ntr = (int)div_up(side[s].rows, TR);
+    gm.ntiles = gm.ntr * p.B * p.H;
+    return gm;
+  }
+};
+
+template <int SIDE, int D>
+cudaError_t launch_feat(const Host& h) {
+  using C = FeatCfg<D>;
+  FeatArgs a{};
+  const int BH = h.p.B * h.p.H, rows = h.side[SIDE].rows;
+  if (!h.map_x(&a.tm_x, SIDE, 128) || !h.map_y(&a.tm_y, SIDE, 128) || !map_w(&a.tm_hi, h.at<void>(h.ws.fwd.phiq), D, 64) ||
+      !map_w(&a.tm_lo, h.at<void>(h.ws.wlo), D, 64) || !map_rows(&a.tm_f, h.at<void>(h.ws.feat[SIDE]), C::M, rows, BH, 128))
+    return cudaErrorInvalidValue;
+  a.lengths = h.p.key_lengths;
+  a.beta = h.at<float>(h.ws.fwd.beta);
+  a.n2 = h.at<float>(h.ws.n2);
+  a.delta = h.at<float>(h.ws.delta);
+  a.partial = h.at<float>(h.ws.partial);
+  a.status = h.at<int>(h.ws.fwd.status);
+  a.H = h.p.H;
+  a.rows = rows;
+  a.Tp = h.ws.Tp;
+  a.nsplit = h.ws.nsplit[SIDE];
+  a.tau = h.p.softmax_temp;
+  a.half_log_m = (float)(log((double)C::M) / 2.0);
+  cudaError_t e = allow_smem(bwd_feat_kernel<SIDE, D>, C::SMEM, &h.dev->attr_bwd[D == 128][0][SIDE]);
+  if (e != cudaSuccess) return e;
+  bwd_feat_kernel<SIDE, D><<<dim3((unsigned)(a.nsplit * (C::M / 128)), (unsigned)BH), C::NTHR, C::SMEM, h.st>>>(a);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  const int64_t n = (int64_t)BH * C::M;
+  bwd_combine_kernel<D><<<(unsigned)div_up(n * (D / 4 + 1), 256), 256, 0, h.st>>>(
+      a.partial, a.nsplit, n, C::M, h.at<__nv_bfloat16>(h.ws.sum[SIDE]), h.at<float>(h.ws.sum1[SIDE]));
+  return cudaGetLastError();
+}
+
+template <int SIDE, int D>
+cudaError_t launch_side(const Host& h, void* dx, int64_t ob, int64_t orow, int64_t oh) {
+  constexpr int OTHER = 1 - SIDE;
+  const int BH = h.p.B * h.p.H;
+  cudaError_t e;
+  {
+    using C = WinCfg<D>;
+    WinArgs a{};
+    if (!h.map_x(&a.tm_x, SIDE, 128) || !h.map_y(&a.tm_y, SIDE, 128) || !h.map_x(&a.tm_xo, OTHER, 64) ||
+        !h.map_y(&a.tm_yo, OTHER, 64))
+      return cudaErrorInvalidValue;
+    a.g = h.geom(SIDE);
+    a.n2 = h.at<float>(h.ws.n2);
+    a.delta = h.at<float>(h.ws.delta);
+    a.part = h.at<float>(h.ws.part);
+    a.status = h.at<int>(h.ws.fwd.status);
+    a.Tp = h.ws.Tp;
+    a.tau = h.p.softmax_temp;
+    if ((e = allow_smem(bwd_window_kernel<SIDE, D>, C::SMEM, &h.dev->attr_bwd[D == 128][1][SIDE])) != cudaSuccess) return e;
+    bwd_window_kernel<SIDE, D><<<(unsigned)(a.g.ntiles < h.dev->sms ? a.g.ntiles : h.dev->sms), C::NTHR, C::SMEM, h.st>>>(a);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  }
+  using C = LowCfg<D>;
+  LowArgs a{};
+  if (!h.map_y(&a.tm_y, SIDE, 128) || !h.map_y(&a.tm_yo, OTHER, 64) ||
+      !map_rows(&a.tm_fo, h.at<void>(h.ws.feat[OTHER]), C::M, h.side[OTHER].rows, BH, 64) ||
+      !map_rows(&a.tm_sum, h.at<void>(h.ws.sum[OTHER]), D, C::M, BH, 128) ||
+      !map_w(&a.tm_hi, h.at<void>(h.ws.fwd.phiq), D, 128) || !map_w(&a.tm_lo, h.at<void>(h.ws.wlo), D, 128))
+    return cudaErrorInvalidValue;
+  a.g = h.geom(SIDE);
+  a.f = h.at<__nv_bfloat16>(h.ws.feat[SIDE]);
+  a.sum1 = h.at<float>(h.ws.sum1[OTHER]);
+  a.delta = h.at<float>(h.ws.delta);
+  a.part = h.at<float>(h.ws.part);
+  a.x = static_cast<const __nv_bfloat16*>(h.side[SIDE].x);
+  a.xb = h.side[SIDE].xb; a.xr = h.side[SIDE].xr; a.xh = h.side[SIDE].xh;
+  a.dx = static_cast<__nv_bfloat16*>(dx);
+  a.ob = ob; a.orow = orow; a.oh = oh;
+  a.status = h.at<int>(h.ws.fwd.status);
+  a.Tp = h.ws.Tp;
+  // Few columns: the sum over those outside the window instead of all - inside (accuracy, see the top).  It visits
+  // every column, so it is used while that is at most the window's own steps and four more.
+  a.whole = div_up(h.side[OTHER].rows, 64) <= div_up((int64_t)a.g.w + TR, 64) + 4;
+  a.tau = h.p.softmax_temp;
+  if ((e = allow_smem(bwd_lowrank_kernel<SIDE, D>, C::SMEM, &h.dev->attr_bwd[D == 128][2][SIDE])) != cudaSuccess) return e;
+  bwd_lowrank_kernel<SIDE, D><<<(unsigned)(a.g.ntiles < h.dev->sms ? a.g.ntiles : h.dev->sms), C::NTHR, C::SMEM, h.st>>>(a);
+  return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t backward(const Host& h) {
+  using C = ValCfg<D>;
+  const SblParams& p = h.p;
+  const SblGrads& g = h.g;
+  const int BH = p.B * p.H;
+  cudaError_t e;
+  float* beta = h.at<float>(h.ws.fwd.beta);
+  if ((e = tc_prepare_projection(p, h.ws.fwd, h.base, h.st, true, beta, h.at<__nv_bfloat16>(h.ws.wlo))) != cudaSuccess)
+    return e;
+  if ((e = tc_key_logscale_bound(p, h.ws.fwd, h.base, beta, h.st, true)) != cudaSuccess) return e;
+  const int64_t lanes = (int64_t)BH * h.ws.Tp * (D / 8);
+  bwd_rows_kernel<D><<<(unsigned)div_up(lanes, 256), 256, 0, h.st>>>(
+      static_cast<const __nv_bfloat16*>(p.out), p.o_stride_b, p.o_stride_t, p.o_stride_h,
+      static_cast<const __nv_bfloat16*>(g.dout), g.do_stride_b, g.do_stride_t, g.do_stride_h, g.row_stats, p.B, p.H, p.T,
+      h.ws.Tp, h.at<float>(h.ws.n2), h.at<float>(h.ws.delta));
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  if ((e = launch_feat<KEYS, D>(h)) != cudaSuccess) return e;
+  if ((e = launch_feat<QUERIES, D>(h)) != cudaSuccess) return e;
+  ValArgs a{};
+  if (!h.map_x(&a.tm_k, KEYS, 128) || !h.map_x(&a.tm_q, QUERIES, 128) || !h.map_y(&a.tm_do, QUERIES, 128) ||
+      !map_rows(&a.tm_phi, h.at<void>(h.ws.feat[KEYS]), C::M, p.S, BH, 128) ||
+      !map_rows(&a.tm_psi, h.at<void>(h.ws.feat[QUERIES]), C::M, p.T, BH, 128) ||
+      !map_rows(&a.tm_sum, h.at<void>(h.ws.sum[QUERIES]), D, C::M, BH, 128))
+    return cudaErrorInvalidValue;
+  a.g = h.geom(KEYS);
+  a.n2 = h.at<float>(h.ws.n2);
+  a.dv = static_cast<__nv_bfloat16*>(g.dv);
+  a.vb = g.dv_stride_b; a.vs = g.dv_stride_s; a.vh = g.dv_stride_h;
+  a.status = h.at<int>(h.ws.fwd.status);
+  a.Tp = h.ws.Tp;
+  a.tau = p.softmax_temp;
+  if ((e = allow_smem(bwd_value_kernel<D>, C::SMEM, &h.dev->attr_bwd[D == 128][3][0])) != cudaSuccess) return e;
+  bwd_value_kernel<D><<<(unsigned)(a.g.ntiles < h.dev->sms ? a.g.ntiles : h.dev->sms), C::NTHR, C::SMEM, h.st>>>(a);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  if ((e = launch_side<QUERIES, D>(h, g.dq, g.dq_stride_b, g.dq_stride_t, g.dq_stride_h)) != cudaSuccess) return e;
+  return launch_side<KEYS, D>(h, g.dk, g.dk_stride_b, g.dk_stride_s, g.dk_stride_h);
+}
+
+}  // namespace
+
+const char* tc_backward_strides(const SblGrads& g, const SblParams& p) {
+  struct { const char* name; const void* ptr; int64_t b, r, h; } t[] = {
+      {"dout", g.dout, g.do_stride_b, g.do_stride_t, g.do_stride_h},
+      {"dq", g.dq, g.dq_stride_b, g.dq_stride_t, g.dq_stride_h},
+      {"dk", g.dk, g.dk_stride_b, g.dk_stride_s, g.dk_stride_h},
+      {"dv", g.dv, g.dv_stride_b, g.dv_stride_s, g.dv_stride_h}};
+  for (const auto& x : t) {
+    if (!aligned16(x.ptr)) return x.name;
+    // a size-1 axis may carry any stride
+    for (int64_t s : {p.B > 1 ? x.b : 8, x.r, p.H > 1 ? x.h : 8})
+      if (s % 8 != 0 || s <= 0) return x.name;
+    if (x.r < p.E) return x.name;
+  }
+  return nullptr;
+}
+
+void tc_plan_backward(const SblParams& p, TcBwdWorkspace* ws) {
+  const size_t BH = (size_t)p.B * p.H, m = 2 * (size_t)p.r, D = p.D, T = p.T, S = p.S;
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off = (off + bytes + 255) & ~(size_t)255;
+    return at;
+  };
+  Workspace& f = ws->fwd;
+  f = Workspace{};
+  f.tensor = true;
+  f.status = take(64);                       // first: hosts read the words without asking where they are
+  f.wt = take((size_t)p.r * p.E * 4);
+  f.phiq = take((size_t)p.r * p.E * 2);      // the projection's first bf16 term
+  ws->wlo = take((size_t)p.r * p.E * 2);     // ... and its second
+  f.beta = take(BH * 4);
+  ws->Tp = (int)(div_up(p.T, TR) * TR);
+  ws->n2 = take(BH * ws->Tp * 4);
+  ws->delta = take(BH * ws->Tp * 4);
+  ws->feat[QUERIES] = take(BH * T * m * 2);
+  ws->feat[KEYS] = take(BH * S * m * 2);
+  size_t partial = 0;
+  for (int s = 0; s < 2; ++s) {
+    ws->sum[s] = take(BH * m * D * 2);
+    ws->sum1[s] = take(BH * m * 4);
+    // about two waves of CTAs over (b*h, blocks of 128 features)
+    const int ntiles = (int)div_up(s == QUERIES ? p.T : p.S, TR);
+    const size_t units = BH * (m / 128);
+    int ns = (int)((296 + units / 2) / units);
+    ns = ns < 1 ? 1 : ns;
+    ws->nsplit[s] = ns > ntiles ? ntiles : ns;
+    const size_t bytes = BH * ws->nsplit[s] * m * (D + 4) * 4;
+    partial = bytes > partial ? bytes : partial;
+  }
+  ws->partial = take(partial);
+  ws->part = take(BH * (T > S ? T : S) * D * 4);
+  f.total = off;
+}
+
+cudaError_t tc_backward(const SblParams& p, const SblGrads& g, const TcBwdWorkspace& ws, char* base, cudaStream_t st) {
+  DeviceInfo* dev = nullptr;
+  cudaError_t e = device_info(&dev);
+  if (e != cudaSuccess) return e;
+  Host h{p, g, ws, base, st, dev,
+         {{p.q, g.dout, p.q_stride_b, p.q_stride_t, p.q_stride_h, g.do_stride_b, g.do_stride_t, g.do_stride_h, p.T},
+          {p.k, p.v, p.k_stride_b, p.k_stride_s, p.k_stride_h, p.v_stride_b, p.v_stride_s, p.v_stride_h, p.S}}};
+  return p.E == 64 ? backward<64>(h) : backward<128>(h);
+}
+
+}  // namespace sbl

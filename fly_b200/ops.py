@@ -175,13 +175,17 @@ class Problem:
         _cabi.check(_cabi.load().sbl_backward_workspace_bytes(ctypes.byref(self.params), ctypes.byref(n)))
         return n.value
 
-    def backward(self, grad_out, row_stats):
-        """(dq, dk, dv) of sum(grad_out * out); the problem's `out` must hold the output of `forward_train`."""
+    def backward(self, grad_out, row_stats, watch=False):
+        """(dq, dk, dv) of sum(grad_out * out); the problem's `out` must hold the output of `forward_train`.
+        watch: as in `forward`."""
         query, key, value = self._keep[:3]
         B, H, T, S, E, D = self.shape
         if grad_out.shape != (B, T, H, D) or grad_out.dtype != query.dtype or grad_out.device != self.device:
             raise ValueError('grad_out must be (B,T,H,D) in the input dtype on the problem device')
-        if grad_out.stride(-1) != 1:
+        # (the tensor-core kernels read it through tensor maps: no broadcast axes, 16-byte steps)
+        tensor = self.status_offset is not None
+        if grad_out.stride(-1) != 1 or tensor and (grad_out.data_ptr() % 16 or grad_out.stride(1) < D or any(
+                n > 1 and (st <= 0 or st % 8) for n, st in zip(grad_out.shape[:3], grad_out.stride()))):
             grad_out = grad_out.contiguous()
         nbytes = self.backward_workspace_bytes()
         dq, dk, dv = (torch.empty(x.shape, device=self.device, dtype=x.dtype) for x in (query, key, value))
@@ -196,7 +200,9 @@ class Problem:
         with torch.cuda.device(self.device):
             stream = torch.cuda.current_stream(self.device).cuda_stream
             rc = _cabi.load().sbl_backward(ctypes.byref(self.params), ctypes.byref(g), ws.data_ptr(), nbytes, stream)
-        _cabi.check(rc)
+            _cabi.check(rc)
+            if tensor and watch and not torch.cuda.is_current_stream_capturing():
+                status_watch.post(ws, 0, self.device)
         return dq, dk, dv
 
     def check_status(self, workspace=None):
@@ -275,7 +281,7 @@ class _SBLocal(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths, watch):
         prob = Problem(query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths)
-        ctx.args = (local_context, softmax_temp, softmax_eps)
+        ctx.args, ctx.watch = (local_context, softmax_temp, softmax_eps), watch
         if softmax_eps != 0:
             # the forward is built for eps != 0, its gradients are not
             ctx.stats = None
@@ -297,7 +303,7 @@ class _SBLocal(torch.autograd.Function):
             raise NotImplementedError('sblocal_b200: gradients are built for softmax_eps = 0 only')
         query, key, value, W, key_lengths, out, stats = ctx.saved_tensors
         prob = Problem(query, key, value, W, *ctx.args, key_lengths, out=out)
-        dq, dk, dv = prob.backward(grad_out, stats)
+        dq, dk, dv = prob.backward(grad_out, stats, watch=ctx.watch)
         return dq, dk, dv, None, None, None, None, None, None
 
 

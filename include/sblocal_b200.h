@@ -240,7 +240,9 @@ int sbl_forward_train(const SblParams* p, void* workspace, size_t workspace_byte
 /*
  * Gradients of sbl_forward_train.  Layouts as in SblParams: dout like out, dq
  * like q, dk like k, dv like v, same dtype, last axis contiguous, element
- * strides for the others (a stride of 0 is allowed in dout only).
+ * strides for the others (a stride of 0 is allowed in dout only).  Where the
+ * tensor-core kernels run (sbl_status_words succeeds), all four are 16-byte
+ * aligned with positive strides that are multiples of 8.
  */
 typedef struct SblGrads {
   const void* dout; int64_t do_stride_b, do_stride_t, do_stride_h;
@@ -251,7 +253,10 @@ typedef struct SblGrads {
   int32_t reserved[4];        /* must be 0                                                 */
 } SblGrads;
 
-/* Bytes of workspace sbl_backward needs (256-byte aligned base); nothing of a forward's workspace is reused. */
+/*
+ * Bytes of workspace sbl_backward needs (256-byte aligned base); nothing of a forward's workspace is reused.  The
+ * tensor-core kernels leave the status words of sbl_status_words at its start (word 0 only; the others stay 0).
+ */
 int sbl_backward_workspace_bytes(const SblParams* p, size_t* bytes);
 
 /*

@@ -78,6 +78,66 @@ def test_gradients_any_shape(case, dtype, sbl_lib):
                 assert (got[0][b] == 0).all() and (got[1][b] == 0).all()
 
 
+TENSOR = [
+    # B, H, T, S, d, w, tau, lengths: both head dims of the tensor-core kernels
+    (1, 1, 128, 128, 64, 64, None, None),
+    (2, 3, 1000, 1000, 64, 256, None, None),
+    (2, 2, 1200, 1200, 64, 8, None, (1200, 333)),
+    (1, 2, 900, 2000, 64, 100, None, None),          # more keys than queries: key tiles nobody sees
+    (1, 2, 2000, 900, 64, 33, None, None),           # queries behind the last key
+    (3, 2, 777, 777, 64, 257, 576 ** -0.5, (777, 128, 0)),
+    (1, 1, 300, 1, 64, 16, None, None),
+    (2, 1, 3, 1500, 64, 2048, None, None),
+    (1, 2, 1500, 1500, 64, 1000, None, (1400,)),
+    (1, 1, 16, 16, 64, 256, None, None),             # a short sequence, all of it in every window
+    (4, 40, 130, 130, 64, 20, None, None),           # more tiles than SMs
+    (1, 1, 128, 128, 128, 64, None, None),
+    (2, 2, 1000, 1000, 128, 512, None, (1000, 513)),
+    (1, 2, 700, 1900, 128, 64, None, None),
+    (1, 2, 1900, 700, 128, 129, None, None),
+    (2, 1, 1, 1300, 128, 5, None, None),
+    (1, 1, 40, 40, 128, 512, None, None),
+    (2, 40, 200, 260, 128, 4000, None, None),
+]
+
+
+@pytest.mark.parametrize('case', TENSOR, ids=lambda c: '-'.join(str(x) for x in c[:6]))
+def test_gradients_on_the_tensor_cores(case, sbl_lib):
+    from fly_b200 import ops
+    B, H, T, S, d, w, tau, lengths = case
+    q, k, v, dout, W = inputs(B, T, S, H, d, d, 2 * d, torch.bfloat16, tau, seed=1)
+    lengths = torch.tensor(lengths, device='cuda') if lengths else None
+    prob = ops.Problem(q, k, v, W, w, tau, key_lengths=lengths)
+    assert (prob.status_offset is not None) == (w <= 2048 or d == 128)
+    got = grads_of(q, k, v, dout, W, w, tau, lengths)
+    ref = sblocal_grads(q, k, v, dout, W, w, tau, lengths)
+    if S == 1:   # the logits have no gradient: held to the size of what cancels in it
+        size = float((dout.float().norm(dim=-1) * v.float().norm(dim=-1)).max())
+        assert got[1].float().abs().max() <= BF16_TENSOR * size
+        got, ref = (got[0], got[3]), (ref[0], ref[3])
+        assert all(rel2(x, y) <= BF16_TENSOR for x, y in zip(got, ref))
+        return
+    check(got, ref, BF16_TENSOR)
+    if lengths is not None:
+        for b, n in enumerate(lengths.tolist()):
+            assert (got[2][b, n:] == 0).all() and (got[3][b, n:] == 0).all()
+            if n == 0:
+                assert (got[0][b] == 0).all() and (got[1][b] == 0).all()
+
+
+def test_gradients_of_long_sequences(sbl_lib):
+    """One (batch, head) of the long configuration, against the kernels for any shape on the same inputs (which the
+    tests above hold to the definition): the difference is at most the sum of both tolerances."""
+    from fly_b200 import ops
+    for d, N, w in ((64, 16384, 256), (128, 8192, 512)):
+        q, k, v, dout, W = inputs(1, N, N, 1, d, d, 2 * d, torch.bfloat16)
+        got = grads_of(q, k, v, dout, W, w)
+        prob = ops.Problem(q, k, v, W, w, generic=True)
+        ws = torch.empty(prob.workspace_bytes, dtype=torch.uint8, device='cuda')
+        out, stats = prob.forward_train(ws)
+        check(got, (out, *prob.backward(dout, stats)), BF16_TENSOR + BF16_ANY)
+
+
 def test_single_key_has_no_gradient_in_the_logits(sbl_lib):
     """One key: its weight is 1 whatever the logit, so dq = dk = 0 up to roundings of dout.v, and dv = sum dout."""
     for dtype, tol in ((torch.float32, 64 * 2.0 ** -24), (torch.bfloat16, 4 * 2.0 ** -8)):
