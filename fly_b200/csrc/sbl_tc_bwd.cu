@@ -108,6 +108,18 @@ __device__ __forceinline__ uint32_t seen(const Geom& g, const RowTile& t, int ro
 __device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
   return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~(uintptr_t)1023);
 }
+// mbar_wait without the call.  A call makes the issuing warp rebuild every matrix descriptor behind it: about 130
+// cycles per group of four MMAs (256 cycles of work at N = 128), 30 with the loop in line.
+__device__ __forceinline__ void wait_inline(uint64_t* bar, uint32_t parity, int* status, int code) {
+  uint32_t n = 0;
+  while (!mbar_try_wait(bar, parity)) {
+    ++n;
+    if (n >= kWaitLimit || ((n & 255u) == 255u && *reinterpret_cast<volatile int*>(status) != 0)) {
+      atomicCAS(status, 0, code);
+      break;
+    }
+  }
+}
 // start-address steps (in 16-byte units) of K step k inside a K-major operand of [rows][64] pieces
 __device__ __forceinline__ uint64_t kmajor(int k, uint32_t piece_bytes) {
   return (uint64_t)((uint32_t)(k >> 2) * (piece_bytes >> 4) + (uint32_t)(k & 3) * 2);
@@ -117,34 +129,47 @@ __device__ __forceinline__ uint32_t packed(int k) { return 32u * (uint32_t)(k >>
 
 // ---------------------------------------------------------------------------
 // Per query row: n2 = log-normaliser * log2(e), delta = dout . out; both (BH, Tp), zero in the padding rows.
+// D / 8 lanes per row, four rows per group of lanes with all their loads in flight.
 template <int D>
 __global__ void __launch_bounds__(256) bwd_rows_kernel(const __nv_bfloat16* out, int64_t ob, int64_t ot, int64_t oh,
                                                        const __nv_bfloat16* dout, int64_t db, int64_t dt, int64_t dh,
                                                        const float* stats, int B, int H, int T, int Tp, float* n2,
                                                        float* delta) {
-  constexpr int LPR = D / 8;
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;   // (b, t, h), heads innermost
+  constexpr int LPR = D / 8, RPB = 256 / LPR;
   const int sub = threadIdx.x % LPR;
-  const int h = (int)(i % H), t = (int)((i / H) % Tp), b = (int)(i / ((int64_t)H * Tp));
-  float s = 0.f;
-  if (b < B && t < T) {
-    const uint4 x = __ldg(reinterpret_cast<const uint4*>(out + b * ob + t * ot + h * oh) + sub);
-    const uint4 y = __ldg(reinterpret_cast<const uint4*>(dout + b * db + t * dt + h * dh) + sub);
-    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+  const int64_t total = (int64_t)B * H * Tp, rows = (int64_t)B * H * T;
+  uint4 x[4], y[4];
+  int h[4], t[4], b[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t i = ((int64_t)blockIdx.x * 4 + u) * RPB + threadIdx.x / LPR;   // (b, t, h), heads innermost
+    h[u] = (int)(i % H);
+    t[u] = (int)((i / H) % Tp);
+    b[u] = i < total ? (int)(i / ((int64_t)H * Tp)) : -1;
+    x[u] = y[u] = make_uint4(0, 0, 0, 0);
+    if (b[u] >= 0 && t[u] < T) {
+      x[u] = __ldg(reinterpret_cast<const uint4*>(out + b[u] * ob + t[u] * ot + h[u] * oh) + sub);
+      y[u] = __ldg(reinterpret_cast<const uint4*>(dout + b[u] * db + t[u] * dt + h[u] * dh) + sub);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, yw[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+    float s = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       s = fmaf(bf16_lo(xw[j]), bf16_lo(yw[j]), s);
       s = fmaf(bf16_hi(xw[j]), bf16_hi(yw[j]), s);
     }
-  }
 #pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (b < B && sub == 0) {
-    const int64_t bh = (int64_t)b * H + h, rows = (int64_t)B * H * T;
-    float n = 0.f;
-    if (t < T) n = stats[bh * T + t] * kLog2e + log2f(stats[rows + bh * T + t]);
-    n2[bh * Tp + t] = n;
-    delta[bh * Tp + t] = s;
+    for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (b[u] >= 0 && sub == 0) {
+      const int64_t bh = (int64_t)b[u] * H + h[u];
+      float n = 0.f;
+      if (t[u] < T) n = stats[bh * T + t[u]] * kLog2e + log2f(stats[rows + bh * T + t[u]]);
+      n2[bh * Tp + t[u]] = n;
+      delta[bh * Tp + t[u]] = s;
+    }
   }
 }
 
@@ -228,19 +253,25 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
         tma_load_2d(smem + C::OFF_W + C::WB + j * 8192, &a.tm_lo, bar_w, 64 * j, 64 * fb);
       }
     }
-    for (int i = 0; i < nt; ++i) {
-      const int r0 = (t_lo + i) * TR, xs = i % C::XD, s = i & 1;
-      if (i >= C::XD) mbar_wait(x_free + xs, ((i / C::XD) - 1) & 1, a.status, 201);
-      if (leader) {
-        mbar_expect_tx(x_full + xs, C::XB);
-        for (int j = 0; j < C::NB; ++j)
-          tma_load_4d(smem + C::OFF_X + xs * C::XB + j * 16384, &a.tm_x, x_full + xs, 64 * j, r0, h, b);
+    // X runs one tile ahead of Y: a Y slot is freed by the summary of two tiles back, an X slot long before
+    for (int i = 0; i <= nt; ++i) {
+      if (i < nt) {
+        const int xs = i % C::XD;
+        if (i >= C::XD) wait_inline(x_free + xs, ((i / C::XD) - 1) & 1, a.status, 201);
+        if (leader) {
+          mbar_expect_tx(x_full + xs, C::XB);
+          for (int j = 0; j < C::NB; ++j)
+            tma_load_4d(smem + C::OFF_X + xs * C::XB + j * 16384, &a.tm_x, x_full + xs, 64 * j, (t_lo + i) * TR, h, b);
+        }
       }
-      if (i >= 2) mbar_wait(y_free + s, ((i >> 1) - 1) & 1, a.status, 202);
-      if (leader) {
-        mbar_expect_tx(y_full + s, C::XB);
-        for (int j = 0; j < C::NB; ++j)
-          tma_load_4d(smem + C::OFF_Y + s * C::YB + j * 16384, &a.tm_y, y_full + s, 64 * j, r0, h, b);
+      if (i >= 1) {
+        const int y = i - 1, s = y & 1;
+        if (y >= 2) wait_inline(y_free + s, ((y >> 1) - 1) & 1, a.status, 202);
+        if (leader) {
+          mbar_expect_tx(y_full + s, C::XB);
+          for (int j = 0; j < C::NB; ++j)
+            tma_load_4d(smem + C::OFF_Y + s * C::YB + j * 16384, &a.tm_y, y_full + s, 64 * j, (t_lo + y) * TR, h, b);
+        }
       }
     }
     __syncwarp();
@@ -254,8 +285,8 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
     const uint64_t dA = smem_desc_sw128(smem_u32(smem + C::OFF_A), 16384, 1024);
     auto summary = [&](int u) {
       const int s = u & 1;
-      mbar_wait(a_full + s, (u >> 1) & 1, a.status, 203);
-      mbar_wait(y_full + s, (u >> 1) & 1, a.status, 204);
+      wait_inline(a_full + s, (u >> 1) & 1, a.status, 203);
+      wait_inline(y_full + s, (u >> 1) & 1, a.status, 204);
       tc_fence_after_sync();
       if (leader) {
         tma_store_3d(&a.tm_f, smem + C::OFF_A + s * 32768, 128 * fb, (t_lo + u) * TR, bh);
@@ -275,11 +306,11 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
       }
       __syncwarp();
     };
-    mbar_wait(bar_w, 0, a.status, 205);
+    wait_inline(bar_w, 0, a.status, 205);
     for (int i = 0; i < nt; ++i) {
       const int s = i & 1, xs = i % C::XD;
-      mbar_wait(x_full + xs, (i / C::XD) & 1, a.status, 206);
-      if (i >= 2) mbar_wait(u_free + s, ((i >> 1) - 1) & 1, a.status, 207);
+      wait_inline(x_full + xs, (i / C::XD) & 1, a.status, 206);
+      if (i >= 2) wait_inline(u_free + s, ((i >> 1) - 1) & 1, a.status, 207);
       tc_fence_after_sync();
       if (leader) {
 #pragma unroll
@@ -418,7 +449,7 @@ struct WinArgs {
   CUtensorMap tm_x, tm_y, tm_xo, tm_yo;   // own side (128 rows), other side (64 rows)
   Geom g;
   const float *n2, *delta;                // (BH, Tp)
-  float* part;                            // (BH, rows, D)
+  float* part;                            // (tiles, D / 4, 128 rows) float4
   int* status;
   int Tp;
   float tau;
@@ -468,7 +499,7 @@ __global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constan
       const RowTile t = row_tile<SIDE, 64>(a.g, tile, false);
       if (t.n == 0) continue;
       const int buf = ne & 1;
-      if (ne >= 2) mbar_wait(bars + C::XY_FREE + buf, ((ne >> 1) - 1) & 1, a.status, 221);
+      if (ne >= 2) wait_inline(bars + C::XY_FREE + buf, ((ne >> 1) - 1) & 1, a.status, 221);
       if (leader) {
         mbar_expect_tx(bars + C::XY_FULL + buf, 2 * C::TB);
         for (int j = 0; j < C::NB; ++j) {
@@ -479,7 +510,7 @@ __global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constan
       ++ne;
       for (int s = 0; s < t.n; ++s, ++n) {
         const int slot = n % C::NS;
-        if (n >= C::NS) mbar_wait(bars + C::R_FREE + slot, ((n / C::NS) - 1) & 1, a.status, 222);
+        if (n >= C::NS) wait_inline(bars + C::R_FREE + slot, ((n / C::NS) - 1) & 1, a.status, 222);
         if (leader) {
           uint8_t* dst = smem + C::OFF_RING + slot * C::SLOT;
           mbar_expect_tx(bars + C::R_FULL + slot, C::SLOT);
@@ -521,8 +552,8 @@ __global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constan
     auto issue_st = [&]() {
       if (st.tile >= a.g.ntiles) return;
       const int buf = gs & 1, xb = st.ne & 1, slot = gs % C::NS;
-      if (st.s == 0) mbar_wait(bars + C::XY_FULL + xb, (st.ne >> 1) & 1, a.status, 223);
-      mbar_wait(bars + C::R_FULL + slot, (gs / C::NS) & 1, a.status, 224);
+      if (st.s == 0) wait_inline(bars + C::XY_FULL + xb, (st.ne >> 1) & 1, a.status, 223);
+      wait_inline(bars + C::R_FULL + slot, (gs / C::NS) & 1, a.status, 224);
       tc_fence_after_sync();
       if (leader) {
         const uint64_t x = dX + (uint64_t)(xb * (C::TB >> 4)), y = dY + (uint64_t)(xb * (C::TB >> 4));
@@ -545,8 +576,8 @@ __global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constan
     issue_st();
     for (int g = 0; dx.tile < a.g.ntiles; ++g, next(dx)) {
       const int buf = g & 1, db = dx.ne & 1, slot = g % C::NS;
-      mbar_wait(bars + C::DS_DONE + buf, (g >> 1) & 1, a.status, 225);
-      if (dx.s == 0 && dx.ne >= 2) mbar_wait(bars + C::DX_FREE + db, ((dx.ne >> 1) - 1) & 1, a.status, 226);
+      wait_inline(bars + C::DS_DONE + buf, (g >> 1) & 1, a.status, 225);
+      if (dx.s == 0 && dx.ne >= 2) wait_inline(bars + C::DX_FREE + db, ((dx.ne >> 1) - 1) & 1, a.status, 226);
       tc_fence_after_sync();
       if (leader) {
 #pragma unroll
@@ -641,14 +672,12 @@ __global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constan
 #pragma unroll
         for (int j = 0; j < NC; ++j) v[j] = 0u;
       }
-      if (row < t.nr) {
-        const int rows = SIDE == QUERIES ? a.g.T : a.g.S;
-        float4* dst = reinterpret_cast<float4*>(a.part + ((int64_t)t.bh * rows + r) * D + c);
+      // part: per tile (D / 4 groups of four columns) x 128 rows, so that a warp writes whole lines
+      float4* dst = reinterpret_cast<float4*>(a.part) + ((int64_t)tile * (D / 4) + c / 4) * TR + row;
 #pragma unroll
-        for (int j = 0; j < NC / 4; ++j)
-          dst[j] = make_float4(a.tau * __uint_as_float(v[4 * j]), a.tau * __uint_as_float(v[4 * j + 1]),
-                               a.tau * __uint_as_float(v[4 * j + 2]), a.tau * __uint_as_float(v[4 * j + 3]));
-      }
+      for (int j = 0; j < NC / 4; ++j)
+        dst[j * TR] = make_float4(a.tau * __uint_as_float(v[4 * j]), a.tau * __uint_as_float(v[4 * j + 1]),
+                                  a.tau * __uint_as_float(v[4 * j + 2]), a.tau * __uint_as_float(v[4 * j + 3]));
     }
   }
   tc_fence_before_sync();
@@ -662,25 +691,26 @@ __global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constan
 // ---------------------------------------------------------------------------
 // Low-rank part of dq or dk, and the sum of both.
 struct LowArgs {
-  CUtensorMap tm_y, tm_yo, tm_fo, tm_sum, tm_hi, tm_lo;
+  CUtensorMap tm_y, tm_yo, tm_fo, tm_sum, tm_hi, tm_lo, tm_f, tm_x, tm_dx;
   Geom g;
-  const __nv_bfloat16* f;                  // own features (BH, rows, m)
   const float* sum1;                       // (BH, m): extra column of the other side's summary
   const float* delta;                      // (BH, Tp)
-  const float* part;                       // (BH, rows, D): exact part
-  const __nv_bfloat16* x; int64_t xb, xr, xh;
-  __nv_bfloat16* dx; int64_t ob, orow, oh;
+  const float* part;                       // (tiles, D / 4, 128 rows) float4: exact part
   int* status;
   int Tp, whole;
   float tau;
 };
 
+// A unit is a (tile, pass of 256 features); head dim 128 takes two passes.  Ring slots of a unit, in order: one per
+// column step (256 features, then Y'), the own features of the unit's two blocks of 128 ("+", "-"), and in a tile's
+// last unit its X rows, over which dx is staged for a bulk store.
 template <int D>
 struct LowCfg {
   static constexpr int NB = D / 64, M = 4 * D, PASS = M / 256, NS = D == 64 ? 3 : 2;
+  static constexpr int AHEAD = NS - 1;                   // G products of the next unit issued before this one's end
   static constexpr uint32_t TB = NB * 16384;             // own Y tile
   static constexpr uint32_t AUX = 512 * D;               // 256 features x D of the summary; 2 terms x 128 x D of Wt
-  static constexpr uint32_t SLOT = 32768 + NB * 8192;    // 64 columns: 256 features, then Y'
+  static constexpr uint32_t SLOT = 32768 + NB * 8192;
   static constexpr uint32_t OFF_Y = 0, OFF_SUM = 2 * TB;
   static constexpr uint32_t OFF_W = D == 64 ? OFF_SUM + AUX : OFF_SUM;   // head dim 128: one buffer for both, in turn
   static constexpr uint32_t OFF_RING = OFF_W + AUX, OFF_H = OFF_RING + NS * SLOT, OFF_BAR = OFF_H + 1024;
@@ -717,43 +747,47 @@ __global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_consta
   if (tid == 0 && *tmem_slot != 0) atomicCAS(a.status, 0, 241);
   const int step = gridDim.x;
   const bool whole = a.whole != 0;
-  // number of tiles of this CTA; a unit is a (tile, pass of 256 features)
   const int n_it = (a.g.ntiles - (int)blockIdx.x + step - 1) / step, n_u = n_it * C::PASS;
 
   if (warp == C::W_LOAD) {
     const bool leader = elect_one();
     int n = 0;
+    // the next ring slot, free; its barrier expects `bytes`
+    auto slot_for = [&](uint32_t bytes, uint64_t** bar) {
+      const int slot = n % C::NS;
+      if (n >= C::NS) wait_inline(bars + C::R_FREE + slot, ((n / C::NS) - 1) & 1, a.status, 262);
+      *bar = bars + C::R_FULL + slot;
+      if (leader) mbar_expect_tx(*bar, bytes);
+      ++n;
+      return smem + C::OFF_RING + slot * C::SLOT;
+    };
     for (int u = 0; u < n_u; ++u) {
       const int it = u / C::PASS, pass = u % C::PASS;
       const RowTile t = row_tile<SIDE, 64>(a.g, blockIdx.x + it * step, whole);
+      uint64_t* bar;
+      auto column_step = [&](int s) {
+        uint8_t* dst = slot_for(C::SLOT, &bar);
+        if (leader) {
+          for (int j = 0; j < C::NB; ++j)
+            tma_load_4d(dst + 32768 + j * 8192, &a.tm_yo, bar, 64 * j, t.c0 + 64 * s, t.h, t.b);
+          for (int j = 0; j < 4; ++j) tma_load_3d(dst + j * 8192, &a.tm_fo, bar, 256 * pass + 64 * j, t.c0 + 64 * s, t.bh);
+        }
+      };
       if (pass == 0) {
         const int buf = it & 1;
-        if (it >= 2) mbar_wait(bars + C::Y_FREE + buf, ((it >> 1) - 1) & 1, a.status, 261);
+        if (it >= 2) wait_inline(bars + C::Y_FREE + buf, ((it >> 1) - 1) & 1, a.status, 261);
         if (leader) {
           mbar_expect_tx(bars + C::Y_FULL + buf, C::TB);
           for (int j = 0; j < C::NB; ++j)
             tma_load_4d(smem + C::OFF_Y + buf * C::TB + j * 16384, &a.tm_y, bars + C::Y_FULL + buf, 64 * j, t.r0, t.h, t.b);
         }
       }
-      for (int s = 0; s < t.n; ++s, ++n) {
-        const int slot = n % C::NS;
-        if (n >= C::NS) mbar_wait(bars + C::R_FREE + slot, ((n / C::NS) - 1) & 1, a.status, 262);
-        if (leader) {
-          uint8_t* dst = smem + C::OFF_RING + slot * C::SLOT;
-          mbar_expect_tx(bars + C::R_FULL + slot, C::SLOT);
-          for (int j = 0; j < C::NB; ++j)
-            tma_load_4d(dst + 32768 + j * 8192, &a.tm_yo, bars + C::R_FULL + slot, 64 * j, t.c0 + 64 * s, t.h, t.b);
-          for (int j = 0; j < 4; ++j)
-            tma_load_3d(dst + j * 8192, &a.tm_fo, bars + C::R_FULL + slot, 256 * pass + 64 * j, t.c0 + 64 * s, t.bh);
-        }
-      }
-      // Head dim 64: the summary has a buffer of its own and Wt stays.  Head dim 128: summary and Wt of the pass
+      int s = 0;
+      if (s < t.n) column_step(s++);
+      // Head dim 64: the summary has a buffer of its own and Wt stays.  Head dim 128: summary and Wt of the unit
       // take turns in one buffer (summary -> its product -> Wt -> its product -> next summary).
       if (!whole) {
-        if (u >= 1) {
-          if (D == 64) mbar_wait(bars + C::SUM_FREE, (u - 1) & 1, a.status, 263);
-          else mbar_wait(bars + C::W_FREE, (u - 1) & 1, a.status, 264);
-        }
+        if (u >= 1) wait_inline(bars + (D == 64 ? C::SUM_FREE : C::W_FREE), (u - 1) & 1, a.status, 263);
         if (leader) {
           mbar_expect_tx(bars + C::SUM_FULL, C::AUX);
           for (int j = 0; j < C::NB; ++j)
@@ -762,10 +796,11 @@ __global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_consta
                           256 * pass + 128 * f, t.bh);
         }
       }
+      for (; s < t.n && s < 3; ++s) column_step(s);
       if (D != 64 || u == 0) {
         if (D != 64) {
-          if (!whole) mbar_wait(bars + C::SUM_FREE, u & 1, a.status, 265);
-          else if (u >= 1) mbar_wait(bars + C::W_FREE, (u - 1) & 1, a.status, 266);
+          if (!whole) wait_inline(bars + C::SUM_FREE, u & 1, a.status, 265);
+          else if (u >= 1) wait_inline(bars + C::W_FREE, (u - 1) & 1, a.status, 266);
         }
         if (leader) {
           mbar_expect_tx(bars + C::W_FULL, C::AUX);
@@ -774,6 +809,18 @@ __global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_consta
             tma_load_2d(smem + C::OFF_W + C::AUX / 2 + j * 16384, &a.tm_lo, bars + C::W_FULL, 64 * j, 128 * pass);
           }
         }
+      }
+      for (; s < t.n; ++s) column_step(s);
+      for (int blk = 0; blk < 2; ++blk) {
+        uint8_t* dst = slot_for(32768, &bar);
+        if (leader)
+          for (int j = 0; j < 2; ++j)
+            tma_load_3d(dst + j * 16384, &a.tm_f, bar, 256 * pass + 128 * blk + 64 * j, t.r0, t.bh);
+      }
+      if (pass == C::PASS - 1) {
+        uint8_t* dst = slot_for(C::TB, &bar);
+        if (leader)
+          for (int j = 0; j < C::NB; ++j) tma_load_4d(dst + j * 16384, &a.tm_x, bar, 64 * j, t.r0, t.h, t.b);
       }
     }
     __syncwarp();
@@ -788,11 +835,11 @@ __global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_consta
     const uint64_t dFo = smem_desc_sw128(smem_u32(smem + C::OFF_RING), 8192, 1024);
     const uint64_t dSum = smem_desc_sw128(smem_u32(smem + C::OFF_SUM), 16, 1024);
     const uint64_t dW = smem_desc_sw128(smem_u32(smem + C::OFF_W), 16384, 1024);
-    // G of step s of unit u; gg: its number in the CTA's stream of steps
-    auto issue_t = [&](int u, int s, int gg) {
-      const int it = u / C::PASS, slot = gg % C::NS;
-      if (u % C::PASS == 0 && s == 0) mbar_wait(bars + C::Y_FULL + (it & 1), (it >> 1) & 1, a.status, 267);
-      mbar_wait(bars + C::R_FULL + slot, (gg / C::NS) & 1, a.status, 268);
+    // G of step s of unit u; gg: its number in the CTA's stream of steps, rp: its ring number
+    auto issue_t = [&](int u, int s, int gg, int rp) {
+      const int it = u / C::PASS, slot = rp % C::NS;
+      if (u % C::PASS == 0 && s == 0) wait_inline(bars + C::Y_FULL + (it & 1), (it >> 1) & 1, a.status, 267);
+      wait_inline(bars + C::R_FULL + slot, (rp / C::NS) & 1, a.status, 268);
       tc_fence_after_sync();
       if (leader) {
         const uint64_t y = dY + (uint64_t)((it & 1) * (C::TB >> 4)), o = dYo + (uint64_t)(slot * (C::SLOT >> 4));
@@ -803,57 +850,66 @@ __global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_consta
       }
       __syncwarp();
     };
-    int g0 = 0, n = 0, n_next = 0;
+    int g0 = 0, r0 = 0, n = 0, n_next = 0;   // numbers of the unit's first step and first ring slot; its steps
     if (n_u > 0) {
       n_next = row_tile<SIDE, 64>(a.g, blockIdx.x, whole).n;
-      for (int s = 0; s < 2 && s < n_next; ++s) issue_t(0, s, s);
+      for (int s = 0; s < C::AHEAD && s < n_next; ++s) issue_t(0, s, s, s);
     }
     for (int u = 0; u < n_u; ++u) {
       const int it = u / C::PASS, pass = u % C::PASS;
       n = n_next;
-      for (int s = 0; s < n; ++s) {
-        const int gg = g0 + s, slot = gg % C::NS;
-        mbar_wait(bars + C::G_DONE + (gg & 1), (gg >> 1) & 1, a.status, 269);
-        tc_fence_after_sync();
-        if (leader) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_ts(tb + C::T_DF, tb + C::T_G + 64 * (gg & 1) + packed(k),
-                   dFo + (uint64_t)(slot * (C::SLOT >> 4) + k * 128), id_df, s > 0 || k > 0);
-          mma_commit(bars + C::R_FREE + slot);
-        }
-        __syncwarp();
-        if (s + 2 < n) issue_t(u, s + 2, gg + 2);
-      }
+      // (the previous tile's X rows had the ring slot before: see below)
+      if (u >= 1 && pass == 0) wait_inline(bars + C::R_FULL + (r0 - 1) % C::NS, ((r0 - 1) / C::NS) & 1, a.status, 294);
+      for (int s = C::AHEAD; s < 2 && s < n; ++s) issue_t(u, s, g0 + s, r0 + s);
       // without steps nobody has waited for the Y tile yet
-      if (n == 0 && pass == 0) mbar_wait(bars + C::Y_FULL + (it & 1), (it >> 1) & 1, a.status, 270);
+      if (n == 0 && pass == 0) wait_inline(bars + C::Y_FULL + (it & 1), (it >> 1) & 1, a.status, 270);
       if (!whole) {
-        mbar_wait(bars + C::SUM_FULL, u & 1, a.status, 271);
+        wait_inline(bars + C::SUM_FULL, u & 1, a.status, 271);
         tc_fence_after_sync();
         if (leader) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
             mma_ss(tb + C::T_DF, dY + (uint64_t)((it & 1) * (C::TB >> 4)) + kmajor(k, 16384), dSum + kmajor(k, 32768),
-                   id_sum, n > 0 || k > 0);
+                   id_sum, k > 0);
           mma_commit(bars + C::SUM_FREE);
         }
         __syncwarp();
+      }
+      for (int s = 0; s < n; ++s) {
+        const int gg = g0 + s, slot = (r0 + s) % C::NS;
+        wait_inline(bars + C::G_DONE + (gg & 1), (gg >> 1) & 1, a.status, 269);
+        tc_fence_after_sync();
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_ts(tb + C::T_DF, tb + C::T_G + 64 * (gg & 1) + packed(k),
+                   dFo + (uint64_t)(slot * (C::SLOT >> 4) + k * 128), id_df, !whole || s > 0 || k > 0);
+          mma_commit(bars + C::R_FREE + slot);
+        }
+        __syncwarp();
+        if (s + 2 < n) issue_t(u, s + 2, gg + 2, r0 + s + 2);
       }
       if (leader) {
         if (pass == C::PASS - 1) mma_commit(bars + C::Y_FREE + (it & 1));
         mma_commit(bars + C::DF_FULL);
       }
       __syncwarp();
-      // the next unit's first two G run while this unit's df turns into du
+      // The next unit's first G products run while this unit's df turns into du.  (Their ring slots are those of the
+      // own features, which the compute warps free by themselves; never that of the X rows, freed behind DX_FULL.)
+      // A wait tells phases apart by parity alone, so this warp has to have seen every use of a slot, those that it
+      // does not read among them.
+      for (int blk = 0; blk < 2; ++blk)
+        wait_inline(bars + C::R_FULL + (r0 + n + blk) % C::NS, ((r0 + n + blk) / C::NS) & 1, a.status, 295);
       g0 += n;
+      r0 += n + (pass == C::PASS - 1 ? 3 : 2);
       if (u + 1 < n_u) {
         if (pass == C::PASS - 1) n_next = row_tile<SIDE, 64>(a.g, blockIdx.x + (it + 1) * step, whole).n;
-        for (int s = 0; s < 2 && s < n_next; ++s) issue_t(u + 1, s, g0 + s);
+        for (int s = 0; s < C::AHEAD && s < n_next; ++s) issue_t(u + 1, s, g0 + s, r0 + s);
       }
-      mbar_wait(bars + C::DU_DONE, u & 1, a.status, 272);
-      if (pass == 0 && it >= 1) mbar_wait(bars + C::DX_FREE, (it - 1) & 1, a.status, 273);
-      if (D != 64) mbar_wait(bars + C::W_FULL, u & 1, a.status, 274);
-      else if (u == 0) mbar_wait(bars + C::W_FULL, 0, a.status, 275);
+      wait_inline(bars + C::DU_DONE, u & 1, a.status, 272);
+      if (pass == 0 && it >= 1) wait_inline(bars + C::DX_FREE, (it - 1) & 1, a.status, 273);
+      if (D != 64) wait_inline(bars + C::W_FULL, u & 1, a.status, 274);
+      else if (u == 0) wait_inline(bars + C::W_FULL, 0, a.status, 275);
       tc_fence_after_sync();
       if (leader) {
 #pragma unroll
@@ -871,18 +927,17 @@ __global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_consta
     const int qd = warp & 3, cq = warp >> 2;
     const int row = qd * 32 + lane;
     const uint32_t lane_base = tb + ((uint32_t)(qd * 32) << 16);
-    const int rows = SIDE == QUERIES ? a.g.T : a.g.S;
     const float sign = whole ? 1.f : -1.f;   // the window's G enters with a minus
-    int gg = 0;
+    int gg = 0, rp = 0;
     float hs = 0.f;
     for (int u = 0; u < n_u; ++u) {
       const int it = u / C::PASS, pass = u % C::PASS;
-      const RowTile t = row_tile<SIDE, 64>(a.g, blockIdx.x + it * step, whole);
+      const int tile = blockIdx.x + it * step;
+      const RowTile t = row_tile<SIDE, 64>(a.g, tile, whole);
       const int r = t.r0 + row;
-      const bool mine = row < t.nr;
       const float* dl = a.delta + (int64_t)t.bh * a.Tp;
       const float rd = SIDE == QUERIES ? __ldg(dl + r) : 0.f;
-      for (int s = 0; s < t.n; ++s, ++gg) {
+      for (int s = 0; s < t.n; ++s, ++gg, ++rp) {
         const int c = t.c0 + 64 * s + 32 * cq;
         const uint32_t vis = seen<SIDE>(a.g, t, r, c, whole);
         const uint32_t tg = lane_base + C::T_G + 64 * (gg & 1) + 32 * cq;
@@ -918,13 +973,15 @@ __global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_consta
       const bool none = whole && t.n == 0;
       const float d1 = whole ? 0.f : (SIDE == QUERIES ? rd : 1.f);
       if (pass == 0) hs = 0.f;
-      const __nv_bfloat16* frow = a.f + ((int64_t)t.bh * rows + (mine ? r : t.r0)) * C::M + 256 * pass + 32 * cq;
       const float* s1 = a.sum1 + (int64_t)t.bh * C::M + 256 * pass + 32 * cq;
       mbar_wait(bars + C::DF_FULL, u & 1, a.status, 277);
       tc_fence_after_sync();
 #pragma unroll 1
       for (int blk = 0; blk < 2; ++blk) {
+        const int slot = (rp + blk) % C::NS;
         const uint32_t td = lane_base + C::T_DF + 128 * blk + 32 * cq;
+        const uint8_t* line = smem + C::OFF_RING + slot * C::SLOT + row * 128;
+        mbar_wait(bars + C::R_FULL + slot, ((rp + blk) / C::NS) & 1, a.status, 279);
         uint32_t o[16];
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
@@ -934,8 +991,9 @@ __global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_consta
           uint4 fp[2], fm[2];
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            fp[q] = __ldg(reinterpret_cast<const uint4*>(frow + 128 * blk + 16 * hf) + q);
-            fm[q] = __ldg(reinterpret_cast<const uint4*>(frow + 128 * blk + 64 + 16 * hf) + q);
+            const uint32_t at = (uint32_t)(((4 * cq + 2 * hf + q) ^ (row & 7)) << 4);
+            fp[q] = *reinterpret_cast<const uint4*>(line + at);
+            fm[q] = *reinterpret_cast<const uint4*>(line + 16384 + at);
           }
           tmem_ld_wait();
 #pragma unroll
@@ -957,43 +1015,60 @@ __global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_consta
       tmem_st_wait();
       tc_fence_before_sync();
       warp_arrive(bars + C::DU_DONE, lane);
+      if (pass == C::PASS - 1) s_h[cq * 128 + row] = hs;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (tid < 2) mbar_arrive(bars + C::R_FREE + (rp + tid) % C::NS);   // the own features have been read
+      rp += 2;
       if (pass == C::PASS - 1) {
-        s_h[cq * 128 + row] = hs;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const int slot = rp % C::NS;
+        uint8_t* xs = smem + C::OFF_RING + slot * C::SLOT;
         const float hsum = a.tau * (s_h[row] + s_h[128 + row]);
+        const float4* part = reinterpret_cast<const float4*>(a.part) + (int64_t)tile * (D / 4) * TR + row;
+        float4 e[D / 8];
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) e[j] = __ldg(part + (D / 8 * cq + j) * TR);
+        mbar_wait(bars + C::R_FULL + slot, (rp / C::NS) & 1, a.status, 280);
         mbar_wait(bars + C::DX_FULL, it & 1, a.status, 278);
         tc_fence_after_sync();
-        const __nv_bfloat16* x = a.x + t.b * a.xb + t.h * a.xh + (int64_t)r * a.xr;
-        __nv_bfloat16* dx = a.dx + t.b * a.ob + t.h * a.oh + (int64_t)r * a.orow;
-        const float* part = a.part + ((int64_t)t.bh * rows + r) * D;
 #pragma unroll
         for (int q = 0; q < D / 32; ++q) {
           const int c = (D / 2) * cq + 16 * q;
           uint32_t v[16];
           tmem_ld16(lane_base + C::T_DX + c, v);
           tmem_ld_wait();
-          if (mine) {
-            uint4 xv[2];
-            xv[0] = __ldg(reinterpret_cast<const uint4*>(x + c));
-            xv[1] = __ldg(reinterpret_cast<const uint4*>(x + c) + 1);
-            uint32_t o[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const uint32_t w = (&xv[j >> 2].x)[j & 3];
-              const float2 e = __ldg(reinterpret_cast<const float2*>(part + c) + j);
-              o[j] = pack_bf16(fmaf(-hsum, bf16_lo(w), __uint_as_float(v[2 * j]) + e.x),
-                               fmaf(-hsum, bf16_hi(w), __uint_as_float(v[2 * j + 1]) + e.y));
-            }
-            reinterpret_cast<uint4*>(dx + c)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            reinterpret_cast<uint4*>(dx + c)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+          for (int j = 0; j < 2; ++j) {
+            // eight entries: 16 bytes of the row's swizzled line, dx over x
+            uint4* at = reinterpret_cast<uint4*>(xs + (c >> 6) * 16384 + row * 128 + ((((c & 63) >> 3) + j) ^ (row & 7)) * 16);
+            const uint4 xv = *at;
+            const float4 e0 = e[4 * q + 2 * j], e1 = e[4 * q + 2 * j + 1];
+            uint4 o;
+            o.x = pack_bf16(fmaf(-hsum, bf16_lo(xv.x), __uint_as_float(v[8 * j]) + e0.x),
+                            fmaf(-hsum, bf16_hi(xv.x), __uint_as_float(v[8 * j + 1]) + e0.y));
+            o.y = pack_bf16(fmaf(-hsum, bf16_lo(xv.y), __uint_as_float(v[8 * j + 2]) + e0.z),
+                            fmaf(-hsum, bf16_hi(xv.y), __uint_as_float(v[8 * j + 3]) + e0.w));
+            o.z = pack_bf16(fmaf(-hsum, bf16_lo(xv.z), __uint_as_float(v[8 * j + 4]) + e1.x),
+                            fmaf(-hsum, bf16_hi(xv.z), __uint_as_float(v[8 * j + 5]) + e1.y));
+            o.w = pack_bf16(fmaf(-hsum, bf16_lo(xv.w), __uint_as_float(v[8 * j + 6]) + e1.z),
+                            fmaf(-hsum, bf16_hi(xv.w), __uint_as_float(v[8 * j + 7]) + e1.w));
+            *at = o;
           }
         }
         tc_fence_before_sync();
         warp_arrive(bars + C::DX_FREE, lane);
-        // s_h may be written again once everyone has read it: the next write is behind another barrier of this kind
+        fence_async_smem();
         asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (tid == 0) {
+          // rows past the end are clipped by the tensor map
+          for (int j = 0; j < C::NB; ++j) tma_store_4d(&a.tm_dx, xs + j * 16384, 64 * j, t.r0, t.h, t.b);
+          tma_store_commit();
+          tma_store_wait_read0();
+          mbar_arrive(bars + C::R_FREE + slot);
+        }
+        ++rp;
       }
     }
+    if (tid == 0) tma_store_wait_all();
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -1099,14 +1174,14 @@ struct ValLoader {
 
   __device__ uint8_t* piece() {
     const int slot = n % C::NS;
-    if (n >= C::NS) mbar_wait(bars + C::R_FREE + slot, ((n / C::NS) - 1) & 1, a.status, 281);
+    if (n >= C::NS) wait_inline(bars + C::R_FREE + slot, ((n / C::NS) - 1) & 1, a.status, 281);
     if (leader) mbar_expect_tx(bars + C::R_FULL + slot, 16384);
     return smem + C::OFF_RING + slot * 16384;
   }
   __device__ uint64_t* full() { return bars + C::R_FULL + (n++ % C::NS); }
   __device__ void phi(const RowTile& t, int it) {
     const int buf = it % C::KBUF;
-    if (it >= C::KBUF) mbar_wait(bars + C::F_FREE + buf, ((it / C::KBUF) - 1) & 1, a.status, 282);
+    if (it >= C::KBUF) wait_inline(bars + C::F_FREE + buf, ((it / C::KBUF) - 1) & 1, a.status, 282);
     if (leader) {
       mbar_expect_tx(bars + C::F_FULL + buf, C::FB);
       for (int j = 0; j < C::M / 64; ++j)
@@ -1117,7 +1192,7 @@ struct ValLoader {
   __device__ void score(const RowTile& t, int s, int ke, int) {
     if (s == 0) {
       const int buf = ke % C::KBUF;
-      if (ke >= C::KBUF) mbar_wait(bars + C::K_FREE + buf, ((ke / C::KBUF) - 1) & 1, a.status, 283);
+      if (ke >= C::KBUF) wait_inline(bars + C::K_FREE + buf, ((ke / C::KBUF) - 1) & 1, a.status, 283);
       if (leader) {
         mbar_expect_tx(bars + C::K_FULL + buf, C::KB);
         for (int j = 0; j < C::NB; ++j)
@@ -1174,14 +1249,14 @@ struct ValIssuer {
 
   __device__ int take() {          // the next ring piece, landed
     const int slot = n % C::NS;
-    mbar_wait(bars + C::R_FULL + slot, (n / C::NS) & 1, a.status, 284);
+    wait_inline(bars + C::R_FULL + slot, (n / C::NS) & 1, a.status, 284);
     ++n;
     tc_fence_after_sync();
     return slot;
   }
   __device__ void score(const RowTile& t, int s, int ke, int g) {
     const int kb = ke % C::KBUF;
-    if (s == 0) mbar_wait(bars + C::K_FULL + kb, (ke / C::KBUF) & 1, a.status, 285);
+    if (s == 0) wait_inline(bars + C::K_FULL + kb, (ke / C::KBUF) & 1, a.status, 285);
     constexpr uint32_t id = idesc_bf16(128, 128, false, false);
     for (int j = 0; j < C::NB; ++j) {
       const int slot = take();
@@ -1201,10 +1276,10 @@ struct ValIssuer {
     __syncwarp();
   }
   __device__ void begin(const RowTile&, int it) {
-    mbar_wait(bars + C::F_FULL + it % C::KBUF, (it / C::KBUF) & 1, a.status, 286);
+    wait_inline(bars + C::F_FULL + it % C::KBUF, (it / C::KBUF) & 1, a.status, 286);
   }
   __device__ void minus(const RowTile&, int it, int, int g) {
-    mbar_wait(bars + C::E_DONE + g % 3, (g / 3) & 1, a.status, 287);
+    wait_inline(bars + C::E_DONE + g % 3, (g / 3) & 1, a.status, 287);
     constexpr uint32_t id = idesc_bf16(128, 128, false, false) | (1u << 13);   // bit 13 negates A
     const int fb = it % C::KBUF;
     for (int j = 0; j < C::M / 64; ++j) {
@@ -1222,8 +1297,8 @@ struct ValIssuer {
     __syncwarp();
   }
   __device__ void value(const RowTile&, int it, int, int g, bool first, bool last) {
-    mbar_wait(bars + C::D_DONE + g % 3, (g / 3) & 1, a.status, 288);
-    if (first && it >= 1) mbar_wait(bars + C::DV_FREE, (it - 1) & 1, a.status, 289);
+    wait_inline(bars + C::D_DONE + g % 3, (g / 3) & 1, a.status, 288);
+    if (first && it >= 1) wait_inline(bars + C::DV_FREE, (it - 1) & 1, a.status, 289);
     constexpr uint32_t id = idesc_bf16(128, 64, false, true);
     for (int j = 0; j < C::NB; ++j) {
       const int slot = take();
@@ -1239,7 +1314,7 @@ struct ValIssuer {
     __syncwarp();
   }
   __device__ void rank(const RowTile&, int it, bool first, bool alone) {
-    if (first && it >= 1) mbar_wait(bars + C::DV_FREE, (it - 1) & 1, a.status, 290);
+    if (first && it >= 1) wait_inline(bars + C::DV_FREE, (it - 1) & 1, a.status, 290);
     constexpr uint32_t id = idesc_bf16(128, 64, false, true);
     const int fb = it % C::KBUF;
     for (int f = 0; f < C::M / 128; ++f)
@@ -1505,17 +1580,14 @@ cudaError_t launch_side(const Host& h, void* dx, int64_t ob, int64_t orow, int64
   if (!h.map_y(&a.tm_y, SIDE, 128) || !h.map_y(&a.tm_yo, OTHER, 64) ||
       !map_rows(&a.tm_fo, h.at<void>(h.ws.feat[OTHER]), C::M, h.side[OTHER].rows, BH, 64) ||
       !map_rows(&a.tm_sum, h.at<void>(h.ws.sum[OTHER]), D, C::M, BH, 128) ||
-      !map_w(&a.tm_hi, h.at<void>(h.ws.fwd.phiq), D, 128) || !map_w(&a.tm_lo, h.at<void>(h.ws.wlo), D, 128))
+      !map_w(&a.tm_hi, h.at<void>(h.ws.fwd.phiq), D, 128) || !map_w(&a.tm_lo, h.at<void>(h.ws.wlo), D, 128) ||
+      !map_rows(&a.tm_f, h.at<void>(h.ws.feat[SIDE]), C::M, h.side[SIDE].rows, BH, 128) || !h.map_x(&a.tm_x, SIDE, 128) ||
+      !map_bthe(&a.tm_dx, dx, h.p.B, h.side[SIDE].rows, h.p.H, D, ob, orow, oh, 128))
     return cudaErrorInvalidValue;
   a.g = h.geom(SIDE);
-  a.f = h.at<__nv_bfloat16>(h.ws.feat[SIDE]);
   a.sum1 = h.at<float>(h.ws.sum1[OTHER]);
   a.delta = h.at<float>(h.ws.delta);
   a.part = h.at<float>(h.ws.part);
-  a.x = static_cast<const __nv_bfloat16*>(h.side[SIDE].x);
-  a.xb = h.side[SIDE].xb; a.xr = h.side[SIDE].xr; a.xh = h.side[SIDE].xh;
-  a.dx = static_cast<__nv_bfloat16*>(dx);
-  a.ob = ob; a.orow = orow; a.oh = oh;
   a.status = h.at<int>(h.ws.fwd.status);
   a.Tp = h.ws.Tp;
   // Few columns: the sum over those outside the window instead of all - inside (accuracy, see the top).  It visits
@@ -1539,7 +1611,7 @@ cudaError_t backward(const Host& h) {
     return e;
   if ((e = tc_key_logscale_bound(p, h.ws.fwd, h.base, beta, h.st, true)) != cudaSuccess) return e;
   const int64_t lanes = (int64_t)BH * h.ws.Tp * (D / 8);
-  bwd_rows_kernel<D><<<(unsigned)div_up(lanes, 256), 256, 0, h.st>>>(
+  bwd_rows_kernel<D><<<(unsigned)div_up(lanes, 1024), 256, 0, h.st>>>(
       static_cast<const __nv_bfloat16*>(p.out), p.o_stride_b, p.o_stride_t, p.o_stride_h,
       static_cast<const __nv_bfloat16*>(g.dout), g.do_stride_b, g.do_stride_t, g.do_stride_h, g.row_stats, p.B, p.H, p.T,
       h.ws.Tp, h.at<float>(h.ws.n2), h.at<float>(h.ws.delta));
@@ -1609,17 +1681,25 @@ void tc_plan_backward(const SblParams& p, TcBwdWorkspace* ws) {
   for (int s = 0; s < 2; ++s) {
     ws->sum[s] = take(BH * m * D * 2);
     ws->sum1[s] = take(BH * m * 4);
-    // about two waves of CTAs over (b*h, blocks of 128 features)
+    // one CTA per SM at a time: the fewest rounds of tiles over whole waves of CTAs; a CTA's prologue and its partial
+    // summary cost about as much as three tiles
     const int ntiles = (int)div_up(s == QUERIES ? p.T : p.S, TR);
     const size_t units = BH * (m / 128);
-    int ns = (int)((296 + units / 2) / units);
-    ns = ns < 1 ? 1 : ns;
-    ws->nsplit[s] = ns > ntiles ? ntiles : ns;
+    int best = 1;
+    int64_t least = INT64_MAX;
+    for (int ns = 1; ns <= 16 && ns <= ntiles; ++ns) {
+      const int64_t cost = div_up((int64_t)units * ns, 148) * (div_up(ntiles, ns) + 3);
+      if (cost < least) {
+        least = cost;
+        best = ns;
+      }
+    }
+    ws->nsplit[s] = best;
     const size_t bytes = BH * ws->nsplit[s] * m * (D + 4) * 4;
     partial = bytes > partial ? bytes : partial;
   }
   ws->partial = take(partial);
-  ws->part = take(BH * (T > S ? T : S) * D * 4);
+  ws->part = take(BH * div_up(T > S ? T : S, TR) * TR * D * 4);
   f.total = off;
 }
 
