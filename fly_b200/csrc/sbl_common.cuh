@@ -106,9 +106,11 @@ struct TcBwdWorkspace {
   size_t wlo;               // what is left of Wt, in bf16
   size_t n2, delta;         // (BH,Tp)
   size_t feat[2];           // psi (BH,T,m), phi (BH,S,m) bf16
-  size_t sum[2], sum1[2];   // (BH,m,D) bf16, (BH,m) fp32
+  size_t sum[2], sum_lo[2]; // (BH,m,D): two bf16 terms of the summary
+  size_t sum1[2];           // (BH,m) fp32: its extra column
+  size_t off[2];            // (BH, rows padded to tiles of 128): exponent offsets of the features
   size_t partial;           // split partials of one side's summary
-  size_t part;              // (BH,max(T,S),D) fp32: exact part of dq or dk
+  size_t part;              // head dim 128: exact part of dq or dk, (tiles, D/4, 128 rows) float4
   int Tp, nsplit[2];
 };
 void tc_plan_backward(const SblParams& p, TcBwdWorkspace* ws);

@@ -8,19 +8,19 @@
 //             phi (keys) or psi (queries, over the row's normaliser) -> bf16 to the
 //             workspace, and the summary phi^T [V | 1] or psi^T [dout | delta]
 //   combine   sums the splits -> summary in bf16, its extra column in fp32
-//   window    exact part of dq or dk: S = X X'^T, G = Y Y'^T, p (G - delta) -> bf16,
+//   window    (head dim 128) exact part of dq or dk: S = X X'^T, G = Y Y'^T, p (G - delta) -> bf16,
 //             dx += (p g) X', over the 64-column steps of the window -> fp32
 //   dvalue    S = K Q^T -> p, minus phi psi^T (same buffer, A operand negated),
 //             packed, dv += (p - a) dout; dv += phi QG
-//   lowrank   G = Y Y'^T - delta -> bf16, df -= G f' over the window (256 features at
-//             a time in tensor memory), df += Y summary^T; du = (f df)_+ - (f df)_-,
-//             dx += du Wt; adds the exact part, writes dq or dk
+//   grad      G = Y Y'^T - delta -> bf16, df -= G f' over the window (256 features at a time in tensor
+//             memory), df += Y summary^T; U = X Wt^T, du = (f df)_+ - (f df)_-, dx += du Wt; writes dq or dk.
+//             Head dim 64: the exact part too (S beside G, dx += (p g) X'); 128: adds the window kernel's
 //
 // Numerics.  Products take bf16 operands and accumulate in fp32.  Rounded to bf16
-// (half a step, 2^-9 on average): features, summaries, g, p g, p - a, du.  The
-// projection is carried as two bf16 terms (16 bits of mantissa): rounded to one,
-// it alone was half of the error of dq and dk (U enters an exponential, and the
-// same rounding comes back with du Wt).
+// (half a step, 2^-9 on average): phi and psi as operands, g, p g, p - a.  Carried
+// as two bf16 terms (16 bits): the projection, the summaries and du -- each alone
+// would add as much to the error of dq and dk as the features do.  The own
+// features of a row are formed again in fp32 for du instead of being read back.
 //
 // Where a tile's columns are few (`complement`), df is summed over the columns
 // OUTSIDE the window directly instead of all - inside: a short sequence lies
@@ -179,6 +179,7 @@ struct FeatArgs {
   CUtensorMap tm_x, tm_y, tm_hi, tm_lo, tm_f;
   const int64_t* lengths;
   const float *beta, *n2, *delta;   // (BH); (BH, Tp)
+  float* off;                       // (BH, rows padded to tiles): exponent offset (base 2) of every row, -inf if padding
   float* partial;                   // (BH, nsplit, m, D + 4)
   int* status;
   int H, rows, Tp, nsplit;
@@ -357,6 +358,7 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
         off = (-g - a.half_log_m + beta) * kLog2e - __ldg(a.n2 + (int64_t)bh * a.Tp + r);
         dl = __ldg(a.delta + (int64_t)bh * a.Tp + r);
       }
+      if (fb == 0 && cq == 0) a.off[((int64_t)bh * ntiles + t_lo + i) * TR + row] = live ? off : -INFINITY;
       mbar_wait(u_full + s, (i >> 1) & 1, a.status, 209);   // U computed: the X tile has been read too
       tc_fence_after_sync();
       warp_arrive(x_free + xs, lane);
@@ -420,10 +422,10 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
   }
 }
 
-// summary (BH, m, D) bf16 and its extra column (BH, m) fp32 = sums over the splits
+// summary (BH, m, D) in two bf16 terms and its extra column (BH, m) fp32 = sums over the splits
 template <int D>
 __global__ void __launch_bounds__(256) bwd_combine_kernel(const float* partial, int nsplit, int64_t rows, int m,
-                                                          __nv_bfloat16* sum, float* sum1) {
+                                                          __nv_bfloat16* sum, __nv_bfloat16* sum_lo, float* sum1) {
   constexpr int G = D / 4 + 1;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * G) return;
@@ -439,8 +441,14 @@ __global__ void __launch_bounds__(256) bwd_combine_kernel(const float* partial, 
       v.x += *p;
     }
   }
-  if (g < D / 4) *reinterpret_cast<uint2*>(sum + row * D + 4 * g) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-  else sum1[row] = v.x;
+  if (g < D / 4) {
+    const uint2 hi = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+    *reinterpret_cast<uint2*>(sum + row * D + 4 * g) = hi;
+    *reinterpret_cast<uint2*>(sum_lo + row * D + 4 * g) =
+        make_uint2(pack_bf16(v.x - bf16_lo(hi.x), v.y - bf16_hi(hi.x)), pack_bf16(v.z - bf16_lo(hi.y), v.w - bf16_hi(hi.y)));
+  } else {
+    sum1[row] = v.x;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -689,51 +697,61 @@ __global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constan
 }
 
 // ---------------------------------------------------------------------------
-// Low-rank part of dq or dk, and the sum of both.
-struct LowArgs {
-  CUtensorMap tm_y, tm_yo, tm_fo, tm_sum, tm_hi, tm_lo, tm_f, tm_x, tm_dx;
+// dq or dk.  Head dim 64: both parts; head dim 128 (no tensor memory left for S): the low-rank part, and adds the
+// exact part that the window kernel left.
+struct GradArgs {
+  CUtensorMap tm_x, tm_y, tm_xo, tm_yo, tm_fo, tm_sum, tm_sum_lo, tm_hi, tm_lo, tm_dx;
   Geom g;
+  const float *n2, *delta;                 // (BH, Tp)
+  const float* off;                        // (BH, rows padded): exponent offsets of the own features
   const float* sum1;                       // (BH, m): extra column of the other side's summary
-  const float* delta;                      // (BH, Tp)
-  const float* part;                       // (tiles, D / 4, 128 rows) float4: exact part
+  const float* part;                       // head dim 128: (tiles, D / 4, 128 rows) float4
   int* status;
   int Tp, whole;
   float tau;
 };
 
-// A unit is a (tile, pass of 256 features); head dim 128 takes two passes.  Ring slots of a unit, in order: one per
-// column step (256 features, then Y'), the own features of the unit's two blocks of 128 ("+", "-"), and in a tile's
-// last unit its X rows, over which dx is staged for a bulk store.
+// A unit is a (tile, pass of 256 features); head dim 128 takes two passes.
+//
+// Tensor memory: df 256 | dx D | G of two steps 2 x 64 | (head dim 64) S 64.  A step's packed G lies over the first 16
+// of every 32 columns of its G buffer and p g over the next 16, so S is free for the next step as soon as it has been
+// read.  After the last step the G buffers take U of the own features.
+//
+// Bound: the stream into shared memory.  A step's 64 columns are 32 KB of features and 16 KB of X' and Y'; with the
+// summary and the own rows 368 KB per tile and side, 8.8 k cycles at the 41.7 B/clk one SM's TMA loads sustain.
 template <int D>
-struct LowCfg {
-  static constexpr int NB = D / 64, M = 4 * D, PASS = M / 256, NS = D == 64 ? 3 : 2;
-  static constexpr int AHEAD = NS - 1;                   // G products of the next unit issued before this one's end
-  static constexpr uint32_t TB = NB * 16384;             // own Y tile
+struct GradCfg {
+  static constexpr bool FUSE = D == 64;
+  static constexpr int NB = D / 64, M = 4 * D, PASS = M / 256, XBUF = FUSE ? 2 : 1, NF = 2, NC = FUSE ? 3 : 2;
+  static constexpr uint32_t TB = NB * 16384;             // own tile of X or Y
   static constexpr uint32_t AUX = 512 * D;               // 256 features x D of the summary; 2 terms x 128 x D of Wt
-  static constexpr uint32_t SLOT = 32768 + NB * 8192;
-  static constexpr uint32_t OFF_Y = 0, OFF_SUM = 2 * TB;
-  static constexpr uint32_t OFF_W = D == 64 ? OFF_SUM + AUX : OFF_SUM;   // head dim 128: one buffer for both, in turn
-  static constexpr uint32_t OFF_RING = OFF_W + AUX, OFF_H = OFF_RING + NS * SLOT, OFF_BAR = OFF_H + 1024;
-  static constexpr uint32_t SMEM = OFF_BAR + 256 + 1024;
-  static constexpr int NTHR = 320, W_LOAD = 8, W_MMA = 9;
-  static constexpr uint32_t T_DF = 0, T_DX = 256, T_G = 384;   // 256 | D | 2 x 64
-  enum { Y_FULL = 0, Y_FREE = 2, R_FULL = 4, R_FREE = R_FULL + NS, SUM_FULL = R_FREE + NS, SUM_FREE, W_FULL, W_FREE,
-         T_FULL, G_DONE = T_FULL + 2, DF_FULL = G_DONE + 2, DU_DONE, DX_FULL, DX_FREE, COUNT };
-  static_assert(SMEM <= 232448 && COUNT <= 30, "shared memory of one CTA");
+  static constexpr uint32_t CSLOT = 16384;               // Y' of a step, and X' (head dim 64)
+  static constexpr uint32_t OFF_X = 0, OFF_Y = XBUF * TB, OFF_SUM = OFF_Y + TB;
+  static constexpr uint32_t OFF_W = FUSE ? OFF_SUM + AUX : OFF_SUM;   // head dim 128: one buffer for both, in turn
+  static constexpr uint32_t OFF_F = OFF_W + AUX, OFF_C = OFF_F + NF * 32768, OFF_S1 = OFF_C + NC * CSLOT;
+  static constexpr uint32_t OFF_BAR = OFF_S1 + 2048, SMEM = OFF_BAR + 256 + 768;   // (the base is 256-byte aligned)
+  static constexpr int NCOMP = 512, NTHR = NCOMP + 96, W_LOAD = 16, W_MMA = 17, W_STORE = 18;
+  static constexpr uint32_t T_DF = 0, T_DX = 256, T_G = FUSE ? 320 : 384, T_S = 448;
+  enum { X_FULL = 0, X_FREE = 2, Y_FULL = 4, Y_FREE, SUM_FULL, SUM_FREE, W_FULL, W_FREE, F_FULL, F_FREE = F_FULL + NF,
+         C_FULL = F_FREE + NF, C_FREE = C_FULL + NC, T_FULL = C_FREE + NC, S_READ = T_FULL + 2, G_DONE = S_READ + 2,
+         DF_FULL = G_DONE + 2, DU_DONE, DX_FULL, DX_FREE, STAGED, COUNT };
+  static_assert(SMEM <= 232448 && COUNT * 8 + 4 <= 256, "shared memory of one CTA");
 };
 
 template <int SIDE, int D>
-__global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_constant__ LowArgs a) {
-  using C = LowCfg<D>;
-  extern __shared__ uint8_t smem_raw[];
+__global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant__ GradArgs a) {
+  using C = GradCfg<D>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::COUNT);
-  float* s_h = reinterpret_cast<float*>(smem + C::OFF_H);   // [2 column halves][128 rows]
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   if (tid == 0) {
-    for (int i = 0; i < C::COUNT; ++i)
-      mbar_init(bars + i, (i >= C::G_DONE && i < C::DF_FULL) || i == C::DU_DONE || i == C::DX_FREE ? 8 : 1);
+    for (int i = 0; i < C::COUNT; ++i) {
+      const bool group = i >= C::S_READ && i < C::DF_FULL;
+      const bool all = i == C::DU_DONE || i == C::DX_FREE || i == C::STAGED;
+      mbar_init(bars + i, group ? 8 : all ? 16 : 1);
+    }
     fence_mbar_init();
   }
   if (warp == C::W_LOAD) {
@@ -751,56 +769,64 @@ __global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_consta
 
   if (warp == C::W_LOAD) {
     const bool leader = elect_one();
-    int n = 0;
-    // the next ring slot, free; its barrier expects `bytes`
-    auto slot_for = [&](uint32_t bytes, uint64_t** bar) {
-      const int slot = n % C::NS;
-      if (n >= C::NS) wait_inline(bars + C::R_FREE + slot, ((n / C::NS) - 1) & 1, a.status, 262);
-      *bar = bars + C::R_FULL + slot;
-      if (leader) mbar_expect_tx(*bar, bytes);
-      ++n;
-      return smem + C::OFF_RING + slot * C::SLOT;
-    };
+    int nf = 0, nc = 0, ns = 0;     // loads so far: features, column tiles, summary terms
     for (int u = 0; u < n_u; ++u) {
       const int it = u / C::PASS, pass = u % C::PASS;
       const RowTile t = row_tile<SIDE, 64>(a.g, blockIdx.x + it * step, whole);
-      uint64_t* bar;
-      auto column_step = [&](int s) {
-        uint8_t* dst = slot_for(C::SLOT, &bar);
+      auto load_x = [&]() {
+        const int buf = it % C::XBUF;
+        if (it >= C::XBUF) wait_inline(bars + C::X_FREE + buf, ((it / C::XBUF) - 1) & 1, a.status, 261);
         if (leader) {
+          mbar_expect_tx(bars + C::X_FULL + buf, C::TB);
           for (int j = 0; j < C::NB; ++j)
-            tma_load_4d(dst + 32768 + j * 8192, &a.tm_yo, bar, 64 * j, t.c0 + 64 * s, t.h, t.b);
-          for (int j = 0; j < 4; ++j) tma_load_3d(dst + j * 8192, &a.tm_fo, bar, 256 * pass + 64 * j, t.c0 + 64 * s, t.bh);
+            tma_load_4d(smem + C::OFF_X + buf * C::TB + j * 16384, &a.tm_x, bars + C::X_FULL + buf, 64 * j, t.r0, t.h, t.b);
         }
       };
-      if (pass == 0) {
-        const int buf = it & 1;
-        if (it >= 2) wait_inline(bars + C::Y_FREE + buf, ((it >> 1) - 1) & 1, a.status, 261);
+      auto load_c = [&](int s) {
+        const int slot = nc % C::NC;
+        if (nc >= C::NC) wait_inline(bars + C::C_FREE + slot, ((nc / C::NC) - 1) & 1, a.status, 262);
+        ++nc;
         if (leader) {
-          mbar_expect_tx(bars + C::Y_FULL + buf, C::TB);
+          uint8_t* dst = smem + C::OFF_C + slot * C::CSLOT;
+          mbar_expect_tx(bars + C::C_FULL + slot, C::CSLOT);
           for (int j = 0; j < C::NB; ++j)
-            tma_load_4d(smem + C::OFF_Y + buf * C::TB + j * 16384, &a.tm_y, bars + C::Y_FULL + buf, 64 * j, t.r0, t.h, t.b);
+            tma_load_4d(dst + j * 8192, &a.tm_yo, bars + C::C_FULL + slot, 64 * j, t.c0 + 64 * s, t.h, t.b);
+          if (C::FUSE) tma_load_4d(dst + 8192, &a.tm_xo, bars + C::C_FULL + slot, 0, t.c0 + 64 * s, t.h, t.b);
         }
-      }
-      int s = 0;
-      if (s < t.n) column_step(s++);
-      // Head dim 64: the summary has a buffer of its own and Wt stays.  Head dim 128: summary and Wt of the unit
-      // take turns in one buffer (summary -> its product -> Wt -> its product -> next summary).
-      if (!whole) {
-        if (u >= 1) wait_inline(bars + (D == 64 ? C::SUM_FREE : C::W_FREE), (u - 1) & 1, a.status, 263);
+      };
+      auto load_f = [&](int s) {
+        const int slot = nf % C::NF;
+        if (nf >= C::NF) wait_inline(bars + C::F_FREE + slot, ((nf / C::NF) - 1) & 1, a.status, 263);
+        ++nf;
+        if (leader) {
+          uint8_t* dst = smem + C::OFF_F + slot * 32768;
+          mbar_expect_tx(bars + C::F_FULL + slot, 32768);
+          for (int j = 0; j < 4; ++j)
+            tma_load_3d(dst + j * 8192, &a.tm_fo, bars + C::F_FULL + slot, 256 * pass + 64 * j, t.c0 + 64 * s, t.bh);
+        }
+      };
+      // Head dim 64: the summary's terms take turns in a buffer of their own and Wt stays.  Head dim 128: they and
+      // Wt of the unit take turns in one (term, its product, term, its product, Wt, its products, next unit).
+      auto load_sum = [&](int term) {
+        if (term == 0 && !C::FUSE) {
+          if (u >= 1) wait_inline(bars + C::W_FREE, (u - 1) & 1, a.status, 264);
+        } else if (ns >= 1) {
+          wait_inline(bars + C::SUM_FREE, (ns - 1) & 1, a.status, 265);
+        }
+        ++ns;
         if (leader) {
           mbar_expect_tx(bars + C::SUM_FULL, C::AUX);
           for (int j = 0; j < C::NB; ++j)
             for (int f = 0; f < 2; ++f)
-              tma_load_3d(smem + C::OFF_SUM + j * 32768 + f * 16384, &a.tm_sum, bars + C::SUM_FULL, 64 * j,
-                          256 * pass + 128 * f, t.bh);
+              tma_load_3d(smem + C::OFF_SUM + j * 32768 + f * 16384, term ? &a.tm_sum_lo : &a.tm_sum, bars + C::SUM_FULL,
+                          64 * j, 256 * pass + 128 * f, t.bh);
         }
-      }
-      for (; s < t.n && s < 3; ++s) column_step(s);
-      if (D != 64 || u == 0) {
-        if (D != 64) {
-          if (!whole) wait_inline(bars + C::SUM_FREE, u & 1, a.status, 265);
-          else if (u >= 1) wait_inline(bars + C::W_FREE, (u - 1) & 1, a.status, 266);
+      };
+      auto load_w = [&]() {
+        if (C::FUSE && u > 0) return;
+        if (!C::FUSE) {
+          if (!whole) wait_inline(bars + C::SUM_FREE, (ns - 1) & 1, a.status, 266);
+          else if (u >= 1) wait_inline(bars + C::W_FREE, (u - 1) & 1, a.status, 267);
         }
         if (leader) {
           mbar_expect_tx(bars + C::W_FULL, C::AUX);
@@ -809,19 +835,32 @@ __global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_consta
             tma_load_2d(smem + C::OFF_W + C::AUX / 2 + j * 16384, &a.tm_lo, bars + C::W_FULL, 64 * j, 128 * pass);
           }
         }
+      };
+      if (pass == 0) {
+        if (it >= 1) wait_inline(bars + C::Y_FREE, (it - 1) & 1, a.status, 268);
+        if (leader) {
+          mbar_expect_tx(bars + C::Y_FULL, C::TB);
+          for (int j = 0; j < C::NB; ++j)
+            tma_load_4d(smem + C::OFF_Y + j * 16384, &a.tm_y, bars + C::Y_FULL, 64 * j, t.r0, t.h, t.b);
+        }
+        if (C::FUSE) load_x();
       }
-      for (; s < t.n; ++s) column_step(s);
-      for (int blk = 0; blk < 2; ++blk) {
-        uint8_t* dst = slot_for(32768, &bar);
-        if (leader)
-          for (int j = 0; j < 2; ++j)
-            tma_load_3d(dst + j * 16384, &a.tm_f, bar, 256 * pass + 128 * blk + 64 * j, t.r0, t.bh);
+      // column tiles run one step ahead of the features; the summary's terms behind steps 0 and 1, Wt behind step 2
+      if (t.n > 0) load_c(0);
+      int sums = whole ? 2 : 0;
+      bool w = false;
+      for (int s = 0; s < t.n; ++s) {
+        if (s + 1 < t.n) load_c(s + 1);
+        load_f(s);
+        if (sums < 2) load_sum(sums++);
+        if (s == 2) {
+          load_w();
+          w = true;
+        }
       }
-      if (pass == C::PASS - 1) {
-        uint8_t* dst = slot_for(C::TB, &bar);
-        if (leader)
-          for (int j = 0; j < C::NB; ++j) tma_load_4d(dst + j * 16384, &a.tm_x, bar, 64 * j, t.r0, t.h, t.b);
-      }
+      while (sums < 2) load_sum(sums++);
+      if (!w) load_w();
+      if (!C::FUSE && pass == 0) load_x();
     }
     __syncwarp();
   } else if (warp == C::W_MMA) {
@@ -829,246 +868,316 @@ __global__ void __launch_bounds__(320, 1) bwd_lowrank_kernel(const __grid_consta
     constexpr uint32_t id_t = idesc_bf16(128, 64, false, false);
     constexpr uint32_t id_df = idesc_bf16(128, 256, false, true);
     constexpr uint32_t id_sum = idesc_bf16(128, 256, false, false);
+    constexpr uint32_t id_u = idesc_bf16(128, 128, false, false);
     constexpr uint32_t id_dx = idesc_bf16(128, D, false, true);
+    const uint64_t dX = smem_desc_sw128(smem_u32(smem + C::OFF_X), 16, 1024);
     const uint64_t dY = smem_desc_sw128(smem_u32(smem + C::OFF_Y), 16, 1024);
-    const uint64_t dYo = smem_desc_sw128(smem_u32(smem + C::OFF_RING + 32768), 16, 1024);
-    const uint64_t dFo = smem_desc_sw128(smem_u32(smem + C::OFF_RING), 8192, 1024);
+    const uint64_t dC = smem_desc_sw128(smem_u32(smem + C::OFF_C), 16, 1024);
+    const uint64_t dCt = smem_desc_sw128(smem_u32(smem + C::OFF_C + 8192), 8192, 1024);   // X', MN-major
+    const uint64_t dF = smem_desc_sw128(smem_u32(smem + C::OFF_F), 8192, 1024);
     const uint64_t dSum = smem_desc_sw128(smem_u32(smem + C::OFF_SUM), 16, 1024);
-    const uint64_t dW = smem_desc_sw128(smem_u32(smem + C::OFF_W), 16384, 1024);
-    // G of step s of unit u; gg: its number in the CTA's stream of steps, rp: its ring number
-    auto issue_t = [&](int u, int s, int gg, int rp) {
-      const int it = u / C::PASS, slot = rp % C::NS;
-      if (u % C::PASS == 0 && s == 0) wait_inline(bars + C::Y_FULL + (it & 1), (it >> 1) & 1, a.status, 267);
-      wait_inline(bars + C::R_FULL + slot, (rp / C::NS) & 1, a.status, 268);
-      tc_fence_after_sync();
-      if (leader) {
-        const uint64_t y = dY + (uint64_t)((it & 1) * (C::TB >> 4)), o = dYo + (uint64_t)(slot * (C::SLOT >> 4));
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          mma_ss(tb + C::T_G + 64 * (gg & 1), y + kmajor(k, 16384), o + kmajor(k, 8192), id_t, k > 0);
-        mma_commit(bars + C::T_FULL + (gg & 1));
-      }
-      __syncwarp();
-    };
-    int g0 = 0, r0 = 0, n = 0, n_next = 0;   // numbers of the unit's first step and first ring slot; its steps
-    if (n_u > 0) {
-      n_next = row_tile<SIDE, 64>(a.g, blockIdx.x, whole).n;
-      for (int s = 0; s < C::AHEAD && s < n_next; ++s) issue_t(0, s, s, s);
-    }
+    const uint64_t dWk = smem_desc_sw128(smem_u32(smem + C::OFF_W), 16, 1024);
+    const uint64_t dWt = smem_desc_sw128(smem_u32(smem + C::OFF_W), 16384, 1024);
+    int g0 = 0, ns = 0;             // number of the unit's first step; summary terms so far
     for (int u = 0; u < n_u; ++u) {
-      const int it = u / C::PASS, pass = u % C::PASS;
-      n = n_next;
-      // (the previous tile's X rows had the ring slot before: see below)
-      if (u >= 1 && pass == 0) wait_inline(bars + C::R_FULL + (r0 - 1) % C::NS, ((r0 - 1) / C::NS) & 1, a.status, 294);
-      for (int s = C::AHEAD; s < 2 && s < n; ++s) issue_t(u, s, g0 + s, r0 + s);
-      // without steps nobody has waited for the Y tile yet
-      if (n == 0 && pass == 0) wait_inline(bars + C::Y_FULL + (it & 1), (it >> 1) & 1, a.status, 270);
-      if (!whole) {
-        wait_inline(bars + C::SUM_FULL, u & 1, a.status, 271);
+      const int it = u / C::PASS, pass = u % C::PASS, xb = it % C::XBUF;
+      const int n = row_tile<SIDE, 64>(a.g, blockIdx.x + it * step, whole).n;
+      const uint64_t x = dX + (uint64_t)(xb * (C::TB >> 4));
+      // G = Y Y'^T of step s; gg: its number in the CTA's stream of steps
+      auto issue_g = [&](int gg) {
+        const int slot = gg % C::NC;
+        wait_inline(bars + C::C_FULL + slot, (gg / C::NC) & 1, a.status, 271);
+        tc_fence_after_sync();
+        if (leader) {
+          const uint64_t o = dC + (uint64_t)(slot * (C::CSLOT >> 4));
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_ss(tb + C::T_G + 64 * (gg & 1), dY + kmajor(k, 16384), o + kmajor(k, 8192), id_t, k > 0);
+          if (!C::FUSE) {
+            mma_commit(bars + C::T_FULL + (gg & 1));
+            mma_commit(bars + C::C_FREE + slot);
+          }
+        }
+        __syncwarp();
+      };
+      // S = X X'^T; its column tile is that of the G product issued before
+      auto issue_s = [&](int gg) {
+        if (leader) {
+          const uint64_t o = dC + (uint64_t)((gg % C::NC) * (C::CSLOT >> 4) + 512);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) mma_ss(tb + C::T_S, x + kmajor(k, 16384), o + kmajor(k, 8192), id_t, k > 0);
+          mma_commit(bars + C::T_FULL + (gg & 1));
+        }
+        __syncwarp();
+      };
+      bool fresh = true;            // df of this unit has not been written to
+      auto touch = [&]() {          // before its first product: the previous tile's dx (and what lies in df) has been read
+        if (fresh && pass == 0 && it >= 1) wait_inline(bars + C::DX_FREE, (it - 1) & 1, a.status, 272);
+      };
+      int sums = whole ? 2 : 0;
+      auto issue_sum = [&]() {      // df += Y summary^T, one term
+        touch();
+        wait_inline(bars + C::SUM_FULL, ns & 1, a.status, 273);
+        ++ns;
         tc_fence_after_sync();
         if (leader) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            mma_ss(tb + C::T_DF, dY + (uint64_t)((it & 1) * (C::TB >> 4)) + kmajor(k, 16384), dSum + kmajor(k, 32768),
-                   id_sum, k > 0);
+            mma_ss(tb + C::T_DF, dY + kmajor(k, 16384), dSum + kmajor(k, 32768), id_sum, !fresh || k > 0);
           mma_commit(bars + C::SUM_FREE);
         }
         __syncwarp();
+        fresh = false;
+        ++sums;
+      };
+      if (pass == 0) wait_inline(bars + C::Y_FULL, it & 1, a.status, 274);
+      if (C::FUSE) wait_inline(bars + C::X_FULL + xb, (it / C::XBUF) & 1, a.status, 275);
+      if (n > 0) {
+        issue_g(g0);
+        if (C::FUSE) issue_s(g0);
+        if (n > 1) issue_g(g0 + 1);
       }
       for (int s = 0; s < n; ++s) {
-        const int gg = g0 + s, slot = (r0 + s) % C::NS;
-        wait_inline(bars + C::G_DONE + (gg & 1), (gg >> 1) & 1, a.status, 269);
+        const int gg = g0 + s, slot = gg % C::NF;
+        if (C::FUSE && s + 1 < n) {
+          wait_inline(bars + C::S_READ + (gg & 1), (gg >> 1) & 1, a.status, 276);
+          tc_fence_after_sync();
+          issue_s(gg + 1);
+        }
+        wait_inline(bars + C::F_FULL + slot, (gg / C::NF) & 1, a.status, 277);
+        touch();
+        wait_inline(bars + C::G_DONE + (gg & 1), (gg >> 1) & 1, a.status, 278);
         tc_fence_after_sync();
         if (leader) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mma_ts(tb + C::T_DF, tb + C::T_G + 64 * (gg & 1) + packed(k),
-                   dFo + (uint64_t)(slot * (C::SLOT >> 4) + k * 128), id_df, !whole || s > 0 || k > 0);
-          mma_commit(bars + C::R_FREE + slot);
+            mma_ts(tb + C::T_DF, tb + C::T_G + 64 * (gg & 1) + packed(k), dF + (uint64_t)(slot * 2048 + k * 128), id_df,
+                   !fresh || k > 0);
+          mma_commit(bars + C::F_FREE + slot);
+          if (C::FUSE) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_ts(tb + C::T_DX, tb + C::T_G + 64 * (gg & 1) + 16 + packed(k),
+                     dCt + (uint64_t)((gg % C::NC) * (C::CSLOT >> 4) + k * 128), id_dx, s > 0 || k > 0);
+            mma_commit(bars + C::C_FREE + gg % C::NC);
+          }
         }
         __syncwarp();
-        if (s + 2 < n) issue_t(u, s + 2, gg + 2, r0 + s + 2);
+        fresh = false;
+        if (s + 2 < n) issue_g(gg + 2);
+        if (sums < 2) issue_sum();
       }
-      if (leader) {
-        if (pass == C::PASS - 1) mma_commit(bars + C::Y_FREE + (it & 1));
-        mma_commit(bars + C::DF_FULL);
-      }
-      __syncwarp();
-      // The next unit's first G products run while this unit's df turns into du.  (Their ring slots are those of the
-      // own features, which the compute warps free by themselves; never that of the X rows, freed behind DX_FULL.)
-      // A wait tells phases apart by parity alone, so this warp has to have seen every use of a slot, those that it
-      // does not read among them.
-      for (int blk = 0; blk < 2; ++blk)
-        wait_inline(bars + C::R_FULL + (r0 + n + blk) % C::NS, ((r0 + n + blk) / C::NS) & 1, a.status, 295);
+      while (sums < 2) issue_sum();
       g0 += n;
-      r0 += n + (pass == C::PASS - 1 ? 3 : 2);
-      if (u + 1 < n_u) {
-        if (pass == C::PASS - 1) n_next = row_tile<SIDE, 64>(a.g, blockIdx.x + (it + 1) * step, whole).n;
-        for (int s = 0; s < C::AHEAD && s < n_next; ++s) issue_t(u + 1, s, g0 + s, r0 + s);
-      }
-      wait_inline(bars + C::DU_DONE, u & 1, a.status, 272);
-      if (pass == 0 && it >= 1) wait_inline(bars + C::DX_FREE, (it - 1) & 1, a.status, 273);
-      if (D != 64) wait_inline(bars + C::W_FULL, u & 1, a.status, 274);
-      else if (u == 0) wait_inline(bars + C::W_FULL, 0, a.status, 275);
+      // U of the own features over the G buffers, for du
+      wait_inline(bars + C::W_FULL, C::FUSE ? 0 : u & 1, a.status, 279);
+      if (!C::FUSE && pass == 0) wait_inline(bars + C::X_FULL + xb, (it / C::XBUF) & 1, a.status, 280);
       tc_fence_after_sync();
       if (leader) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x)        // the two terms of Wt
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int k = 0; k < 8; ++k)      // 128 projections
-            mma_ts(tb + C::T_DX, tb + C::T_DF + 128 * (k >> 2) + packed(k & 3),
-                   dW + (uint64_t)(x * (C::AUX >> 5) + k * 128), id_dx, pass > 0 || x > 0 || k > 0);
+          for (int k = 0; k < D / 16; ++k)
+            mma_ss(tb + C::T_G, x + kmajor(k, 16384), dWk + (uint64_t)(t * (C::AUX >> 5)) + kmajor(k, 16384), id_u,
+                   t > 0 || k > 0);
+        if (pass == C::PASS - 1) mma_commit(bars + C::Y_FREE);
+        mma_commit(bars + C::DF_FULL);
+      }
+      __syncwarp();
+      wait_inline(bars + C::DU_DONE, u & 1, a.status, 281);
+      const bool first = pass == 0 && !(C::FUSE && n > 0);   // nothing of this tile is in dx yet
+      if (first && it >= 1) wait_inline(bars + C::DX_FREE, (it - 1) & 1, a.status, 282);
+      tc_fence_after_sync();
+      if (leader) {
+        // du Wt: high x high, high x low, low x high; du's low term lies behind its high one
+#pragma unroll
+        for (int t = 0; t < 3; ++t)
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_ts(tb + C::T_DX, tb + C::T_DF + 128 * (k >> 2) + packed(k & 3) + (t == 2 ? 16 : 0),
+                   dWt + (uint64_t)((t == 1 ? (C::AUX >> 5) : 0) + k * 128), id_dx, !first || t > 0 || k > 0);
         mma_commit(bars + C::W_FREE);
         if (pass == C::PASS - 1) mma_commit(bars + C::DX_FULL);
       }
       __syncwarp();
     }
+  } else if (warp == C::W_STORE) {
+    // the staged dx (over the X rows) -> memory; rows past the end are clipped by the tensor map
+    const bool leader = elect_one();
+    for (int it = 0; it < n_it; ++it) {
+      const RowTile t = row_tile<SIDE, 64>(a.g, blockIdx.x + it * step, whole);
+      const int buf = it % C::XBUF;
+      wait_inline(bars + C::STAGED, it & 1, a.status, 283);
+      if (leader) {
+        for (int j = 0; j < C::NB; ++j)
+          tma_store_4d(&a.tm_dx, smem + C::OFF_X + buf * C::TB + j * 16384, 64 * j, t.r0, t.h, t.b);
+        tma_store_commit();
+        tma_store_wait_read0();
+        mbar_arrive(bars + C::X_FREE + buf);
+      }
+      __syncwarp();
+    }
+    if (leader) tma_store_wait_all();
+    __syncwarp();
   } else {
-    const int qd = warp & 3, cq = warp >> 2;
+    // Two groups of eight warps take the steps in turn; a thread owns a row and 32 of a step's 64 columns.  For du the
+    // groups take a block of 128 features each, for dx every thread a quarter of the row.
+    const int grp = warp >> 3, qd = warp & 3, cq = (warp >> 2) & 1;
     const int row = qd * 32 + lane;
     const uint32_t lane_base = tb + ((uint32_t)(qd * 32) << 16);
-    const float sign = whole ? 1.f : -1.f;   // the window's G enters with a minus
-    int gg = 0, rp = 0;
+    float* s_s1 = reinterpret_cast<float*>(smem + C::OFF_S1);    // [2][256], by parity of the unit
+    const float sc = a.tau * kLog2e;
+    const float lt = log2f(a.tau);
+    int gg = 0;
     float hs = 0.f;
     for (int u = 0; u < n_u; ++u) {
       const int it = u / C::PASS, pass = u % C::PASS;
       const int tile = blockIdx.x + it * step;
       const RowTile t = row_tile<SIDE, 64>(a.g, tile, whole);
       const int r = t.r0 + row;
+      const float* n2 = a.n2 + (int64_t)t.bh * a.Tp;
       const float* dl = a.delta + (int64_t)t.bh * a.Tp;
-      const float rd = SIDE == QUERIES ? __ldg(dl + r) : 0.f;
-      for (int s = 0; s < t.n; ++s, ++gg, ++rp) {
+      const float off = __ldg(a.off + ((int64_t)t.bh * a.g.ntr) * TR + r);
+      float rn = 0.f, rd = 0.f;
+      if (SIDE == QUERIES) {
+        rn = __ldg(n2 + r) - lt;    // tau p = 2^(S sc - (n2 - log2 tau))
+        rd = __ldg(dl + r);
+      }
+      if (tid < 256) s_s1[256 * (u & 1) + tid] = __ldg(a.sum1 + (int64_t)t.bh * C::M + 256 * pass + tid);
+      for (int s = 0; s < t.n; ++s, ++gg) {
+        if ((gg & 1) != grp) continue;
         const int c = t.c0 + 64 * s + 32 * cq;
-        const uint32_t vis = seen<SIDE>(a.g, t, r, c, whole);
-        const uint32_t tg = lane_base + C::T_G + 64 * (gg & 1) + 32 * cq;
-        uint32_t o[16];
-        mbar_wait(bars + C::T_FULL + (gg & 1), (gg >> 1) & 1, a.status, 276);
+        const uint32_t in = seen<SIDE>(a.g, t, r, c, false);
+        const uint32_t vis = whole ? seen<SIDE>(a.g, t, r, c, true) : in;
+        const uint32_t tg = lane_base + C::T_G + 64 * grp + 32 * cq;
+        mbar_wait(bars + C::T_FULL + grp, (gg >> 1) & 1, a.status, 286);
         tc_fence_after_sync();
-        if (__any_sync(0xffffffffu, vis != 0u)) {
-          uint32_t y[32];
-          tmem_ld32(tg, y);
-          tmem_ld_wait();
+        uint32_t x[32], y[32];
+        if (C::FUSE) tmem_ld32(lane_base + C::T_S + 32 * cq, x);
+        tmem_ld32(tg, y);
+        tmem_ld_wait();
+        if (C::FUSE) {
+          tc_fence_before_sync();
+          warp_arrive(bars + C::S_READ + grp, lane);
+        }
+        uint32_t o[16], e[16];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            float4 cd = make_float4(rd, rd, rd, rd);
-            if (SIDE == KEYS) cd = __ldg(reinterpret_cast<const float4*>(dl + c) + q);
-            const float dd[4] = {cd.x, cd.y, cd.z, cd.w};
-            float v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              v[j] = keep_if_bit(sign * (__uint_as_float(y[4 * q + j]) - dd[j]), vis, 4 * q + j);
-            o[2 * q] = pack_bf16(v[0], v[1]);
-            o[2 * q + 1] = pack_bf16(v[2], v[3]);
+        for (int q = 0; q < 8; ++q) {
+          float4 cn = make_float4(rn, rn, rn, rn), cd = make_float4(rd, rd, rd, rd);
+          if (SIDE == KEYS) {
+            // c < Tp: the row arrays are padded to whole tiles
+            if (C::FUSE) cn = __ldg(reinterpret_cast<const float4*>(n2 + c) + q);
+            cd = __ldg(reinterpret_cast<const float4*>(dl + c) + q);
           }
-        } else {
+          const float nn[4] = {cn.x, cn.y, cn.z, cn.w}, dd[4] = {cd.x, cd.y, cd.z, cd.w};
+          float v[4], w[4];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) o[j] = 0u;
+          for (int j = 0; j < 4; ++j) {
+            const float d = __uint_as_float(y[4 * q + j]) - dd[j];
+            v[j] = keep_if_bit(whole ? d : -d, vis, 4 * q + j);   // the window's G enters df with a minus
+            if (C::FUSE) {
+              const float p = ex2(fmaf(__uint_as_float(x[4 * q + j]), sc, SIDE == KEYS ? lt - nn[j] : -nn[j]));
+              w[j] = keep_if_bit(p * d, in, 4 * q + j);
+            }
+          }
+          o[2 * q] = pack_bf16(v[0], v[1]);
+          o[2 * q + 1] = pack_bf16(v[2], v[3]);
+          if (C::FUSE) {
+            e[2 * q] = pack_bf16(w[0], w[1]);
+            e[2 * q + 1] = pack_bf16(w[2], w[3]);
+          }
         }
         tmem_st16(tg, o);
+        if (C::FUSE) tmem_st16(tg + 16, e);
         tmem_st_wait();
         tc_fence_before_sync();
-        warp_arrive(bars + C::G_DONE + (gg & 1), lane);
+        warp_arrive(bars + C::G_DONE + grp, lane);
       }
-      // df -> du of this thread's 2 x 32 projections
+      // df -> du of this thread's 32 projections: du = f+ df+ - f- df-, in two bf16 terms
       const bool none = whole && t.n == 0;
       const float d1 = whole ? 0.f : (SIDE == QUERIES ? rd : 1.f);
       if (pass == 0) hs = 0.f;
-      const float* s1 = a.sum1 + (int64_t)t.bh * C::M + 256 * pass + 32 * cq;
-      mbar_wait(bars + C::DF_FULL, u & 1, a.status, 277);
+      asm volatile("bar.sync 1, 512;" ::: "memory");   // sum1 of the unit is in shared memory
+      const float* s1 = s_s1 + 256 * (u & 1) + 128 * grp + 32 * cq;
+      const uint32_t td = lane_base + C::T_DF + 128 * grp + 32 * cq;
+      mbar_wait(bars + C::DF_FULL, u & 1, a.status, 287);
       tc_fence_after_sync();
-#pragma unroll 1
-      for (int blk = 0; blk < 2; ++blk) {
-        const int slot = (rp + blk) % C::NS;
-        const uint32_t td = lane_base + C::T_DF + 128 * blk + 32 * cq;
-        const uint8_t* line = smem + C::OFF_RING + slot * C::SLOT + row * 128;
-        mbar_wait(bars + C::R_FULL + slot, ((rp + blk) / C::NS) & 1, a.status, 279);
-        uint32_t o[16];
+      uint32_t hi[16], lo[16];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t p[16], m[16];
-          tmem_ld16(td + 16 * hf, p);
-          tmem_ld16(td + 64 + 16 * hf, m);
-          uint4 fp[2], fm[2];
+      for (int hf = 0; hf < 2; ++hf) {
+        uint32_t p[16], m[16], uu[16];
+        tmem_ld16(td + 16 * hf, p);
+        tmem_ld16(td + 64 + 16 * hf, m);
+        tmem_ld16(lane_base + C::T_G + 64 * grp + 32 * cq + 16 * hf, uu);
+        tmem_ld_wait();
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const uint32_t at = (uint32_t)(((4 * cq + 2 * hf + q) ^ (row & 7)) << 4);
-            fp[q] = *reinterpret_cast<const uint4*>(line + at);
-            fm[q] = *reinterpret_cast<const uint4*>(line + 16384 + at);
-          }
-          tmem_ld_wait();
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const uint32_t wp = (&fp[q >> 2].x)[q & 3], wm = (&fm[q >> 2].x)[q & 3];
-            const float2 sp = __ldg(reinterpret_cast<const float2*>(s1 + 128 * blk + 16 * hf) + q);
-            const float2 sm = __ldg(reinterpret_cast<const float2*>(s1 + 128 * blk + 64 + 16 * hf) + q);
-            const float p0 = none ? 0.f : __uint_as_float(p[2 * q]), p1 = none ? 0.f : __uint_as_float(p[2 * q + 1]);
-            const float m0 = none ? 0.f : __uint_as_float(m[2 * q]), m1 = none ? 0.f : __uint_as_float(m[2 * q + 1]);
-            const float hp0 = bf16_lo(wp) * fmaf(-d1, sp.x, p0), hp1 = bf16_hi(wp) * fmaf(-d1, sp.y, p1);
-            const float hm0 = bf16_lo(wm) * fmaf(-d1, sm.x, m0), hm1 = bf16_hi(wm) * fmaf(-d1, sm.y, m1);
-            hs += (hp0 + hm0) + (hp1 + hm1);
-            o[8 * hf + q] = pack_bf16(hp0 - hm0, hp1 - hm1);
-          }
+        for (int q = 0; q < 8; ++q) {
+          const float2 sp = *reinterpret_cast<const float2*>(s1 + 16 * hf + 2 * q);
+          const float2 sm = *reinterpret_cast<const float2*>(s1 + 64 + 16 * hf + 2 * q);
+          const float u0 = __uint_as_float(uu[2 * q]), u1 = __uint_as_float(uu[2 * q + 1]);
+          const float hp0 = ex2(fmaf(u0, kLog2e, off)) * fmaf(-d1, sp.x, none ? 0.f : __uint_as_float(p[2 * q]));
+          const float hp1 = ex2(fmaf(u1, kLog2e, off)) * fmaf(-d1, sp.y, none ? 0.f : __uint_as_float(p[2 * q + 1]));
+          const float hm0 = ex2(fmaf(u0, -kLog2e, off)) * fmaf(-d1, sm.x, none ? 0.f : __uint_as_float(m[2 * q]));
+          const float hm1 = ex2(fmaf(u1, -kLog2e, off)) * fmaf(-d1, sm.y, none ? 0.f : __uint_as_float(m[2 * q + 1]));
+          hs += (hp0 + hm0) + (hp1 + hm1);
+          const float d0 = hp0 - hm0, d2 = hp1 - hm1;
+          const uint32_t h2 = pack_bf16(d0, d2);
+          hi[8 * hf + q] = h2;
+          lo[8 * hf + q] = pack_bf16(d0 - bf16_lo(h2), d2 - bf16_hi(h2));
         }
-        // (both threads of a row write over their own "+" columns, which only they read)
-        tmem_st16(td, o);
       }
+      tmem_st16(td, hi);            // over the thread's own "+" columns
+      tmem_st16(td + 16, lo);
+      if (pass == C::PASS - 1) tmem_st1(td + 64, __float_as_uint(hs));   // ... and the first of its "-" columns
       tmem_st_wait();
       tc_fence_before_sync();
       warp_arrive(bars + C::DU_DONE, lane);
-      if (pass == C::PASS - 1) s_h[cq * 128 + row] = hs;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (tid < 2) mbar_arrive(bars + C::R_FREE + (rp + tid) % C::NS);   // the own features have been read
-      rp += 2;
       if (pass == C::PASS - 1) {
-        const int slot = rp % C::NS;
-        uint8_t* xs = smem + C::OFF_RING + slot * C::SLOT;
-        const float hsum = a.tau * (s_h[row] + s_h[128 + row]);
-        const float4* part = reinterpret_cast<const float4*>(a.part) + (int64_t)tile * (D / 4) * TR + row;
-        float4 e[D / 8];
+        constexpr int NQ = D / 4;
+        const int c = NQ * (2 * grp + cq), buf = it % C::XBUF;
+        uint8_t* xs = smem + C::OFF_X + buf * C::TB + (c >> 6) * 16384 + row * 128;
+        float4 e[C::FUSE ? 1 : NQ / 4];
+        if (!C::FUSE) {
+          const float4* part = reinterpret_cast<const float4*>(a.part) + ((int64_t)tile * (D / 4) + c / 4) * TR + row;
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) e[j] = __ldg(part + (D / 8 * cq + j) * TR);
-        mbar_wait(bars + C::R_FULL + slot, (rp / C::NS) & 1, a.status, 280);
-        mbar_wait(bars + C::DX_FULL, it & 1, a.status, 278);
-        tc_fence_after_sync();
-#pragma unroll
-        for (int q = 0; q < D / 32; ++q) {
-          const int c = (D / 2) * cq + 16 * q;
-          uint32_t v[16];
-          tmem_ld16(lane_base + C::T_DX + c, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            // eight entries: 16 bytes of the row's swizzled line, dx over x
-            uint4* at = reinterpret_cast<uint4*>(xs + (c >> 6) * 16384 + row * 128 + ((((c & 63) >> 3) + j) ^ (row & 7)) * 16);
-            const uint4 xv = *at;
-            const float4 e0 = e[4 * q + 2 * j], e1 = e[4 * q + 2 * j + 1];
-            uint4 o;
-            o.x = pack_bf16(fmaf(-hsum, bf16_lo(xv.x), __uint_as_float(v[8 * j]) + e0.x),
-                            fmaf(-hsum, bf16_hi(xv.x), __uint_as_float(v[8 * j + 1]) + e0.y));
-            o.y = pack_bf16(fmaf(-hsum, bf16_lo(xv.y), __uint_as_float(v[8 * j + 2]) + e0.z),
-                            fmaf(-hsum, bf16_hi(xv.y), __uint_as_float(v[8 * j + 3]) + e0.w));
-            o.z = pack_bf16(fmaf(-hsum, bf16_lo(xv.z), __uint_as_float(v[8 * j + 4]) + e1.x),
-                            fmaf(-hsum, bf16_hi(xv.z), __uint_as_float(v[8 * j + 5]) + e1.y));
-            o.w = pack_bf16(fmaf(-hsum, bf16_lo(xv.w), __uint_as_float(v[8 * j + 6]) + e1.z),
-                            fmaf(-hsum, bf16_hi(xv.w), __uint_as_float(v[8 * j + 7]) + e1.w));
-            *at = o;
-          }
+          for (int j = 0; j < NQ / 4; ++j) e[j] = __ldg(part + j * TR);
         }
+        mbar_wait(bars + C::X_FULL + buf, (it / C::XBUF) & 1, a.status, 288);
+        mbar_wait(bars + C::DX_FULL, it & 1, a.status, 289);
+        tc_fence_after_sync();
+        uint32_t v[NQ / 16][16];
+        const uint32_t h0 = tmem_ld1(lane_base + C::T_DF + 64), h1 = tmem_ld1(lane_base + C::T_DF + 96);
+        const uint32_t h2 = tmem_ld1(lane_base + C::T_DF + 192), h3 = tmem_ld1(lane_base + C::T_DF + 224);
+#pragma unroll
+        for (int q = 0; q < NQ / 16; ++q) tmem_ld16(lane_base + C::T_DX + c + 16 * q, v[q]);
+        tmem_ld_wait();
         tc_fence_before_sync();
         warp_arrive(bars + C::DX_FREE, lane);
-        fence_async_smem();
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (tid == 0) {
-          // rows past the end are clipped by the tensor map
-          for (int j = 0; j < C::NB; ++j) tma_store_4d(&a.tm_dx, xs + j * 16384, 64 * j, t.r0, t.h, t.b);
-          tma_store_commit();
-          tma_store_wait_read0();
-          mbar_arrive(bars + C::R_FREE + slot);
+        const float hsum = a.tau * ((__uint_as_float(h0) + __uint_as_float(h1)) + (__uint_as_float(h2) + __uint_as_float(h3)));
+#pragma unroll
+        for (int j = 0; j < NQ / 8; ++j) {
+          // eight entries: 16 bytes of the row's swizzled line, dx over x
+          uint4* at = reinterpret_cast<uint4*>(xs + ((((c & 63) >> 3) + j) ^ (row & 7)) * 16);
+          const uint4 xv = *at;
+          const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+          float z[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) z[k] = __uint_as_float(v[j >> 1][8 * (j & 1) + k]);
+          if (!C::FUSE) {
+            const float4 e0 = e[2 * j], e1 = e[2 * j + 1];
+            z[0] += e0.x; z[1] += e0.y; z[2] += e0.z; z[3] += e0.w;
+            z[4] += e1.x; z[5] += e1.y; z[6] += e1.z; z[7] += e1.w;
+          }
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] = pack_bf16(fmaf(-hsum, bf16_lo(xw[k]), z[2 * k]), fmaf(-hsum, bf16_hi(xw[k]), z[2 * k + 1]));
+          *at = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        ++rp;
+        fence_async_smem();
+        warp_arrive(bars + C::STAGED, lane);
       }
     }
-    if (tid == 0) tma_store_wait_all();
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -1535,6 +1644,7 @@ cudaError_t launch_feat(const Host& h) {
   a.beta = h.at<float>(h.ws.fwd.beta);
   a.n2 = h.at<float>(h.ws.n2);
   a.delta = h.at<float>(h.ws.delta);
+  a.off = h.at<float>(h.ws.off[SIDE]);
   a.partial = h.at<float>(h.ws.partial);
   a.status = h.at<int>(h.ws.fwd.status);
   a.H = h.p.H;
@@ -1549,7 +1659,8 @@ cudaError_t launch_feat(const Host& h) {
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int64_t n = (int64_t)BH * C::M;
   bwd_combine_kernel<D><<<(unsigned)div_up(n * (D / 4 + 1), 256), 256, 0, h.st>>>(
-      a.partial, a.nsplit, n, C::M, h.at<__nv_bfloat16>(h.ws.sum[SIDE]), h.at<float>(h.ws.sum1[SIDE]));
+      a.partial, a.nsplit, n, C::M, h.at<__nv_bfloat16>(h.ws.sum[SIDE]), h.at<__nv_bfloat16>(h.ws.sum_lo[SIDE]),
+      h.at<float>(h.ws.sum1[SIDE]));
   return cudaGetLastError();
 }
 
@@ -1558,7 +1669,7 @@ cudaError_t launch_side(const Host& h, void* dx, int64_t ob, int64_t orow, int64
   constexpr int OTHER = 1 - SIDE;
   const int BH = h.p.B * h.p.H;
   cudaError_t e;
-  {
+  if constexpr (D == 128) {
     using C = WinCfg<D>;
     WinArgs a{};
     if (!h.map_x(&a.tm_x, SIDE, 128) || !h.map_y(&a.tm_y, SIDE, 128) || !h.map_x(&a.tm_xo, OTHER, 64) ||
@@ -1571,31 +1682,33 @@ cudaError_t launch_side(const Host& h, void* dx, int64_t ob, int64_t orow, int64
     a.status = h.at<int>(h.ws.fwd.status);
     a.Tp = h.ws.Tp;
     a.tau = h.p.softmax_temp;
-    if ((e = allow_smem(bwd_window_kernel<SIDE, D>, C::SMEM, &h.dev->attr_bwd[D == 128][1][SIDE])) != cudaSuccess) return e;
+    if ((e = allow_smem(bwd_window_kernel<SIDE, D>, C::SMEM, &h.dev->attr_bwd[1][1][SIDE])) != cudaSuccess) return e;
     bwd_window_kernel<SIDE, D><<<(unsigned)(a.g.ntiles < h.dev->sms ? a.g.ntiles : h.dev->sms), C::NTHR, C::SMEM, h.st>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
-  using C = LowCfg<D>;
-  LowArgs a{};
-  if (!h.map_y(&a.tm_y, SIDE, 128) || !h.map_y(&a.tm_yo, OTHER, 64) ||
-      !map_rows(&a.tm_fo, h.at<void>(h.ws.feat[OTHER]), C::M, h.side[OTHER].rows, BH, 64) ||
+  using C = GradCfg<D>;
+  GradArgs a{};
+  if (!h.map_x(&a.tm_x, SIDE, 128) || !h.map_y(&a.tm_y, SIDE, 128) || !h.map_x(&a.tm_xo, OTHER, 64) ||
+      !h.map_y(&a.tm_yo, OTHER, 64) || !map_rows(&a.tm_fo, h.at<void>(h.ws.feat[OTHER]), C::M, h.side[OTHER].rows, BH, 64) ||
       !map_rows(&a.tm_sum, h.at<void>(h.ws.sum[OTHER]), D, C::M, BH, 128) ||
+      !map_rows(&a.tm_sum_lo, h.at<void>(h.ws.sum_lo[OTHER]), D, C::M, BH, 128) ||
       !map_w(&a.tm_hi, h.at<void>(h.ws.fwd.phiq), D, 128) || !map_w(&a.tm_lo, h.at<void>(h.ws.wlo), D, 128) ||
-      !map_rows(&a.tm_f, h.at<void>(h.ws.feat[SIDE]), C::M, h.side[SIDE].rows, BH, 128) || !h.map_x(&a.tm_x, SIDE, 128) ||
       !map_bthe(&a.tm_dx, dx, h.p.B, h.side[SIDE].rows, h.p.H, D, ob, orow, oh, 128))
     return cudaErrorInvalidValue;
   a.g = h.geom(SIDE);
-  a.sum1 = h.at<float>(h.ws.sum1[OTHER]);
+  a.n2 = h.at<float>(h.ws.n2);
   a.delta = h.at<float>(h.ws.delta);
-  a.part = h.at<float>(h.ws.part);
+  a.off = h.at<float>(h.ws.off[SIDE]);
+  a.sum1 = h.at<float>(h.ws.sum1[OTHER]);
+  a.part = D == 128 ? h.at<float>(h.ws.part) : nullptr;
   a.status = h.at<int>(h.ws.fwd.status);
   a.Tp = h.ws.Tp;
   // Few columns: the sum over those outside the window instead of all - inside (accuracy, see the top).  It visits
   // every column, so it is used while that is at most the window's own steps and four more.
   a.whole = div_up(h.side[OTHER].rows, 64) <= div_up((int64_t)a.g.w + TR, 64) + 4;
   a.tau = h.p.softmax_temp;
-  if ((e = allow_smem(bwd_lowrank_kernel<SIDE, D>, C::SMEM, &h.dev->attr_bwd[D == 128][2][SIDE])) != cudaSuccess) return e;
-  bwd_lowrank_kernel<SIDE, D><<<(unsigned)(a.g.ntiles < h.dev->sms ? a.g.ntiles : h.dev->sms), C::NTHR, C::SMEM, h.st>>>(a);
+  if ((e = allow_smem(bwd_grad_kernel<SIDE, D>, C::SMEM, &h.dev->attr_bwd[D == 128][2][SIDE])) != cudaSuccess) return e;
+  bwd_grad_kernel<SIDE, D><<<(unsigned)(a.g.ntiles < h.dev->sms ? a.g.ntiles : h.dev->sms), C::NTHR, C::SMEM, h.st>>>(a);
   return cudaGetLastError();
 }
 
@@ -1680,7 +1793,9 @@ void tc_plan_backward(const SblParams& p, TcBwdWorkspace* ws) {
   size_t partial = 0;
   for (int s = 0; s < 2; ++s) {
     ws->sum[s] = take(BH * m * D * 2);
+    ws->sum_lo[s] = take(BH * m * D * 2);
     ws->sum1[s] = take(BH * m * 4);
+    ws->off[s] = take(BH * div_up(s == QUERIES ? p.T : p.S, TR) * TR * 4);
     // one CTA per SM at a time: the fewest rounds of tiles over whole waves of CTAs; a CTA's prologue and its partial
     // summary cost about as much as three tiles
     const int ntiles = (int)div_up(s == QUERIES ? p.T : p.S, TR);
@@ -1699,7 +1814,7 @@ void tc_plan_backward(const SblParams& p, TcBwdWorkspace* ws) {
     partial = bytes > partial ? bytes : partial;
   }
   ws->partial = take(partial);
-  ws->part = take(BH * div_up(T > S ? T : S, TR) * TR * D * 4);
+  ws->part = p.E == 128 ? take(BH * div_up(T > S ? T : S, TR) * TR * D * 4) : off;
   f.total = off;
 }
 

@@ -28,7 +28,7 @@ struct DeviceInfo {
   bool attr_band[2] = {false, false};   // without, with row statistics
   bool attr_keys128 = false;
   bool attr_band128[2] = {false, false};
-  bool attr_bwd[2][4][2] = {};          // head dim 64 / 128; features, window, low-rank, value; side
+  bool attr_bwd[2][4][2] = {};          // head dim 64 / 128; features, window, grad, value; side
 };
 cudaError_t device_info(DeviceInfo** out);
 
