@@ -104,7 +104,8 @@ cudaError_t tc_band(const SblParams& p, const Workspace& ws, char* base, const f
 struct TcBwdWorkspace {
   Workspace fwd;            // status (offset 0), wt, phiq = Wt in bf16, beta; total
   size_t wlo;               // what is left of Wt, in bf16
-  size_t n2, delta;         // (BH,Tp)
+  size_t nd;                // (BH,Tp) float2: log-normaliser (base 2) and delta of every query row
+  size_t delta;             // head dim 128: (BH,Tp), the second of nd
   size_t feat[2];           // psi (BH,T,m), phi (BH,S,m) bf16
   size_t sum[2], sum_lo[2]; // (BH,m,D): two bf16 terms of the summary
   size_t sum1[2];           // (BH,m) fp32: its extra column

@@ -120,6 +120,12 @@ __device__ __forceinline__ void wait_inline(uint64_t* bar, uint32_t parity, int*
     }
   }
 }
+// untiled bulk copy to shared memory: both addresses and the size are multiples of 16 bytes
+__device__ __forceinline__ void bulk_load(void* smem, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 // start-address steps (in 16-byte units) of K step k inside a K-major operand of [rows][64] pieces
 __device__ __forceinline__ uint64_t kmajor(int k, uint32_t piece_bytes) {
   return (uint64_t)((uint32_t)(k >> 2) * (piece_bytes >> 4) + (uint32_t)(k & 3) * 2);
@@ -128,12 +134,13 @@ __device__ __forceinline__ uint64_t kmajor(int k, uint32_t piece_bytes) {
 __device__ __forceinline__ uint32_t packed(int k) { return 32u * (uint32_t)(k >> 1) + 8u * (uint32_t)(k & 1); }
 
 // ---------------------------------------------------------------------------
-// Per query row: n2 = log-normaliser * log2(e), delta = dout . out; both (BH, Tp), zero in the padding rows.
+// Per query row: (log-normaliser * log2(e), delta = dout . out), (BH, Tp); zero in the padding rows.  Head dim 128:
+// delta once more by itself.
 // D / 8 lanes per row, four rows per group of lanes with all their loads in flight.
 template <int D>
 __global__ void __launch_bounds__(256) bwd_rows_kernel(const __nv_bfloat16* out, int64_t ob, int64_t ot, int64_t oh,
                                                        const __nv_bfloat16* dout, int64_t db, int64_t dt, int64_t dh,
-                                                       const float* stats, int B, int H, int T, int Tp, float* n2,
+                                                       const float* stats, int B, int H, int T, int Tp, float2* nd,
                                                        float* delta) {
   constexpr int LPR = D / 8, RPB = 256 / LPR;
   const int sub = threadIdx.x % LPR;
@@ -167,8 +174,8 @@ __global__ void __launch_bounds__(256) bwd_rows_kernel(const __nv_bfloat16* out,
       const int64_t bh = (int64_t)b[u] * H + h[u];
       float n = 0.f;
       if (t[u] < T) n = stats[bh * T + t[u]] * kLog2e + log2f(stats[rows + bh * T + t[u]]);
-      n2[bh * Tp + t[u]] = n;
-      delta[bh * Tp + t[u]] = s;
+      nd[bh * Tp + t[u]] = make_float2(n, s);
+      if (D == 128) delta[bh * Tp + t[u]] = s;
     }
   }
 }
@@ -178,7 +185,8 @@ __global__ void __launch_bounds__(256) bwd_rows_kernel(const __nv_bfloat16* out,
 struct FeatArgs {
   CUtensorMap tm_x, tm_y, tm_hi, tm_lo, tm_f;
   const int64_t* lengths;
-  const float *beta, *n2, *delta;   // (BH); (BH, Tp)
+  const float* beta;                // (BH)
+  const float2* nd;                 // (BH, Tp): log-normaliser (base 2) and delta of every query row
   float* off;                       // (BH, rows padded to tiles): exponent offset (base 2) of every row, -inf if padding
   float* partial;                   // (BH, nsplit, m, D + 4)
   int* status;
@@ -355,8 +363,9 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
         off = (-g - a.half_log_m - beta) * kLog2e;
       } else {
         // r < Tp: the row arrays are padded to whole tiles
-        off = (-g - a.half_log_m + beta) * kLog2e - __ldg(a.n2 + (int64_t)bh * a.Tp + r);
-        dl = __ldg(a.delta + (int64_t)bh * a.Tp + r);
+        const float2 nd = __ldg(a.nd + (int64_t)bh * a.Tp + r);
+        off = (-g - a.half_log_m + beta) * kLog2e - nd.x;
+        dl = nd.y;
       }
       if (fb == 0 && cq == 0) a.off[((int64_t)bh * ntiles + t_lo + i) * TR + row] = live ? off : -INFINITY;
       mbar_wait(u_full + s, (i >> 1) & 1, a.status, 209);   // U computed: the X tile has been read too
@@ -456,7 +465,7 @@ __global__ void __launch_bounds__(256) bwd_combine_kernel(const float* partial, 
 struct WinArgs {
   CUtensorMap tm_x, tm_y, tm_xo, tm_yo;   // own side (128 rows), other side (64 rows)
   Geom g;
-  const float *n2, *delta;                // (BH, Tp)
+  const float2* nd;                       // (BH, Tp)
   float* part;                            // (tiles, D / 4, 128 rows) float4
   int* status;
   int Tp;
@@ -608,13 +617,9 @@ __global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constan
     for (int tile = blockIdx.x; tile < a.g.ntiles; tile += step) {
       const RowTile t = row_tile<SIDE, 64>(a.g, tile, false);
       const int r = t.r0 + row;
-      const float* n2 = a.n2 + (int64_t)t.bh * a.Tp;
-      const float* dl = a.delta + (int64_t)t.bh * a.Tp;
-      float rn = 0.f, rd = 0.f;
-      if (SIDE == QUERIES) {
-        rn = __ldg(n2 + r);
-        rd = __ldg(dl + r);
-      }
+      const float2* nd = a.nd + (int64_t)t.bh * a.Tp;
+      float2 own = make_float2(0.f, 0.f);
+      if (SIDE == QUERIES) own = __ldg(nd + r);
       for (int s = 0; s < t.n; ++s, ++g) {
         if ((g & 1) != grp) continue;
         const int c = t.c0 + 64 * s + 32 * cq;
@@ -630,13 +635,13 @@ __global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constan
           tmem_ld_wait();
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
-            float4 cn = make_float4(rn, rn, rn, rn), cd = make_float4(rd, rd, rd, rd);
+            float4 n01 = make_float4(own.x, own.y, own.x, own.y), n23 = n01;
             if (SIDE == KEYS) {
               // c < Tp: the row arrays are padded to whole tiles
-              cn = __ldg(reinterpret_cast<const float4*>(n2 + c) + q);
-              cd = __ldg(reinterpret_cast<const float4*>(dl + c) + q);
+              n01 = __ldg(reinterpret_cast<const float4*>(nd + c) + 2 * q);
+              n23 = __ldg(reinterpret_cast<const float4*>(nd + c) + 2 * q + 1);
             }
-            const float nn[4] = {cn.x, cn.y, cn.z, cn.w}, dd[4] = {cd.x, cd.y, cd.z, cd.w};
+            const float nn[4] = {n01.x, n01.z, n23.x, n23.z}, dd[4] = {n01.y, n01.w, n23.y, n23.w};
             float v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -702,7 +707,8 @@ __global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constan
 struct GradArgs {
   CUtensorMap tm_x, tm_y, tm_xo, tm_yo, tm_fo, tm_sum, tm_sum_lo, tm_hi, tm_lo, tm_dx;
   Geom g;
-  const float *n2, *delta;                 // (BH, Tp)
+  const float2* nd;                        // (BH, Tp)
+  const float* delta;                      // (BH, Tp): the second of nd
   const float* off;                        // (BH, rows padded): exponent offsets of the own features
   const float* sum1;                       // (BH, m): extra column of the other side's summary
   const float* part;                       // head dim 128: (tiles, D / 4, 128 rows) float4
@@ -728,21 +734,27 @@ struct GradCfg {
   static constexpr uint32_t CSLOT = 16384;               // Y' of a step, and X' (head dim 64)
   static constexpr uint32_t OFF_X = 0, OFF_Y = XBUF * TB, OFF_SUM = OFF_Y + TB;
   static constexpr uint32_t OFF_W = FUSE ? OFF_SUM + AUX : OFF_SUM;   // head dim 128: one buffer for both, in turn
-  static constexpr uint32_t OFF_F = OFF_W + AUX, OFF_C = OFF_F + NF * 32768, OFF_S1 = OFF_C + NC * CSLOT;
-  static constexpr uint32_t OFF_BAR = OFF_S1 + 2048, SMEM = OFF_BAR + 256 + 768;   // (the base is 256-byte aligned)
-  static constexpr int NCOMP = 512, NTHR = NCOMP + 96, W_LOAD = 16, W_MMA = 17, W_STORE = 18;
+  static constexpr uint32_t OFF_F = OFF_W + AUX, OFF_C = OFF_F + NF * 32768;
+  // per step, 64 columns of (n2, delta); head dim 128: of delta, in four slots, because there a column tile is freed
+  // when G has been formed, with G itself still to be read (the load of step g + 4 is behind the products of step g)
+  static constexpr int NND = FUSE ? NC : 4;
+  static constexpr uint32_t NDB = FUSE ? 512 : 256;
+  static constexpr uint32_t OFF_ND = OFF_C + NC * CSLOT, OFF_S1 = OFF_ND + NND * NDB;   // then sum1 of the unit
+  static constexpr uint32_t OFF_BAR = OFF_S1 + 1024, SMEM = OFF_BAR + 320;   // (the base is 1024-byte aligned)
+  static constexpr int NCOMP = 512, NTHR = NCOMP + 128, W_LOAD = 16, W_STORE = 17, W_MMA_A = 18, W_MMA_B = 19;
   static constexpr uint32_t T_DF = 0, T_DX = 256, T_G = FUSE ? 320 : 384, T_S = 448;
   enum { X_FULL = 0, X_FREE = 2, Y_FULL = 4, Y_FREE, SUM_FULL, SUM_FREE, W_FULL, W_FREE, F_FULL, F_FREE = F_FULL + NF,
-         C_FULL = F_FREE + NF, C_FREE = C_FULL + NC, T_FULL = C_FREE + NC, S_READ = T_FULL + 2, G_DONE = S_READ + 2,
-         DF_FULL = G_DONE + 2, DU_DONE, DX_FULL, DX_FREE, STAGED, COUNT };
-  static_assert(SMEM <= 232448 && COUNT * 8 + 4 <= 256, "shared memory of one CTA");
+         C_FULL = F_FREE + NF, C_FREE = C_FULL + NC, T_FULL = C_FREE + NC, G_FREE = T_FULL + 2, S_READ = G_FREE + 2,
+         G_DONE = S_READ + 2, DF_FULL = G_DONE + 2, DU_DONE, DX_FULL, DX_FREE, STAGED, ND_FULL,
+         COUNT = ND_FULL + (FUSE ? 0 : NND) };
+  static_assert(SMEM <= 232448 && COUNT * 8 + 4 <= 320, "shared memory of one CTA");
 };
 
 template <int SIDE, int D>
-__global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant__ GradArgs a) {
+__global__ void __launch_bounds__(640, 1) bwd_grad_kernel(const __grid_constant__ GradArgs a) {
   using C = GradCfg<D>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = align1024(smem_raw);
+  uint8_t* smem = smem_raw;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::COUNT);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -750,7 +762,8 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
     for (int i = 0; i < C::COUNT; ++i) {
       const bool group = i >= C::S_READ && i < C::DF_FULL;
       const bool all = i == C::DU_DONE || i == C::DX_FREE || i == C::STAGED;
-      mbar_init(bars + i, group ? 8 : all ? 16 : 1);
+      const bool both = i == C::DF_FULL || i == C::Y_FREE;   // one commit of either issuing warp
+      mbar_init(bars + i, group ? 8 : all ? 16 : both ? 2 : 1);
     }
     fence_mbar_init();
   }
@@ -762,7 +775,7 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
   __syncthreads();
   tc_fence_after_sync();
   constexpr uint32_t tb = 0;
-  if (tid == 0 && *tmem_slot != 0) atomicCAS(a.status, 0, 241);
+  if (tid == 0 && (*tmem_slot != 0 || (smem_u32(smem) & 1023) != 0)) atomicCAS(a.status, 0, 241);
   const int step = gridDim.x;
   const bool whole = a.whole != 0;
   const int n_it = (a.g.ntiles - (int)blockIdx.x + step - 1) / step, n_u = n_it * C::PASS;
@@ -788,7 +801,16 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
         ++nc;
         if (leader) {
           uint8_t* dst = smem + C::OFF_C + slot * C::CSLOT;
-          mbar_expect_tx(bars + C::C_FULL + slot, C::CSLOT);
+          mbar_expect_tx(bars + C::C_FULL + slot, C::CSLOT + (SIDE == KEYS && C::FUSE ? C::NDB : 0));
+          if (SIDE == KEYS) {
+            const int d = (nc - 1) % C::NND;
+            uint64_t* bar = bars + (C::FUSE ? C::C_FULL + slot : C::ND_FULL + d);
+            if (!C::FUSE) mbar_expect_tx(bar, C::NDB);
+            // c0 + 64 s + 63 < Tp: the row arrays are padded to whole tiles
+            const int64_t at = (int64_t)t.bh * a.Tp + t.c0 + 64 * s;
+            bulk_load(smem + C::OFF_ND + d * C::NDB,
+                      C::FUSE ? static_cast<const void*>(a.nd + at) : static_cast<const void*>(a.delta + at), C::NDB, bar);
+          }
           for (int j = 0; j < C::NB; ++j)
             tma_load_4d(dst + j * 8192, &a.tm_yo, bars + C::C_FULL + slot, 64 * j, t.c0 + 64 * s, t.h, t.b);
           if (C::FUSE) tma_load_4d(dst + 8192, &a.tm_xo, bars + C::C_FULL + slot, 0, t.c0 + 64 * s, t.h, t.b);
@@ -863,30 +885,25 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
       if (!C::FUSE && pass == 0) load_x();
     }
     __syncwarp();
-  } else if (warp == C::W_MMA) {
+  } else if (warp == C::W_MMA_A) {
+    // ---- issuer A: G, S, U.  (Two issuing warps: each spends as long on waits and descriptors as on its products.)
     const bool leader = elect_one();
     constexpr uint32_t id_t = idesc_bf16(128, 64, false, false);
-    constexpr uint32_t id_df = idesc_bf16(128, 256, false, true);
-    constexpr uint32_t id_sum = idesc_bf16(128, 256, false, false);
     constexpr uint32_t id_u = idesc_bf16(128, 128, false, false);
-    constexpr uint32_t id_dx = idesc_bf16(128, D, false, true);
     const uint64_t dX = smem_desc_sw128(smem_u32(smem + C::OFF_X), 16, 1024);
     const uint64_t dY = smem_desc_sw128(smem_u32(smem + C::OFF_Y), 16, 1024);
     const uint64_t dC = smem_desc_sw128(smem_u32(smem + C::OFF_C), 16, 1024);
-    const uint64_t dCt = smem_desc_sw128(smem_u32(smem + C::OFF_C + 8192), 8192, 1024);   // X', MN-major
-    const uint64_t dF = smem_desc_sw128(smem_u32(smem + C::OFF_F), 8192, 1024);
-    const uint64_t dSum = smem_desc_sw128(smem_u32(smem + C::OFF_SUM), 16, 1024);
-    const uint64_t dWk = smem_desc_sw128(smem_u32(smem + C::OFF_W), 16, 1024);
-    const uint64_t dWt = smem_desc_sw128(smem_u32(smem + C::OFF_W), 16384, 1024);
-    int g0 = 0, ns = 0;             // number of the unit's first step; summary terms so far
+    const uint64_t dW = smem_desc_sw128(smem_u32(smem + C::OFF_W), 16, 1024);
+    int g0 = 0;                     // number of the unit's first step in the CTA's stream of steps
     for (int u = 0; u < n_u; ++u) {
       const int it = u / C::PASS, pass = u % C::PASS, xb = it % C::XBUF;
       const int n = row_tile<SIDE, 64>(a.g, blockIdx.x + it * step, whole).n;
       const uint64_t x = dX + (uint64_t)(xb * (C::TB >> 4));
-      // G = Y Y'^T of step s; gg: its number in the CTA's stream of steps
+      // G = Y Y'^T of step gg, into the buffer that the products of step gg - 2 have left
       auto issue_g = [&](int gg) {
         const int slot = gg % C::NC;
         wait_inline(bars + C::C_FULL + slot, (gg / C::NC) & 1, a.status, 271);
+        if (gg >= 2) wait_inline(bars + C::G_FREE + (gg & 1), ((gg >> 1) - 1) & 1, a.status, 272);
         tc_fence_after_sync();
         if (leader) {
           const uint64_t o = dC + (uint64_t)(slot * (C::CSLOT >> 4));
@@ -900,7 +917,7 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
         }
         __syncwarp();
       };
-      // S = X X'^T; its column tile is that of the G product issued before
+      // S = X X'^T; its column tile is that of a G product issued before
       auto issue_s = [&](int gg) {
         if (leader) {
           const uint64_t o = dC + (uint64_t)((gg % C::NC) * (C::CSLOT >> 4) + 512);
@@ -910,14 +927,61 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
         }
         __syncwarp();
       };
+      // U of the unit before has been read
+      if (u >= 1) wait_inline(bars + C::DU_DONE, (u - 1) & 1, a.status, 273);
+      if (pass == 0) wait_inline(bars + C::Y_FULL, it & 1, a.status, 274);
+      if (C::FUSE) wait_inline(bars + C::X_FULL + xb, (it / C::XBUF) & 1, a.status, 275);
+      if (n > 0) issue_g(g0);
+      if (C::FUSE && n > 0) issue_s(g0);
+      if (n > 1) issue_g(g0 + 1);
+      for (int s = 0; s < n; ++s) {
+        const int gg = g0 + s;
+        if (C::FUSE && s + 1 < n) {
+          wait_inline(bars + C::S_READ + (gg & 1), (gg >> 1) & 1, a.status, 276);
+          tc_fence_after_sync();
+          issue_s(gg + 1);
+        }
+        if (s + 2 < n) issue_g(gg + 2);
+      }
+      g0 += n;
+      // U of the own features over the G buffers, for du: the products of the last two steps have to be done
+      for (int gg = g0 - 2 > 0 ? g0 - 2 : 0; gg < g0; ++gg)
+        wait_inline(bars + C::G_FREE + (gg & 1), (gg >> 1) & 1, a.status, 277);
+      wait_inline(bars + C::W_FULL, C::FUSE ? 0 : u & 1, a.status, 279);
+      if (!C::FUSE && pass == 0) wait_inline(bars + C::X_FULL + xb, (it / C::XBUF) & 1, a.status, 280);
+      tc_fence_after_sync();
+      if (leader) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_ss(tb + C::T_G, x + kmajor(k, 16384), dW + (uint64_t)(t * (C::AUX >> 5)) + kmajor(k, 16384), id_u,
+                   t > 0 || k > 0);
+        if (pass == C::PASS - 1) mma_commit(bars + C::Y_FREE);
+        mma_commit(bars + C::DF_FULL);
+      }
+      __syncwarp();
+    }
+  } else if (warp == C::W_MMA_B) {
+    // ---- issuer B: df, dx
+    const bool leader = elect_one();
+    constexpr uint32_t id_df = idesc_bf16(128, 256, false, true);
+    constexpr uint32_t id_sum = idesc_bf16(128, 256, false, false);
+    constexpr uint32_t id_dx = idesc_bf16(128, D, false, true);
+    const uint64_t dY = smem_desc_sw128(smem_u32(smem + C::OFF_Y), 16, 1024);
+    const uint64_t dCt = smem_desc_sw128(smem_u32(smem + C::OFF_C + 8192), 8192, 1024);   // X', MN-major
+    const uint64_t dF = smem_desc_sw128(smem_u32(smem + C::OFF_F), 8192, 1024);
+    const uint64_t dSum = smem_desc_sw128(smem_u32(smem + C::OFF_SUM), 16, 1024);
+    const uint64_t dWt = smem_desc_sw128(smem_u32(smem + C::OFF_W), 16384, 1024);
+    int g0 = 0, ns = 0;             // number of the unit's first step; summary terms so far
+    for (int u = 0; u < n_u; ++u) {
+      const int it = u / C::PASS, pass = u % C::PASS;
+      const int n = row_tile<SIDE, 64>(a.g, blockIdx.x + it * step, whole).n;
       bool fresh = true;            // df of this unit has not been written to
-      auto touch = [&]() {          // before its first product: the previous tile's dx (and what lies in df) has been read
-        if (fresh && pass == 0 && it >= 1) wait_inline(bars + C::DX_FREE, (it - 1) & 1, a.status, 272);
-      };
       int sums = whole ? 2 : 0;
       auto issue_sum = [&]() {      // df += Y summary^T, one term
-        touch();
-        wait_inline(bars + C::SUM_FULL, ns & 1, a.status, 273);
+        if (pass == 0 && sums == 0) wait_inline(bars + C::Y_FULL, it & 1, a.status, 291);
+        wait_inline(bars + C::SUM_FULL, ns & 1, a.status, 292);
         ++ns;
         tc_fence_after_sync();
         if (leader) {
@@ -930,22 +994,11 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
         fresh = false;
         ++sums;
       };
-      if (pass == 0) wait_inline(bars + C::Y_FULL, it & 1, a.status, 274);
-      if (C::FUSE) wait_inline(bars + C::X_FULL + xb, (it / C::XBUF) & 1, a.status, 275);
-      if (n > 0) {
-        issue_g(g0);
-        if (C::FUSE) issue_s(g0);
-        if (n > 1) issue_g(g0 + 1);
-      }
+      // the previous tile's dx, and what lies in df beside it, has been read
+      if (pass == 0 && it >= 1) wait_inline(bars + C::DX_FREE, (it - 1) & 1, a.status, 293);
       for (int s = 0; s < n; ++s) {
         const int gg = g0 + s, slot = gg % C::NF;
-        if (C::FUSE && s + 1 < n) {
-          wait_inline(bars + C::S_READ + (gg & 1), (gg >> 1) & 1, a.status, 276);
-          tc_fence_after_sync();
-          issue_s(gg + 1);
-        }
-        wait_inline(bars + C::F_FULL + slot, (gg / C::NF) & 1, a.status, 277);
-        touch();
+        wait_inline(bars + C::F_FULL + slot, (gg / C::NF) & 1, a.status, 294);
         wait_inline(bars + C::G_DONE + (gg & 1), (gg >> 1) & 1, a.status, 278);
         tc_fence_after_sync();
         if (leader) {
@@ -961,32 +1014,22 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
                      dCt + (uint64_t)((gg % C::NC) * (C::CSLOT >> 4) + k * 128), id_dx, s > 0 || k > 0);
             mma_commit(bars + C::C_FREE + gg % C::NC);
           }
+          mma_commit(bars + C::G_FREE + (gg & 1));
         }
         __syncwarp();
         fresh = false;
-        if (s + 2 < n) issue_g(gg + 2);
         if (sums < 2) issue_sum();
       }
       while (sums < 2) issue_sum();
       g0 += n;
-      // U of the own features over the G buffers, for du
-      wait_inline(bars + C::W_FULL, C::FUSE ? 0 : u & 1, a.status, 279);
-      if (!C::FUSE && pass == 0) wait_inline(bars + C::X_FULL + xb, (it / C::XBUF) & 1, a.status, 280);
-      tc_fence_after_sync();
       if (leader) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            mma_ss(tb + C::T_G, x + kmajor(k, 16384), dWk + (uint64_t)(t * (C::AUX >> 5)) + kmajor(k, 16384), id_u,
-                   t > 0 || k > 0);
         if (pass == C::PASS - 1) mma_commit(bars + C::Y_FREE);
         mma_commit(bars + C::DF_FULL);
       }
       __syncwarp();
+      wait_inline(bars + C::W_FULL, C::FUSE ? 0 : u & 1, a.status, 295);
       wait_inline(bars + C::DU_DONE, u & 1, a.status, 281);
       const bool first = pass == 0 && !(C::FUSE && n > 0);   // nothing of this tile is in dx yet
-      if (first && it >= 1) wait_inline(bars + C::DX_FREE, (it - 1) & 1, a.status, 282);
       tc_fence_after_sync();
       if (leader) {
         // du Wt: high x high, high x low, low x high; du's low term lies behind its high one
@@ -1025,25 +1068,30 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
     const int grp = warp >> 3, qd = warp & 3, cq = (warp >> 2) & 1;
     const int row = qd * 32 + lane;
     const uint32_t lane_base = tb + ((uint32_t)(qd * 32) << 16);
-    float* s_s1 = reinterpret_cast<float*>(smem + C::OFF_S1);    // [2][256], by parity of the unit
+    float* s_s1 = reinterpret_cast<float*>(smem + C::OFF_S1);
     const float sc = a.tau * kLog2e;
     const float lt = log2f(a.tau);
     int gg = 0;
     float hs = 0.f;
+    // What a thread needs of a tile's row, fetched while the tile before is still being finished
+    RowTile t = row_tile<SIDE, 64>(a.g, blockIdx.x, whole);
+    float off, rn = 0.f, rd = 0.f;
+    auto fetch_row = [&]() {
+      const int r = t.r0 + row;     // (the row arrays are padded to whole tiles)
+      off = __ldg(a.off + (int64_t)t.bh * a.g.ntr * TR + r);
+      if (SIDE == QUERIES) {
+        const float2 v = __ldg(a.nd + (int64_t)t.bh * a.Tp + r);   // (r < Tp)
+        rn = v.x - lt;              // tau p = 2^(S sc - (n2 - log2 tau))
+        rd = v.y;
+      }
+    };
+    fetch_row();
     for (int u = 0; u < n_u; ++u) {
       const int it = u / C::PASS, pass = u % C::PASS;
       const int tile = blockIdx.x + it * step;
-      const RowTile t = row_tile<SIDE, 64>(a.g, tile, whole);
       const int r = t.r0 + row;
-      const float* n2 = a.n2 + (int64_t)t.bh * a.Tp;
-      const float* dl = a.delta + (int64_t)t.bh * a.Tp;
-      const float off = __ldg(a.off + ((int64_t)t.bh * a.g.ntr) * TR + r);
-      float rn = 0.f, rd = 0.f;
-      if (SIDE == QUERIES) {
-        rn = __ldg(n2 + r) - lt;    // tau p = 2^(S sc - (n2 - log2 tau))
-        rd = __ldg(dl + r);
-      }
-      if (tid < 256) s_s1[256 * (u & 1) + tid] = __ldg(a.sum1 + (int64_t)t.bh * C::M + 256 * pass + tid);
+      float sum1 = 0.f;
+      if (tid < 256) sum1 = __ldg(a.sum1 + (int64_t)t.bh * C::M + 256 * pass + tid);
       for (int s = 0; s < t.n; ++s, ++gg) {
         if ((gg & 1) != grp) continue;
         const int c = t.c0 + 64 * s + 32 * cq;
@@ -1055,6 +1103,10 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
         uint32_t x[32], y[32];
         if (C::FUSE) tmem_ld32(lane_base + C::T_S + 32 * cq, x);
         tmem_ld32(tg, y);
+        const float4* nd = reinterpret_cast<const float4*>(smem + C::OFF_ND + (gg % C::NND) * C::NDB + cq * (C::NDB / 2));
+        // head dim 64: landed with the step's tile, which is held until its products are done
+        if (SIDE == KEYS && C::FUSE) mbar_wait(bars + C::C_FULL + gg % C::NC, (gg / C::NC) & 1, a.status, 285);
+        if (SIDE == KEYS && !C::FUSE) mbar_wait(bars + C::ND_FULL + (gg & 3), (gg >> 2) & 1, a.status, 283);
         tmem_ld_wait();
         if (C::FUSE) {
           tc_fence_before_sync();
@@ -1063,13 +1115,16 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
         uint32_t o[16], e[16];
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          float4 cn = make_float4(rn, rn, rn, rn), cd = make_float4(rd, rd, rd, rd);
-          if (SIDE == KEYS) {
-            // c < Tp: the row arrays are padded to whole tiles
-            if (C::FUSE) cn = __ldg(reinterpret_cast<const float4*>(n2 + c) + q);
-            cd = __ldg(reinterpret_cast<const float4*>(dl + c) + q);
+          float4 n01 = make_float4(rn, rd, rn, rd), n23 = n01;
+          if (SIDE == KEYS && C::FUSE) {
+            n01 = nd[2 * q];
+            n23 = nd[2 * q + 1];
+          } else if (SIDE == KEYS) {
+            const float4 v = nd[q];
+            n01 = make_float4(0.f, v.x, 0.f, v.y);
+            n23 = make_float4(0.f, v.z, 0.f, v.w);
           }
-          const float nn[4] = {cn.x, cn.y, cn.z, cn.w}, dd[4] = {cd.x, cd.y, cd.z, cd.w};
+          const float nn[4] = {n01.x, n01.z, n23.x, n23.z}, dd[4] = {n01.y, n01.w, n23.y, n23.w};
           float v[4], w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -1097,8 +1152,13 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
       const bool none = whole && t.n == 0;
       const float d1 = whole ? 0.f : (SIDE == QUERIES ? rd : 1.f);
       if (pass == 0) hs = 0.f;
-      asm volatile("bar.sync 1, 512;" ::: "memory");   // sum1 of the unit is in shared memory
-      const float* s1 = s_s1 + 256 * (u & 1) + 128 * grp + 32 * cq;
+      if (tid < 256) {
+        // (every reader of the unit before is through; head dim 64: a tile has one unit, and its dx was waited for)
+        if (!C::FUSE && u >= 1) mbar_wait(bars + C::DU_DONE, (u - 1) & 1, a.status, 284);
+        s_s1[tid] = sum1;
+      }
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+      const float* s1 = s_s1 + 128 * grp + 32 * cq;
       const uint32_t td = lane_base + C::T_DF + 128 * grp + 32 * cq;
       mbar_wait(bars + C::DF_FULL, u & 1, a.status, 287);
       tc_fence_after_sync();
@@ -1141,6 +1201,10 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
           const float4* part = reinterpret_cast<const float4*>(a.part) + ((int64_t)tile * (D / 4) + c / 4) * TR + row;
 #pragma unroll
           for (int j = 0; j < NQ / 4; ++j) e[j] = __ldg(part + j * TR);
+        }
+        if (it + 1 < n_it) {
+          t = row_tile<SIDE, 64>(a.g, tile + step, whole);
+          fetch_row();
         }
         mbar_wait(bars + C::X_FULL + buf, (it / C::XBUF) & 1, a.status, 288);
         mbar_wait(bars + C::DX_FULL, it & 1, a.status, 289);
@@ -1192,7 +1256,7 @@ __global__ void __launch_bounds__(608, 1) bwd_grad_kernel(const __grid_constant_
 struct ValArgs {
   CUtensorMap tm_k, tm_q, tm_do, tm_phi, tm_psi, tm_sum;
   Geom g;
-  const float* n2;                         // (BH, Tp)
+  const float2* nd;                        // (BH, Tp)
   __nv_bfloat16* dv; int64_t vb, vs, vh;
   int* status;
   int Tp;
@@ -1493,7 +1557,7 @@ __global__ void __launch_bounds__(576, 1) bwd_value_kernel(const __grid_constant
     for (int tile = blockIdx.x; tile < a.g.ntiles; tile += step, ++it) {
       const RowTile t = row_tile<KEYS, 128>(a.g, tile, false);
       const int r = t.r0 + row;
-      const float* n2 = a.n2 + (int64_t)t.bh * a.Tp;
+      const float2* nd = a.nd + (int64_t)t.bh * a.Tp;
       for (int s = 0; s < t.n; ++s, ++g) {
         const int buf = g % 3;
         mbar_wait(bars + (exp_group ? C::S_FULL : C::P_FULL) + buf, (g / 3) & 1, a.status, exp_group ? 291 : 292);
@@ -1511,11 +1575,12 @@ __global__ void __launch_bounds__(576, 1) bwd_value_kernel(const __grid_constant
             tmem_ld_wait();
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-              const float4 n = __ldg(reinterpret_cast<const float4*>(n2 + c) + q);
-              x[4 * q] = __float_as_uint(ex2(fmaf(__uint_as_float(x[4 * q]), sc, -n.x)));
-              x[4 * q + 1] = __float_as_uint(ex2(fmaf(__uint_as_float(x[4 * q + 1]), sc, -n.y)));
-              x[4 * q + 2] = __float_as_uint(ex2(fmaf(__uint_as_float(x[4 * q + 2]), sc, -n.z)));
-              x[4 * q + 3] = __float_as_uint(ex2(fmaf(__uint_as_float(x[4 * q + 3]), sc, -n.w)));
+              const float4 n01 = __ldg(reinterpret_cast<const float4*>(nd + c) + 2 * q);
+              const float4 n23 = __ldg(reinterpret_cast<const float4*>(nd + c) + 2 * q + 1);
+              x[4 * q] = __float_as_uint(ex2(fmaf(__uint_as_float(x[4 * q]), sc, -n01.x)));
+              x[4 * q + 1] = __float_as_uint(ex2(fmaf(__uint_as_float(x[4 * q + 1]), sc, -n01.z)));
+              x[4 * q + 2] = __float_as_uint(ex2(fmaf(__uint_as_float(x[4 * q + 2]), sc, -n23.x)));
+              x[4 * q + 3] = __float_as_uint(ex2(fmaf(__uint_as_float(x[4 * q + 3]), sc, -n23.z)));
             }
             tmem_st32(tc, x);
           } else {
@@ -1642,8 +1707,7 @@ cudaError_t launch_feat(const Host& h) {
     return cudaErrorInvalidValue;
   a.lengths = h.p.key_lengths;
   a.beta = h.at<float>(h.ws.fwd.beta);
-  a.n2 = h.at<float>(h.ws.n2);
-  a.delta = h.at<float>(h.ws.delta);
+  a.nd = h.at<float2>(h.ws.nd);
   a.off = h.at<float>(h.ws.off[SIDE]);
   a.partial = h.at<float>(h.ws.partial);
   a.status = h.at<int>(h.ws.fwd.status);
@@ -1676,8 +1740,7 @@ cudaError_t launch_side(const Host& h, void* dx, int64_t ob, int64_t orow, int64
         !h.map_y(&a.tm_yo, OTHER, 64))
       return cudaErrorInvalidValue;
     a.g = h.geom(SIDE);
-    a.n2 = h.at<float>(h.ws.n2);
-    a.delta = h.at<float>(h.ws.delta);
+    a.nd = h.at<float2>(h.ws.nd);
     a.part = h.at<float>(h.ws.part);
     a.status = h.at<int>(h.ws.fwd.status);
     a.Tp = h.ws.Tp;
@@ -1696,7 +1759,7 @@ cudaError_t launch_side(const Host& h, void* dx, int64_t ob, int64_t orow, int64
       !map_bthe(&a.tm_dx, dx, h.p.B, h.side[SIDE].rows, h.p.H, D, ob, orow, oh, 128))
     return cudaErrorInvalidValue;
   a.g = h.geom(SIDE);
-  a.n2 = h.at<float>(h.ws.n2);
+  a.nd = h.at<float2>(h.ws.nd);
   a.delta = h.at<float>(h.ws.delta);
   a.off = h.at<float>(h.ws.off[SIDE]);
   a.sum1 = h.at<float>(h.ws.sum1[OTHER]);
@@ -1727,7 +1790,7 @@ cudaError_t backward(const Host& h) {
   bwd_rows_kernel<D><<<(unsigned)div_up(lanes, 1024), 256, 0, h.st>>>(
       static_cast<const __nv_bfloat16*>(p.out), p.o_stride_b, p.o_stride_t, p.o_stride_h,
       static_cast<const __nv_bfloat16*>(g.dout), g.do_stride_b, g.do_stride_t, g.do_stride_h, g.row_stats, p.B, p.H, p.T,
-      h.ws.Tp, h.at<float>(h.ws.n2), h.at<float>(h.ws.delta));
+      h.ws.Tp, h.at<float2>(h.ws.nd), h.at<float>(h.ws.delta));
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   if ((e = launch_feat<KEYS, D>(h)) != cudaSuccess) return e;
   if ((e = launch_feat<QUERIES, D>(h)) != cudaSuccess) return e;
@@ -1738,7 +1801,7 @@ cudaError_t backward(const Host& h) {
       !map_rows(&a.tm_sum, h.at<void>(h.ws.sum[QUERIES]), D, C::M, BH, 128))
     return cudaErrorInvalidValue;
   a.g = h.geom(KEYS);
-  a.n2 = h.at<float>(h.ws.n2);
+  a.nd = h.at<float2>(h.ws.nd);
   a.dv = static_cast<__nv_bfloat16*>(g.dv);
   a.vb = g.dv_stride_b; a.vs = g.dv_stride_s; a.vh = g.dv_stride_h;
   a.status = h.at<int>(h.ws.fwd.status);
@@ -1786,8 +1849,8 @@ void tc_plan_backward(const SblParams& p, TcBwdWorkspace* ws) {
   ws->wlo = take((size_t)p.r * p.E * 2);     // ... and its second
   f.beta = take(BH * 4);
   ws->Tp = (int)(div_up(p.T, TR) * TR);
-  ws->n2 = take(BH * ws->Tp * 4);
-  ws->delta = take(BH * ws->Tp * 4);
+  ws->nd = take(BH * ws->Tp * 8);
+  ws->delta = p.E == 128 ? take(BH * ws->Tp * 4) : off;
   ws->feat[QUERIES] = take(BH * T * m * 2);
   ws->feat[KEYS] = take(BH * S * m * 2);
   size_t partial = 0;
