@@ -53,8 +53,6 @@ cudaError_t f32_band(const SblParams& p, const Workspace& ws, char* base, const 
 // psi(q_t) = exp(+-u - tau|q|^2/2 - ln(m)/2 - row_scale[t]): query features over a scale per row
 cudaError_t f32_query_features_over(const SblParams& p, const Workspace& ws, char* base, const float* row_scale,
                                     float* psi, cudaStream_t st);
-cudaError_t f32_query_summary(const SblParams& p, const SblGrads& g, const float* psi, const float* delta,
-                              int split_rows, int nsplit, float* partial, float* qg, float* qd, cudaStream_t st);
 cudaError_t f32_attention_weights(const SblParams& p, const Workspace& ws, char* base, const float* beta,
                                   float* attn, float* attn_un, float* attn_lr, cudaStream_t st);
 
@@ -67,11 +65,11 @@ struct BwdWorkspace {
   size_t scale;     // (BH,T) the same minus beta: what psi is divided by
   size_t delta;     // (BH,T) dout . out
   size_t psi;       // (BH,T,m)
-  size_t qg, qd;    // (BH,m,D), (BH,m): query-side summary
+  size_t sum[2], sum1[2];   // summaries over the queries, over the keys: (BH,m,D), extra column (BH,m)
   size_t h;         // (BH,max(T,S),m): feature times its gradient
-  size_t partial;   // split partials of the query-side summary
+  size_t partial;   // split partials of one side's summary
   size_t total;
-  int nsplit, split_rows;
+  int nsplit[2], split_rows[2];
 };
 void f32_plan_backward(const SblParams& p, BwdWorkspace* ws);
 cudaError_t f32_backward(const SblParams& p, const SblGrads& g, const BwdWorkspace& ws, char* base, cudaStream_t st);

@@ -145,13 +145,11 @@ __global__ void __launch_bounds__(NTHR) feat_kernel(FeatArgs a) {
 
 // ---------------------------------------------------------------------------
 // Summary: partial[bh][split] (m x (D+1)) = phi(K)[rows]^T [V | 1]
-// (scatterbrain_utils.py:20,49).  The extra column carries sum_s phi(k_s), or,
-// with `last` (BH, S), sum_s last_s phi(k_s).
+// (scatterbrain_utils.py:20,49).  The extra column carries sum_s phi(k_s).
 template <typename T>
 __global__ void __launch_bounds__(NTHR)
 summary_partial_kernel(const float* phik, const void* vptr, int64_t sb, int64_t ss, int64_t sh, int S, int m,
-                       int D, int H, int row_lo, int row_hi, int split_rows, int dtiles, float* partial,
-                       const float* last) {
+                       int D, int H, int row_lo, int row_hi, int split_rows, int dtiles, float* partial) {
   __shared__ __align__(16) float sA[KS][LDT];
   __shared__ __align__(16) float sB[KS][LDT];
   const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
@@ -173,7 +171,7 @@ summary_partial_kernel(const float* phik, const void* vptr, int64_t sb, int64_t 
       const bool in = s < s_end;
       sA[kk][c] = (in && f0 + c < m) ? pk[(int64_t)s * m + f0 + c] : 0.f;
       const int d = d0 + c;
-      sB[kk][c] = !in ? 0.f : (d < D ? ldf(v + (int64_t)s * ss + d) : (d == D ? (last ? last[(int64_t)bh * S + s] : 1.f) : 0.f));
+      sB[kk][c] = !in ? 0.f : (d < D ? ldf(v + (int64_t)s * ss + d) : (d == D ? 1.f : 0.f));
     }
     __syncthreads();
     float part[4][4] = {};   // two-level sum over the keys
@@ -544,34 +542,14 @@ cudaError_t f32_key_summary(const SblParams& p, const Workspace& ws, char* base,
   if (p.dtype == SBL_DTYPE_F32)
     summary_partial_kernel<float><<<grid, NTHR, 0, st>>>(phik, p.v, p.v_stride_b, p.v_stride_s, p.v_stride_h, p.S,
                                                          m, p.D, p.H, p.sum_lo, p.sum_hi, ws.split_rows, dtiles,
-                                                         partial, nullptr);
+                                                         partial);
   else
     summary_partial_kernel<__nv_bfloat16><<<grid, NTHR, 0, st>>>(phik, p.v, p.v_stride_b, p.v_stride_s,
                                                                  p.v_stride_h, p.S, m, p.D, p.H, p.sum_lo, p.sum_hi,
-                                                                 ws.split_rows, dtiles, partial, nullptr);
+                                                                 ws.split_rows, dtiles, partial);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return f32_combine_partials(p, ws, base, kv, ksum, st);
-}
-
-// The summary of the gradients, over the query rows: qg (BH,m,D) = psi^T dout, qd (BH,m) = sum_t delta_t psi_t.
-cudaError_t f32_query_summary(const SblParams& p, const SblGrads& g, const float* psi, const float* delta,
-                              int split_rows, int nsplit, float* partial, float* qg, float* qd, cudaStream_t st) {
-  const int m = 2 * p.r, bh = p.B * p.H;
-  const int dtiles = (int)div_up(p.D + 1, TILE), mtiles = (int)div_up(m, TILE);
-  dim3 grid((unsigned)(mtiles * dtiles), (unsigned)nsplit, (unsigned)bh);
-  if (p.dtype == SBL_DTYPE_F32)
-    summary_partial_kernel<float><<<grid, NTHR, 0, st>>>(psi, g.dout, g.do_stride_b, g.do_stride_t, g.do_stride_h, p.T,
-                                                         m, p.D, p.H, 0, p.T, split_rows, dtiles, partial, delta);
-  else
-    summary_partial_kernel<__nv_bfloat16><<<grid, NTHR, 0, st>>>(psi, g.dout, g.do_stride_b, g.do_stride_t,
-                                                                 g.do_stride_h, p.T, m, p.D, p.H, 0, p.T, split_rows,
-                                                                 dtiles, partial, delta);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  const int64_t n = (int64_t)bh * m * (p.D + 1);
-  summary_combine_kernel<<<(unsigned)div_up(n, 256), 256, 0, st>>>(partial, nsplit, m, p.D, bh, qg, qd);
-  return cudaGetLastError();
 }
 
 cudaError_t f32_combine_partials(const SblParams& p, const Workspace& ws, char* base, float* kv, float* ksum,
