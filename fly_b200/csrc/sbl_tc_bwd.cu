@@ -717,14 +717,18 @@ struct GradArgs {
   float tau;
 };
 
-// A unit is a (tile, pass of 256 features); head dim 128 takes two passes.
+// A unit is a (tile, pass of 256 features); head dim 128 takes two passes.  The steps of all units form one stream,
+// gg = 0, 1, ..
 //
-// Tensor memory: df 256 | dx D | G of two steps 2 x 64 | (head dim 64) S 64.  A step's packed G lies over the first 16
-// of every 32 columns of its G buffer and p g over the next 16, so S is free for the next step as soon as it has been
-// read.  After the last step the G buffers take U of the own features.
+// Tensor memory: df 256 | dx D | G 64 | (head dim 64) S 64 | packed operands 64.  A step's G and S are read at once,
+// which frees both for the next step; what is made of them, g and p g, goes to the packed columns (head dim 64: 32 of
+// g and 32 of p g of one step; 128: g of two steps).  After the last step U of the own features takes 128 columns from
+// G on.  Every compute warp loads its U before it waits for df, so that the next tile's first G and S form meanwhile;
+// the group whose turn it is packs that step before it finishes the tile.
 //
-// Bound: the stream into shared memory.  A step's 64 columns are 32 KB of features and 16 KB of X' and Y'; with the
-// summary and the own rows 368 KB per tile and side, 8.8 k cycles at the 41.7 B/clk one SM's TMA loads sustain.
+// Bound: the chain of a tile (last step -> df -> du -> dx -> stored) beside the stream into shared memory.  A step's
+// 64 columns are 32 KB of features and 16 KB of X' and Y'; with the summary and the own rows 368 KB per tile and
+// side, 8.8 k cycles at the 41.7 B/clk one SM's TMA loads sustain.
 template <int D>
 struct GradCfg {
   static constexpr bool FUSE = D == 64;
@@ -742,10 +746,10 @@ struct GradCfg {
   static constexpr uint32_t OFF_ND = OFF_C + NC * CSLOT, OFF_S1 = OFF_ND + NND * NDB;   // then sum1 of the unit
   static constexpr uint32_t OFF_BAR = OFF_S1 + 1024, SMEM = OFF_BAR + 320;   // (the base is 1024-byte aligned)
   static constexpr int NCOMP = 512, NTHR = NCOMP + 128, W_LOAD = 16, W_STORE = 17, W_MMA_A = 18, W_MMA_B = 19;
-  static constexpr uint32_t T_DF = 0, T_DX = 256, T_G = FUSE ? 320 : 384, T_S = 448;
+  static constexpr uint32_t T_DF = 0, T_DX = 256, T_G = FUSE ? 320 : 384, T_S = T_G + 64, T_P = 448;
   enum { X_FULL = 0, X_FREE = 2, Y_FULL = 4, Y_FREE, SUM_FULL, SUM_FREE, W_FULL, W_FREE, F_FULL, F_FREE = F_FULL + NF,
-         C_FULL = F_FREE + NF, C_FREE = C_FULL + NC, T_FULL = C_FREE + NC, G_FREE = T_FULL + 2, S_READ = G_FREE + 2,
-         G_DONE = S_READ + 2, DF_FULL = G_DONE + 2, DU_DONE, DX_FULL, DX_FREE, STAGED, ND_FULL,
+         C_FULL = F_FREE + NF, C_FREE = C_FULL + NC, T_FULL = C_FREE + NC, P_FREE = T_FULL + 2, T_READ = P_FREE + 2,
+         G_DONE = T_READ + 2, U_FULL = G_DONE + 2, U_READ, DF_FULL, DU_DONE, DX_FULL, DX_FREE, STAGED, ND_FULL,
          COUNT = ND_FULL + (FUSE ? 0 : NND) };
   static_assert(SMEM <= 232448 && COUNT * 8 + 4 <= 320, "shared memory of one CTA");
 };
@@ -760,9 +764,9 @@ __global__ void __launch_bounds__(640, 1) bwd_grad_kernel(const __grid_constant_
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   if (tid == 0) {
     for (int i = 0; i < C::COUNT; ++i) {
-      const bool group = i >= C::S_READ && i < C::DF_FULL;
-      const bool all = i == C::DU_DONE || i == C::DX_FREE || i == C::STAGED;
-      const bool both = i == C::DF_FULL || i == C::Y_FREE;   // one commit of either issuing warp
+      const bool group = i >= C::T_READ && i < C::U_FULL;
+      const bool all = i == C::U_READ || i == C::DU_DONE || i == C::DX_FREE || i == C::STAGED;
+      const bool both = i == C::Y_FREE;                      // one commit of either issuing warp
       mbar_init(bars + i, group ? 8 : all ? 16 : both ? 2 : 1);
     }
     fence_mbar_init();
@@ -894,78 +898,64 @@ __global__ void __launch_bounds__(640, 1) bwd_grad_kernel(const __grid_constant_
     const uint64_t dY = smem_desc_sw128(smem_u32(smem + C::OFF_Y), 16, 1024);
     const uint64_t dC = smem_desc_sw128(smem_u32(smem + C::OFF_C), 16, 1024);
     const uint64_t dW = smem_desc_sw128(smem_u32(smem + C::OFF_W), 16, 1024);
-    int g0 = 0;                     // number of the unit's first step in the CTA's stream of steps
+    int gg = 0;                     // number of the step in the CTA's stream
     for (int u = 0; u < n_u; ++u) {
       const int it = u / C::PASS, pass = u % C::PASS, xb = it % C::XBUF;
       const int n = row_tile<SIDE, 64>(a.g, blockIdx.x + it * step, whole).n;
       const uint64_t x = dX + (uint64_t)(xb * (C::TB >> 4));
-      // G = Y Y'^T of step gg, into the buffer that the products of step gg - 2 have left
-      auto issue_g = [&](int gg) {
+      if (pass == 0) wait_inline(bars + C::Y_FULL, it & 1, a.status, 274);
+      if (C::FUSE) wait_inline(bars + C::X_FULL + xb, (it / C::XBUF) & 1, a.status, 275);
+      for (int s = 0; s < n; ++s, ++gg) {
         const int slot = gg % C::NC;
         wait_inline(bars + C::C_FULL + slot, (gg / C::NC) & 1, a.status, 271);
-        if (gg >= 2) wait_inline(bars + C::G_FREE + (gg & 1), ((gg >> 1) - 1) & 1, a.status, 272);
+        // the step before has been read, or U of the unit before
+        if (s > 0) wait_inline(bars + C::T_READ + ((gg - 1) & 1), ((gg - 1) >> 1) & 1, a.status, 276);
+        else if (u > 0) wait_inline(bars + C::U_READ, (u - 1) & 1, a.status, 273);
+        // (head dim 128: seen for every step, because U waits for the last two and phases are told apart by parity)
+        if (!C::FUSE && gg >= 2) wait_inline(bars + C::P_FREE + (gg & 1), ((gg >> 1) - 1) & 1, a.status, 275);
         tc_fence_after_sync();
         if (leader) {
           const uint64_t o = dC + (uint64_t)(slot * (C::CSLOT >> 4));
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            mma_ss(tb + C::T_G + 64 * (gg & 1), dY + kmajor(k, 16384), o + kmajor(k, 8192), id_t, k > 0);
-          if (!C::FUSE) {
-            mma_commit(bars + C::T_FULL + (gg & 1));
-            mma_commit(bars + C::C_FREE + slot);
-          }
-        }
-        __syncwarp();
-      };
-      // S = X X'^T; its column tile is that of a G product issued before
-      auto issue_s = [&](int gg) {
-        if (leader) {
-          const uint64_t o = dC + (uint64_t)((gg % C::NC) * (C::CSLOT >> 4) + 512);
+          for (int k = 0; k < D / 16; ++k) mma_ss(tb + C::T_G, dY + kmajor(k, 16384), o + kmajor(k, 8192), id_t, k > 0);
+          if (C::FUSE) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) mma_ss(tb + C::T_S, x + kmajor(k, 16384), o + kmajor(k, 8192), id_t, k > 0);
+            for (int k = 0; k < D / 16; ++k)
+              mma_ss(tb + C::T_S, x + kmajor(k, 16384), o + 512 + kmajor(k, 8192), id_t, k > 0);
+          }
           mma_commit(bars + C::T_FULL + (gg & 1));
+          if (!C::FUSE) mma_commit(bars + C::C_FREE + slot);
         }
         __syncwarp();
-      };
-      // U of the unit before has been read
-      if (u >= 1) wait_inline(bars + C::DU_DONE, (u - 1) & 1, a.status, 273);
-      if (pass == 0) wait_inline(bars + C::Y_FULL, it & 1, a.status, 274);
-      if (C::FUSE) wait_inline(bars + C::X_FULL + xb, (it / C::XBUF) & 1, a.status, 275);
-      if (n > 0) issue_g(g0);
-      if (C::FUSE && n > 0) issue_s(g0);
-      if (n > 1) issue_g(g0 + 1);
-      for (int s = 0; s < n; ++s) {
-        const int gg = g0 + s;
-        if (C::FUSE && s + 1 < n) {
-          wait_inline(bars + C::S_READ + (gg & 1), (gg >> 1) & 1, a.status, 276);
-          tc_fence_after_sync();
-          issue_s(gg + 1);
-        }
-        if (s + 2 < n) issue_g(gg + 2);
       }
-      g0 += n;
-      // U of the own features over the G buffers, for du: the products of the last two steps have to be done
-      for (int gg = g0 - 2 > 0 ? g0 - 2 : 0; gg < g0; ++gg)
-        wait_inline(bars + C::G_FREE + (gg & 1), (gg >> 1) & 1, a.status, 277);
+      // U of the own features, from the columns of G on: the last step has been read (without steps: U of the unit
+      // before); head dim 128: and the products that read the packed columns are done
+      if (n > 0) wait_inline(bars + C::T_READ + ((gg - 1) & 1), ((gg - 1) >> 1) & 1, a.status, 277);
+      else if (u > 0) wait_inline(bars + C::U_READ, (u - 1) & 1, a.status, 278);
+      if (!C::FUSE)
+        for (int g = gg - 2 > 0 ? gg - 2 : 0; g < gg; ++g)
+          wait_inline(bars + C::P_FREE + (g & 1), (g >> 1) & 1, a.status, 272);
       wait_inline(bars + C::W_FULL, C::FUSE ? 0 : u & 1, a.status, 279);
       if (!C::FUSE && pass == 0) wait_inline(bars + C::X_FULL + xb, (it / C::XBUF) & 1, a.status, 280);
       tc_fence_after_sync();
       if (leader) {
+        if (pass == C::PASS - 1) mma_commit(bars + C::Y_FREE);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
             mma_ss(tb + C::T_G, x + kmajor(k, 16384), dW + (uint64_t)(t * (C::AUX >> 5)) + kmajor(k, 16384), id_u,
                    t > 0 || k > 0);
-        if (pass == C::PASS - 1) mma_commit(bars + C::Y_FREE);
-        mma_commit(bars + C::DF_FULL);
+        mma_commit(bars + C::U_FULL);
       }
       __syncwarp();
     }
   } else if (warp == C::W_MMA_B) {
     // ---- issuer B: df, dx
     const bool leader = elect_one();
-    constexpr uint32_t id_df = idesc_bf16(128, 256, false, true);
+    // The packed operands hold delta - y.y' and p times that.  Bit 13 negates A: df takes -g inside the window, g
+    // outside it (`whole`), dx takes p g.
+    const uint32_t id_df = idesc_bf16(128, 256, false, true) | (whole ? 1u << 13 : 0u);
     constexpr uint32_t id_sum = idesc_bf16(128, 256, false, false);
     constexpr uint32_t id_dx = idesc_bf16(128, D, false, true);
     const uint64_t dY = smem_desc_sw128(smem_u32(smem + C::OFF_Y), 16, 1024);
@@ -1004,17 +994,17 @@ __global__ void __launch_bounds__(640, 1) bwd_grad_kernel(const __grid_constant_
         if (leader) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mma_ts(tb + C::T_DF, tb + C::T_G + 64 * (gg & 1) + packed(k), dF + (uint64_t)(slot * 2048 + k * 128), id_df,
-                   !fresh || k > 0);
+            mma_ts(tb + C::T_DF, tb + C::T_P + (C::FUSE ? 0 : 32 * (gg & 1)) + 8 * k, dF + (uint64_t)(slot * 2048 + k * 128),
+                   id_df, !fresh || k > 0);
           mma_commit(bars + C::F_FREE + slot);
           if (C::FUSE) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              mma_ts(tb + C::T_DX, tb + C::T_G + 64 * (gg & 1) + 16 + packed(k),
-                     dCt + (uint64_t)((gg % C::NC) * (C::CSLOT >> 4) + k * 128), id_dx, s > 0 || k > 0);
+              mma_ts(tb + C::T_DX, tb + C::T_P + 32 + 8 * k, dCt + (uint64_t)((gg % C::NC) * (C::CSLOT >> 4) + k * 128),
+                     id_dx | (1u << 13), s > 0 || k > 0);
             mma_commit(bars + C::C_FREE + gg % C::NC);
           }
-          mma_commit(bars + C::G_FREE + (gg & 1));
+          mma_commit(bars + C::P_FREE + (gg & 1));
         }
         __syncwarp();
         fresh = false;
@@ -1071,9 +1061,7 @@ __global__ void __launch_bounds__(640, 1) bwd_grad_kernel(const __grid_constant_
     float* s_s1 = reinterpret_cast<float*>(smem + C::OFF_S1);
     const float sc = a.tau * kLog2e;
     const float lt = log2f(a.tau);
-    int gg = 0;
-    float hs = 0.f;
-    // What a thread needs of a tile's row, fetched while the tile before is still being finished
+    // a tile, and what a thread needs of its row
     RowTile t = row_tile<SIDE, 64>(a.g, blockIdx.x, whole);
     float off, rn = 0.f, rd = 0.f;
     auto fetch_row = [&]() {
@@ -1081,166 +1069,209 @@ __global__ void __launch_bounds__(640, 1) bwd_grad_kernel(const __grid_constant_
       off = __ldg(a.off + (int64_t)t.bh * a.g.ntr * TR + r);
       if (SIDE == QUERIES) {
         const float2 v = __ldg(a.nd + (int64_t)t.bh * a.Tp + r);   // (r < Tp)
-        rn = v.x - lt;              // tau p = 2^(S sc - (n2 - log2 tau))
+        rn = lt - v.x;              // tau p = 2^(S sc + (log2 tau - n2))
         rd = v.y;
       }
     };
+    // Step s of tile t, number gg of the stream: G, S -> delta - y.y' and p times that, packed.
+    auto pack_step = [&](int s, int gg) {
+      const int c = t.c0 + 64 * s + 32 * cq, r = t.r0 + row;
+      const uint32_t in = seen<SIDE>(a.g, t, r, c, false);
+      const uint32_t out = whole ? seen<SIDE>(a.g, t, r, c, true) : 0u;
+      mbar_wait(bars + C::T_FULL + grp, (gg >> 1) & 1, a.status, 286);
+      tc_fence_after_sync();
+      uint32_t x[32], y[32];
+      tmem_ld32(lane_base + C::T_G + 32 * cq, y);
+      if (C::FUSE) tmem_ld32(lane_base + C::T_S + 32 * cq, x);
+      const float4* nd = reinterpret_cast<const float4*>(smem + C::OFF_ND + (gg % C::NND) * C::NDB + cq * (C::NDB / 2));
+      // head dim 64: landed with the step's tile, which is held until its products are done
+      if (SIDE == KEYS && C::FUSE) mbar_wait(bars + C::C_FULL + gg % C::NC, (gg / C::NC) & 1, a.status, 285);
+      if (SIDE == KEYS && !C::FUSE) mbar_wait(bars + C::ND_FULL + (gg & 3), (gg >> 2) & 1, a.status, 283);
+      tmem_ld_wait();
+      tc_fence_before_sync();
+      warp_arrive(bars + C::T_READ + grp, lane);
+      uint32_t o[16], e[16];
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        float2 dd = make_float2(rd, rd), nn = make_float2(rn, rn);
+        if (SIDE == KEYS && C::FUSE) {
+          const float4 v = nd[q];
+          dd = make_float2(v.y, v.w);
+          nn = make_float2(lt - v.x, lt - v.z);
+        } else if (SIDE == KEYS) {
+          dd = reinterpret_cast<const float2*>(nd)[q];
+        }
+        const float2 d = fma2(make_float2(__uint_as_float(y[2 * q]), __uint_as_float(y[2 * q + 1])), make_float2(-1.f, -1.f), dd);
+        float2 g = make_float2(keep_if_bit(d.x, in, 2 * q), keep_if_bit(d.y, in, 2 * q + 1));
+        if (C::FUSE) {
+          // (hidden columns: a weight that is finite, times zero)
+          const float2 arg = fma2(make_float2(__uint_as_float(x[2 * q]), __uint_as_float(x[2 * q + 1])), make_float2(sc, sc), nn);
+          const float2 w = mul2(make_float2(ex2(fminf(arg.x, 126.f)), ex2(fminf(arg.y, 126.f))), g);
+          e[q] = pack_bf16(w.x, w.y);
+        }
+        if (whole) g = make_float2(keep_if_bit(d.x, out, 2 * q), keep_if_bit(d.y, out, 2 * q + 1));
+        o[q] = pack_bf16(g.x, g.y);
+      }
+      // the products that read the packed columns before
+      if (C::FUSE) {
+        if (gg >= 1) mbar_wait(bars + C::P_FREE + (grp ^ 1), ((gg - 1) >> 1) & 1, a.status, 284);
+        tmem_st16(lane_base + C::T_P + 16 * cq, o);
+        tmem_st16(lane_base + C::T_P + 32 + 16 * cq, e);
+      } else {
+        if (gg >= 2) mbar_wait(bars + C::P_FREE + grp, ((gg >> 1) - 1) & 1, a.status, 284);
+        tmem_st16(lane_base + C::T_P + 32 * grp + 16 * cq, o);
+      }
+      tmem_st_wait();
+      tc_fence_before_sync();
+      warp_arrive(bars + C::G_DONE + grp, lane);
+    };
     fetch_row();
+    int gg = 0;                     // number of the unit's first step
+    float hs = 0.f;
+    bool early = false;             // the unit's first step has been packed already
     for (int u = 0; u < n_u; ++u) {
       const int it = u / C::PASS, pass = u % C::PASS;
       const int tile = blockIdx.x + it * step;
-      const int r = t.r0 + row;
       float sum1 = 0.f;
       if (tid < 256) sum1 = __ldg(a.sum1 + (int64_t)t.bh * C::M + 256 * pass + tid);
-      for (int s = 0; s < t.n; ++s, ++gg) {
-        if ((gg & 1) != grp) continue;
-        const int c = t.c0 + 64 * s + 32 * cq;
-        const uint32_t in = seen<SIDE>(a.g, t, r, c, false);
-        const uint32_t vis = whole ? seen<SIDE>(a.g, t, r, c, true) : in;
-        const uint32_t tg = lane_base + C::T_G + 64 * grp + 32 * cq;
-        mbar_wait(bars + C::T_FULL + grp, (gg >> 1) & 1, a.status, 286);
-        tc_fence_after_sync();
-        uint32_t x[32], y[32];
-        if (C::FUSE) tmem_ld32(lane_base + C::T_S + 32 * cq, x);
-        tmem_ld32(tg, y);
-        const float4* nd = reinterpret_cast<const float4*>(smem + C::OFF_ND + (gg % C::NND) * C::NDB + cq * (C::NDB / 2));
-        // head dim 64: landed with the step's tile, which is held until its products are done
-        if (SIDE == KEYS && C::FUSE) mbar_wait(bars + C::C_FULL + gg % C::NC, (gg / C::NC) & 1, a.status, 285);
-        if (SIDE == KEYS && !C::FUSE) mbar_wait(bars + C::ND_FULL + (gg & 3), (gg >> 2) & 1, a.status, 283);
-        tmem_ld_wait();
-        if (C::FUSE) {
-          tc_fence_before_sync();
-          warp_arrive(bars + C::S_READ + grp, lane);
-        }
-        uint32_t o[16], e[16];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          float4 n01 = make_float4(rn, rd, rn, rd), n23 = n01;
-          if (SIDE == KEYS && C::FUSE) {
-            n01 = nd[2 * q];
-            n23 = nd[2 * q + 1];
-          } else if (SIDE == KEYS) {
-            const float4 v = nd[q];
-            n01 = make_float4(0.f, v.x, 0.f, v.y);
-            n23 = make_float4(0.f, v.z, 0.f, v.w);
-          }
-          const float nn[4] = {n01.x, n01.z, n23.x, n23.z}, dd[4] = {n01.y, n01.w, n23.y, n23.w};
-          float v[4], w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float d = __uint_as_float(y[4 * q + j]) - dd[j];
-            v[j] = keep_if_bit(whole ? d : -d, vis, 4 * q + j);   // the window's G enters df with a minus
-            if (C::FUSE) {
-              const float p = ex2(fmaf(__uint_as_float(x[4 * q + j]), sc, SIDE == KEYS ? lt - nn[j] : -nn[j]));
-              w[j] = keep_if_bit(p * d, in, 4 * q + j);
-            }
-          }
-          o[2 * q] = pack_bf16(v[0], v[1]);
-          o[2 * q + 1] = pack_bf16(v[2], v[3]);
-          if (C::FUSE) {
-            e[2 * q] = pack_bf16(w[0], w[1]);
-            e[2 * q + 1] = pack_bf16(w[2], w[3]);
-          }
-        }
-        tmem_st16(tg, o);
-        if (C::FUSE) tmem_st16(tg + 16, e);
-        tmem_st_wait();
-        tc_fence_before_sync();
-        warp_arrive(bars + C::G_DONE + grp, lane);
-      }
-      // df -> du of this thread's 32 projections: du = f+ df+ - f- df-, in two bf16 terms
       const bool none = whole && t.n == 0;
-      const float d1 = whole ? 0.f : (SIDE == QUERIES ? rd : 1.f);
-      if (pass == 0) hs = 0.f;
+      const bool last = pass == C::PASS - 1;
+#pragma unroll 1
+      for (int s = early ? 1 : 0; s < t.n; ++s)
+        if (((gg + s) & 1) == grp) pack_step(s, gg + s);
+      early = false;
+      gg += t.n;
       if (tid < 256) {
         // (every reader of the unit before is through; head dim 64: a tile has one unit, and its dx was waited for)
-        if (!C::FUSE && u >= 1) mbar_wait(bars + C::DU_DONE, (u - 1) & 1, a.status, 284);
+        if (!C::FUSE && u >= 1) mbar_wait(bars + C::DU_DONE, (u - 1) & 1, a.status, 283);
         s_s1[tid] = sum1;
       }
+      if (pass == 0) hs = 0.f;
       asm volatile("bar.sync 1, 512;" ::: "memory");
+      // df -> du of this thread's 32 projections: du = f+ df+ - f- df-, in two bf16 terms
+      const float nd1 = whole ? 0.f : (SIDE == QUERIES ? -rd : -1.f);
+      const float o1 = off;
       const float* s1 = s_s1 + 128 * grp + 32 * cq;
       const uint32_t td = lane_base + C::T_DF + 128 * grp + 32 * cq;
+      mbar_wait(bars + C::U_FULL, u & 1, a.status, 290);
+      tc_fence_after_sync();
+      uint32_t uu[32];
+      tmem_ld32(lane_base + C::T_G + 64 * grp + 32 * cq, uu);
+      tmem_ld_wait();
+      tc_fence_before_sync();
+      warp_arrive(bars + C::U_READ, lane);
+      // the next tile's row, on its way while df is waited for
+      if (last && it + 1 < n_it) {
+        t = row_tile<SIDE, 64>(a.g, tile + step, whole);
+        fetch_row();
+      }
       mbar_wait(bars + C::DF_FULL, u & 1, a.status, 287);
       tc_fence_after_sync();
-      uint32_t hi[16], lo[16];
+      float2 hs2 = make_float2(0.f, 0.f);
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        uint32_t p[16], m[16], uu[16];
+        uint32_t p[16], m[16], hi[8], lo[8];
         tmem_ld16(td + 16 * hf, p);
         tmem_ld16(td + 64 + 16 * hf, m);
-        tmem_ld16(lane_base + C::T_G + 64 * grp + 32 * cq + 16 * hf, uu);
         tmem_ld_wait();
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           const float2 sp = *reinterpret_cast<const float2*>(s1 + 16 * hf + 2 * q);
           const float2 sm = *reinterpret_cast<const float2*>(s1 + 64 + 16 * hf + 2 * q);
-          const float u0 = __uint_as_float(uu[2 * q]), u1 = __uint_as_float(uu[2 * q + 1]);
-          const float hp0 = ex2(fmaf(u0, kLog2e, off)) * fmaf(-d1, sp.x, none ? 0.f : __uint_as_float(p[2 * q]));
-          const float hp1 = ex2(fmaf(u1, kLog2e, off)) * fmaf(-d1, sp.y, none ? 0.f : __uint_as_float(p[2 * q + 1]));
-          const float hm0 = ex2(fmaf(u0, -kLog2e, off)) * fmaf(-d1, sm.x, none ? 0.f : __uint_as_float(m[2 * q]));
-          const float hm1 = ex2(fmaf(u1, -kLog2e, off)) * fmaf(-d1, sm.y, none ? 0.f : __uint_as_float(m[2 * q + 1]));
-          hs += (hp0 + hm0) + (hp1 + hm1);
-          const float d0 = hp0 - hm0, d2 = hp1 - hm1;
-          const uint32_t h2 = pack_bf16(d0, d2);
-          hi[8 * hf + q] = h2;
-          lo[8 * hf + q] = pack_bf16(d0 - bf16_lo(h2), d2 - bf16_hi(h2));
+          const float2 uv = make_float2(__uint_as_float(uu[16 * hf + 2 * q]), __uint_as_float(uu[16 * hf + 2 * q + 1]));
+          float2 dp = make_float2(__uint_as_float(p[2 * q]), __uint_as_float(p[2 * q + 1]));
+          float2 dm = make_float2(__uint_as_float(m[2 * q]), __uint_as_float(m[2 * q + 1]));
+          if (none) dp = dm = make_float2(0.f, 0.f);
+          dp = fma2(make_float2(nd1, nd1), sp, dp);
+          dm = fma2(make_float2(nd1, nd1), sm, dm);
+          const float2 ap = fma2(uv, make_float2(kLog2e, kLog2e), make_float2(o1, o1));
+          const float2 am = fma2(uv, make_float2(-kLog2e, -kLog2e), make_float2(o1, o1));
+          const float2 hp = mul2(make_float2(ex2(ap.x), ex2(ap.y)), dp);
+          const float2 hm = mul2(make_float2(ex2(am.x), ex2(am.y)), dm);
+          hs2 = add2(hs2, add2(hp, hm));
+          const float2 d = fma2(hm, make_float2(-1.f, -1.f), hp);
+          const uint32_t h2 = pack_bf16(d.x, d.y);
+          const float2 l = fma2(make_float2(bf16_lo(h2), bf16_hi(h2)), make_float2(-1.f, -1.f), d);
+          hi[q] = h2;
+          lo[q] = pack_bf16(l.x, l.y);
+        }
+        // high terms over the thread's first 16 "+" columns, low ones over the next 16: of the second half these are
+        // read before the first half's are written
+        if (hf == 0) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            uu[q] = hi[q];
+            uu[8 + q] = lo[q];
+          }
+        } else {
+          uint32_t h0[8], l0[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            h0[q] = uu[q];
+            l0[q] = uu[8 + q];
+          }
+          tmem_st8(td, h0);
+          tmem_st8(td + 8, hi);
+          tmem_st8(td + 16, l0);
+          tmem_st8(td + 24, lo);
         }
       }
-      tmem_st16(td, hi);            // over the thread's own "+" columns
-      tmem_st16(td + 16, lo);
-      if (pass == C::PASS - 1) tmem_st1(td + 64, __float_as_uint(hs));   // ... and the first of its "-" columns
+      hs += hs2.x + hs2.y;
+      if (last) tmem_st1(td + 64, __float_as_uint(hs));   // ... and the sum over the first of its "-" columns
       tmem_st_wait();
       tc_fence_before_sync();
       warp_arrive(bars + C::DU_DONE, lane);
-      if (pass == C::PASS - 1) {
-        constexpr int NQ = D / 4;
-        const int c = NQ * (2 * grp + cq), buf = it % C::XBUF;
-        uint8_t* xs = smem + C::OFF_X + buf * C::TB + (c >> 6) * 16384 + row * 128;
-        float4 e[C::FUSE ? 1 : NQ / 4];
-        if (!C::FUSE) {
-          const float4* part = reinterpret_cast<const float4*>(a.part) + ((int64_t)tile * (D / 4) + c / 4) * TR + row;
-#pragma unroll
-          for (int j = 0; j < NQ / 4; ++j) e[j] = __ldg(part + j * TR);
-        }
-        if (it + 1 < n_it) {
-          t = row_tile<SIDE, 64>(a.g, tile + step, whole);
-          fetch_row();
-        }
-        mbar_wait(bars + C::X_FULL + buf, (it / C::XBUF) & 1, a.status, 288);
-        mbar_wait(bars + C::DX_FULL, it & 1, a.status, 289);
-        tc_fence_after_sync();
-        uint32_t v[NQ / 16][16];
-        const uint32_t h0 = tmem_ld1(lane_base + C::T_DF + 64), h1 = tmem_ld1(lane_base + C::T_DF + 96);
-        const uint32_t h2 = tmem_ld1(lane_base + C::T_DF + 192), h3 = tmem_ld1(lane_base + C::T_DF + 224);
-#pragma unroll
-        for (int q = 0; q < NQ / 16; ++q) tmem_ld16(lane_base + C::T_DX + c + 16 * q, v[q]);
-        tmem_ld_wait();
-        tc_fence_before_sync();
-        warp_arrive(bars + C::DX_FREE, lane);
-        const float hsum = a.tau * ((__uint_as_float(h0) + __uint_as_float(h1)) + (__uint_as_float(h2) + __uint_as_float(h3)));
-#pragma unroll
-        for (int j = 0; j < NQ / 8; ++j) {
-          // eight entries: 16 bytes of the row's swizzled line, dx over x
-          uint4* at = reinterpret_cast<uint4*>(xs + ((((c & 63) >> 3) + j) ^ (row & 7)) * 16);
-          const uint4 xv = *at;
-          const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
-          float z[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) z[k] = __uint_as_float(v[j >> 1][8 * (j & 1) + k]);
-          if (!C::FUSE) {
-            const float4 e0 = e[2 * j], e1 = e[2 * j + 1];
-            z[0] += e0.x; z[1] += e0.y; z[2] += e0.z; z[3] += e0.w;
-            z[4] += e1.x; z[5] += e1.y; z[6] += e1.z; z[7] += e1.w;
-          }
-          uint32_t w[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            w[k] = pack_bf16(fmaf(-hsum, bf16_lo(xw[k]), z[2 * k]), fmaf(-hsum, bf16_hi(xw[k]), z[2 * k + 1]));
-          *at = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        fence_async_smem();
-        warp_arrive(bars + C::STAGED, lane);
+      if (!last) continue;
+      // the next tile's first step, before this tile's dx: G and S are there as soon as U has been read
+      if (it + 1 < n_it && t.n > 0 && (gg & 1) == grp) {
+        pack_step(0, gg);
+        early = true;
+      } else if (it + 1 < n_it && t.n > 0) {
+        early = true;               // (the other group's)
       }
+      constexpr int NQ = D / 4;
+      const int c = NQ * (2 * grp + cq), buf = it % C::XBUF;
+      uint8_t* xs = smem + C::OFF_X + buf * C::TB + (c >> 6) * 16384 + row * 128;
+      float4 e[C::FUSE ? 1 : NQ / 4];
+      if (!C::FUSE) {
+        const float4* part = reinterpret_cast<const float4*>(a.part) + ((int64_t)tile * (D / 4) + c / 4) * TR + row;
+#pragma unroll
+        for (int j = 0; j < NQ / 4; ++j) e[j] = __ldg(part + j * TR);
+      }
+      mbar_wait(bars + C::X_FULL + buf, (it / C::XBUF) & 1, a.status, 288);
+      mbar_wait(bars + C::DX_FULL, it & 1, a.status, 289);
+      tc_fence_after_sync();
+      uint32_t v[NQ / 16][16];
+      const uint32_t h0 = tmem_ld1(lane_base + C::T_DF + 64), h1 = tmem_ld1(lane_base + C::T_DF + 96);
+      const uint32_t h2 = tmem_ld1(lane_base + C::T_DF + 192), h3 = tmem_ld1(lane_base + C::T_DF + 224);
+#pragma unroll
+      for (int q = 0; q < NQ / 16; ++q) tmem_ld16(lane_base + C::T_DX + c + 16 * q, v[q]);
+      tmem_ld_wait();
+      tc_fence_before_sync();
+      warp_arrive(bars + C::DX_FREE, lane);
+      const float hsum = a.tau * ((__uint_as_float(h0) + __uint_as_float(h1)) + (__uint_as_float(h2) + __uint_as_float(h3)));
+#pragma unroll
+      for (int j = 0; j < NQ / 8; ++j) {
+        // eight entries: 16 bytes of the row's swizzled line, dx over x
+        uint4* at = reinterpret_cast<uint4*>(xs + ((((c & 63) >> 3) + j) ^ (row & 7)) * 16);
+        const uint4 xv = *at;
+        const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+        float z[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) z[k] = __uint_as_float(v[j >> 1][8 * (j & 1) + k]);
+        if (!C::FUSE) {
+          const float4 e0 = e[2 * j], e1 = e[2 * j + 1];
+          z[0] += e0.x; z[1] += e0.y; z[2] += e0.z; z[3] += e0.w;
+          z[4] += e1.x; z[5] += e1.y; z[6] += e1.z; z[7] += e1.w;
+        }
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          w[k] = pack_bf16(fmaf(-hsum, bf16_lo(xw[k]), z[2 * k]), fmaf(-hsum, bf16_hi(xw[k]), z[2 * k + 1]));
+        *at = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      fence_async_smem();
+      warp_arrive(bars + C::STAGED, lane);
     }
   }
   tc_fence_before_sync();
