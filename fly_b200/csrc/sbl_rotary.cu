@@ -26,6 +26,7 @@ namespace sbl {
 namespace {
 
 constexpr int kWarps = 4;                               // warps per block
+constexpr int kStages = 4;                              // row steps in the ring of a warp
 constexpr int kMaxPairs = SBL_NORM_ROTARY_MAX_E / 2;
 
 struct RotaryArgs {
@@ -54,6 +55,19 @@ __device__ __forceinline__ double position_of(const SblNormRotarySide& s, int b,
   return (double)(s.positions ? s.positions[b * s.pos_stride_b + t * s.pos_stride_t] : s.pos0 + t);
 }
 
+// 8 consecutive entries of a row into shared memory, asynchronously
+template <typename T>
+__device__ __forceinline__ void copy_row8(T* dst, const T* src) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + 16 * i), "l"(reinterpret_cast<const char*>(src) + 16 * i)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // 8 consecutive entries as raw words
 template <typename T>
 struct Raw8;
@@ -61,7 +75,7 @@ template <>
 struct Raw8<__nv_bfloat16> {
   uint32_t w[4];
   __device__ void load(const __nv_bfloat16* p) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
     w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   }
   __device__ void zero() { w[0] = w[1] = w[2] = w[3] = 0u; }
@@ -84,7 +98,7 @@ template <>
 struct Raw8<float> {
   float w[8];
   __device__ void load(const float* p) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
     w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
   }
   __device__ void zero() {
@@ -136,43 +150,83 @@ __global__ void __launch_bounds__(32 * kWarps) vec_kernel(const __grid_constant_
   }
   const int H = s.H, per = (H + gridDim.y - 1) / gridDim.y;
   const int h_lo = blockIdx.y * per, h_hi = min(H, h_lo + per);
-  const int64_t tokens = (int64_t)a.B * s.T;
   const float inv_e = 1.f / (float)E;
-  for (int64_t tok = (int64_t)blockIdx.x * kWarps + warp; tok < tokens; tok += (int64_t)gridDim.x * kWarps) {
-    const int b = (int)(tok / s.T), t = (int)(tok - (int64_t)b * s.T);
-    if (half > 0) {
-      const double pos = position_of(s, b, t);
-      __syncwarp();
-      for (int i = lane; i < half; i += 32) s_turn[warp][i] = turn(pos, s_rate[i]);
-      __syncwarp();
-    }
-    float cs[8], sn[8];                                 // y = z * cs + z_partner * sn
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      cs[i] = 1.f;
-      sn[i] = 0.f;
-      if (INTER) {
-        if (e0 + i < a.rotary) {
-          const float2 c = s_turn[warp][(e0 + i) / 2];
-          cs[i] = c.x;
-          sn[i] = (i & 1) ? c.y : -c.y;
-        }
-      } else if (turned) {
-        const float2 c = s_turn[warp][low ? e0 + i : e0 + i - half];
-        cs[i] = c.x;
-        sn[i] = low ? -c.y : c.y;
+  // The warp's steps, RPW rows of a token each, form one stream.  Rows travel kStages - 1 steps ahead through a ring in
+  // shared memory; a lane reads back what it copied itself, so that nothing but its own copies is waited for.
+  __shared__ __align__(16) T s_ring[kWarps][kStages][BWD ? 2 : 1][32 * 8];
+  const uint32_t T_ = (uint32_t)s.T, hop = gridDim.x * kWarps, first = blockIdx.x * kWarps + warp;
+  const uint32_t hop_b = T_ ? hop / T_ : 0, hop_t = T_ ? hop % T_ : 0;
+  struct Cursor { uint32_t b, t; int h; };
+  Cursor at = {T_ ? first / T_ : 0, T_ ? first % T_ : 0, h_lo};
+  const uint32_t none = (uint32_t)a.B;
+  if (T_ == 0 || h_lo >= h_hi) at.b = none;
+  auto advance = [&](Cursor& c) {
+    c.h += RPW;
+    if (c.h >= h_hi) {
+      c.h = h_lo;
+      c.b += hop_b;
+      c.t += hop_t;                                     // (both below 2^31)
+      if (c.t >= T_) {
+        c.t -= T_;
+        ++c.b;
       }
     }
-    const T* x = static_cast<const T*>(s.x) + b * s.x_stride_b + t * s.x_stride_t + e0;
-    const T* dy = BWD ? static_cast<const T*>(s.dy) + b * s.dy_stride_b + t * s.dy_stride_t + e0 : nullptr;
-    T* y = static_cast<T*>(s.y) + b * s.y_stride_b + t * s.y_stride_t + e0;
-#pragma unroll 2
-    for (int hb = h_lo; hb < h_hi; hb += RPW) {
-      const int h = hb + grp;
+  };
+  Cursor ahead = at;
+  auto fetch = [&](int slot) {
+    if (ahead.b < none) {
+      if (held && ahead.h + grp < h_hi) {
+        const int64_t h = ahead.h + grp;
+        copy_row8(&s_ring[warp][slot][0][8 * lane],
+                  static_cast<const T*>(s.x) + ahead.b * s.x_stride_b + ahead.t * s.x_stride_t + h * s.x_stride_h + e0);
+        if (BWD)
+          copy_row8(&s_ring[warp][slot][BWD ? 1 : 0][8 * lane],
+                    static_cast<const T*>(s.dy) + ahead.b * s.dy_stride_b + ahead.t * s.dy_stride_t + h * s.dy_stride_h + e0);
+      }
+      advance(ahead);
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(i);
+  float cs[8], sn[8];                                   // y = z * cs + z_partner * sn
+  T* y = nullptr;
+  for (uint32_t step = 0; at.b < none; ++step, advance(at)) {
+    const int slot = (int)(step % kStages);
+    // into the slot of the step before, whose rows are in registers or stored
+    fetch((int)((step + kStages - 1) % kStages));
+    if (at.h == h_lo) {
+      if (half > 0) {
+        const double pos = position_of(s, at.b, at.t);
+        __syncwarp();
+        for (int i = lane; i < half; i += 32) s_turn[warp][i] = turn(pos, s_rate[i]);
+        __syncwarp();
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        cs[i] = 1.f;
+        sn[i] = 0.f;
+        if (INTER) {
+          if (e0 + i < a.rotary) {
+            const float2 c = s_turn[warp][(e0 + i) / 2];
+            cs[i] = c.x;
+            sn[i] = (i & 1) ? c.y : -c.y;
+          }
+        } else if (turned) {
+          const float2 c = s_turn[warp][low ? e0 + i : e0 + i - half];
+          cs[i] = c.x;
+          sn[i] = low ? -c.y : c.y;
+        }
+      }
+      y = static_cast<T*>(s.y) + at.b * s.y_stride_b + at.t * s.y_stride_t + e0;
+    }
+    {
+      const int64_t h = at.h + grp;
       const bool row = held && h < h_hi;
+      copies_wait<kStages - 1>();
       Raw8<T> rx, rp;
       rx.zero();
-      if (row) rx.load(x + h * s.x_stride_h);
+      if (row) rx.load(&s_ring[warp][slot][0][8 * lane]);
       float v[8], sq = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -195,7 +249,7 @@ __global__ void __launch_bounds__(32 * kWarps) vec_kernel(const __grid_constant_
       } else {
         Raw8<T> rd;
         rd.zero();
-        if (row) rd.load(dy + h * s.dy_stride_h);
+        if (row) rd.load(&s_ring[warp][slot][1][8 * lane]);
         float dz[8], dot = 0.f;
         // the inverse turn: the sign of the sine flips
         if (INTER) {
