@@ -6,14 +6,22 @@
 //   dz = R(pos)^T dy,  dweight = sum_rows dz * u,
 //   dx = r (dz * weight - u * mean(dz * weight * u))
 //
-// Bound by memory: forward 2 and backward 3 passes over the rows.  A warp owns
-// the tokens it visits and loops over their heads, so the angles of a token
-// (one fp64 product, a reduction to a fraction of a turn and one sincospi per
-// pair) are formed once per token, shared through 8 bytes per pair of shared
-// memory, and cost about a tenth of the row work at 16 heads.
+// Bound by memory (forward 2 and backward 3 passes over the rows), close behind
+// it by issuing: a warp owns the tokens it visits and loops over their heads, so
+// the angles of a token (one fp64 product, a reduction to a fraction of a turn
+// and one sincospi per pair) are formed once per token and shared through 8
+// bytes per pair of shared memory; with equal positions once for queries and
+// keys.  Arithmetic goes in packed fp32 pairs.
+//
+// B2 N16384 H16 E64 bf16: forward 58 us, backward 85 us, 4.6 and 4.7 TB/s (70 %
+// of a plain copy); B1 N32768 H8 E128: 70 and 91 us.  Steps that led there, at
+// the first size: 97 / 134 us with plain loads in front of their use; 71 / 91
+// with the ring; 64 / 86 with packed arithmetic and the weights folded into the
+// angles; 58 / 85 with the angles shared by both sides.  Eight stages in the
+// ring instead of four, alone: no difference.
 //
 // Two layouts.  `vec`: a row is held by LPR lanes with 8 consecutive entries
-// each (16-byte accesses of bf16, two of fp32), several rows per warp; pairs of
+// each (16-byte copies of bf16, two of fp32), several rows per warp; pairs of
 // halves meet through one shuffle of the raw words.  It needs E % 8 == 0,
 // E <= 256, rotary % 16 == 0 (halves), 16-byte aligned rows.  `scalar`: one row
 // per warp, entry lane + 32 j per lane, partners re-read through L1; any E up to
@@ -21,17 +29,20 @@
 #include <cmath>
 
 #include "sbl_common.cuh"
+#include "sbl_tc_dev.cuh"
 
 namespace sbl {
 namespace {
 
+using namespace tcdev;
+
 constexpr int kWarps = 4;                               // warps per block
-constexpr int kStages = 4;                              // row steps in the ring of a warp
 constexpr int kMaxPairs = SBL_NORM_ROTARY_MAX_E / 2;
 
 struct RotaryArgs {
   SblNormRotarySide side[2];
   int B, E, rotary, wbf16;
+  int joint;                                            // vec: both sides in one warp
   float eps;
   float* partial;                                       // backward: (2, blocks, E), null = no weight gradients
   double rate[kMaxPairs];                               // turns per position of pair i
@@ -83,7 +94,7 @@ struct Raw8<__nv_bfloat16> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = __shfl_sync(0xffffffffu, o.w[i], src);
   }
-  __device__ float at(int i) const { return __uint_as_float((i & 1) ? (w[i >> 1] & 0xffff0000u) : (w[i >> 1] << 16)); }
+  __device__ float2 pair(int i) const { return make_float2(bf16_lo(w[i]), bf16_hi(w[i])); }
   static __device__ void store(__nv_bfloat16* p, const float (&v)[8]) {
     uint4 o;
     __nv_bfloat162 h[4];
@@ -109,7 +120,7 @@ struct Raw8<float> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = __shfl_sync(0xffffffffu, o.w[i], src);
   }
-  __device__ float at(int i) const { return w[i]; }
+  __device__ float2 pair(int i) const { return make_float2(w[2 * i], w[2 * i + 1]); }
   static __device__ void store(float* p, const float (&v)[8]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
     reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -123,47 +134,52 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// grid (blocks over tokens, parts of the heads, sides)
+// grid (blocks over tokens, parts of the heads, sides or 1).  With one part per side a warp takes a token's heads of both
+// sides one after the other (`RotaryArgs::joint`: same tokens, same positions): the angles, a third of the instructions
+// at 16 heads of 64 entries, are formed once for both.
 template <typename T, int LPR, bool BWD, bool INTER>
-__global__ void __launch_bounds__(32 * kWarps) vec_kernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(32 * kWarps, BWD ? 4 : 6) vec_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int RPW = 32 / LPR;                         // rows per warp
+  constexpr int EP = 8 * LPR;                           // entries held
+  constexpr int kStages = sizeof(T) == 4 ? 4 : 8;        // 16 KB per block, 32 KB backward
   __shared__ double s_rate[kMaxPairs / 2];              // E <= 256: 128 pairs
   __shared__ float2 s_turn[kWarps][kMaxPairs / 2];
-  __shared__ float s_dw[BWD ? kWarps : 1][BWD ? 8 * LPR : 1];
-  const SblNormRotarySide& s = a.side[blockIdx.z];
+  __shared__ __align__(16) float s_w[2][EP];
+  __shared__ float s_dw[BWD ? kWarps : 1][BWD ? 2 : 1][BWD ? EP : 1];
+  // The warp's steps, RPW rows of a token each, form one stream.  Rows travel kStages - 1 steps ahead through a ring in
+  // shared memory; a lane reads back what it copied itself, so that nothing but its own copies is waited for.
+  __shared__ __align__(16) T s_ring[kWarps][kStages][BWD ? 2 : 1][32 * 8];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int sub = lane % LPR, grp = lane / LPR;
   const int e0 = 8 * sub, E = a.E, half = a.rotary / 2;
   const bool held = e0 < E;
+  const int side_lo = a.joint ? 0 : blockIdx.z, side_hi = a.joint ? 2 : blockIdx.z + 1;
   for (int i = threadIdx.x; i < half; i += 32 * kWarps) s_rate[i] = a.rate[i];
+  for (int i = threadIdx.x; i < 2 * EP; i += 32 * kWarps)
+    s_w[i / EP][i % EP] = i % EP < E ? weight_at(a.side[i / EP].weight, a.wbf16, i % EP) : 0.f;
   __syncthreads();
   // Halves: entry e is turned with e + half, `half / 8` lanes up (the low one) or down.  rotary % 16 == 0 here.
   const bool low = e0 < half, turned = e0 < a.rotary;
   const int src = INTER || !turned ? lane : (low ? lane + half / 8 : lane - half / 8);
-  float wt[8], wp[8], dw[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int e = e0 + i, ep = INTER || !turned ? e : (low ? e + half : e - half);
-    wt[i] = held ? weight_at(s.weight, a.wbf16, e) : 0.f;
-    wp[i] = held ? weight_at(s.weight, a.wbf16, ep) : 0.f;
-    dw[i] = 0.f;
-  }
-  const int H = s.H, per = (H + gridDim.y - 1) / gridDim.y;
-  const int h_lo = blockIdx.y * per, h_hi = min(H, h_lo + per);
+  const int ep0 = INTER || !turned ? e0 : (low ? e0 + half : e0 - half);
   const float inv_e = 1.f / (float)E;
-  // The warp's steps, RPW rows of a token each, form one stream.  Rows travel kStages - 1 steps ahead through a ring in
-  // shared memory; a lane reads back what it copied itself, so that nothing but its own copies is waited for.
-  __shared__ __align__(16) T s_ring[kWarps][kStages][BWD ? 2 : 1][32 * 8];
-  const uint32_t T_ = (uint32_t)s.T, hop = gridDim.x * kWarps, first = blockIdx.x * kWarps + warp;
+  const uint32_t T_ = (uint32_t)a.side[side_lo].T, hop = gridDim.x * kWarps, first = blockIdx.x * kWarps + warp;
   const uint32_t hop_b = T_ ? hop / T_ : 0, hop_t = T_ ? hop % T_ : 0;
-  struct Cursor { uint32_t b, t; int h; };
-  Cursor at = {T_ ? first / T_ : 0, T_ ? first % T_ : 0, h_lo};
+  struct Cursor { uint32_t b, t; int side, h, end; };
+  auto heads = [&](Cursor& c) {                         // this block's part of the side's heads
+    const int H = a.side[c.side].H, per = (H + gridDim.y - 1) / gridDim.y;
+    c.h = blockIdx.y * per;
+    c.end = min(H, c.h + per);
+  };
+  Cursor at = {T_ ? first / T_ : 0, T_ ? first % T_ : 0, side_lo, 0, 0};
+  heads(at);
   const uint32_t none = (uint32_t)a.B;
-  if (T_ == 0 || h_lo >= h_hi) at.b = none;
-  auto advance = [&](Cursor& c) {
+  if (T_ == 0 || at.h >= at.end) at.b = none;           // (joint: one part, which is never empty)
+  auto advance = [&](Cursor& c) {                       // true: another side or token
     c.h += RPW;
-    if (c.h >= h_hi) {
-      c.h = h_lo;
+    if (c.h < c.end) return false;
+    if (++c.side == side_hi) {
+      c.side = side_lo;
       c.b += hop_b;
       c.t += hop_t;                                     // (both below 2^31)
       if (c.t >= T_) {
@@ -171,124 +187,179 @@ __global__ void __launch_bounds__(32 * kWarps) vec_kernel(const __grid_constant_
         ++c.b;
       }
     }
+    heads(c);
+    return true;
   };
   Cursor ahead = at;
+  const T *x, *dy;
+  int64_t x_hop, dy_hop;
+  auto seek = [&]() {                                   // the lane's row of the step `ahead`
+    const SblNormRotarySide& s = a.side[ahead.side];
+    const int64_t h = ahead.h + grp;
+    x = static_cast<const T*>(s.x) + ahead.b * s.x_stride_b + ahead.t * s.x_stride_t + h * s.x_stride_h + e0;
+    x_hop = RPW * s.x_stride_h;
+    if (BWD) {
+      dy = static_cast<const T*>(s.dy) + ahead.b * s.dy_stride_b + ahead.t * s.dy_stride_t + h * s.dy_stride_h + e0;
+      dy_hop = RPW * s.dy_stride_h;
+    }
+  };
+  T* const ring = &s_ring[warp][0][0][8 * lane];
+  constexpr int SLOT = (BWD ? 2 : 1) * 32 * 8;
   auto fetch = [&](int slot) {
     if (ahead.b < none) {
-      if (held && ahead.h + grp < h_hi) {
-        const int64_t h = ahead.h + grp;
-        copy_row8(&s_ring[warp][slot][0][8 * lane],
-                  static_cast<const T*>(s.x) + ahead.b * s.x_stride_b + ahead.t * s.x_stride_t + h * s.x_stride_h + e0);
-        if (BWD)
-          copy_row8(&s_ring[warp][slot][BWD ? 1 : 0][8 * lane],
-                    static_cast<const T*>(s.dy) + ahead.b * s.dy_stride_b + ahead.t * s.dy_stride_t + h * s.dy_stride_h + e0);
+      if (held && ahead.h + grp < ahead.end) {
+        copy_row8(ring + slot * SLOT, x);
+        if (BWD) copy_row8(ring + slot * SLOT + 32 * 8, dy);
       }
-      advance(ahead);
+      if (advance(ahead)) {
+        seek();
+      } else {
+        x += x_hop;
+        if (BWD) dy += dy_hop;
+      }
     }
     copies_commit();
   };
+  seek();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch(i);
-  float cs[8], sn[8];                                   // y = z * cs + z_partner * sn
+  // y = r (x * cs + x_partner * sn), the weights in them; backward: dz = dy * cs - dy_partner * sn without
+  float2 cs[4], sn[4], wt[4], dw[4], dw_other[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) dw[i] = dw_other[i] = make_float2(0.f, 0.f);
   T* y = nullptr;
-  for (uint32_t step = 0; at.b < none; ++step, advance(at)) {
+  int64_t y_hop = 0;
+  bool fresh = true;
+  for (uint32_t step = 0; at.b < none; ++step) {
     const int slot = (int)(step % kStages);
     // into the slot of the step before, whose rows are in registers or stored
     fetch((int)((step + kStages - 1) % kStages));
-    if (at.h == h_lo) {
-      if (half > 0) {
+    if (fresh) {
+      const SblNormRotarySide& s = a.side[at.side];
+      if (half > 0 && at.side == side_lo) {
         const double pos = position_of(s, at.b, at.t);
         __syncwarp();
         for (int i = lane; i < half; i += 32) s_turn[warp][i] = turn(pos, s_rate[i]);
         __syncwarp();
       }
+      float c[8], n[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        cs[i] = 1.f;
-        sn[i] = 0.f;
+        c[i] = 1.f;
+        n[i] = 0.f;
         if (INTER) {
           if (e0 + i < a.rotary) {
-            const float2 c = s_turn[warp][(e0 + i) / 2];
-            cs[i] = c.x;
-            sn[i] = (i & 1) ? c.y : -c.y;
+            const float2 t = s_turn[warp][(e0 + i) / 2];
+            c[i] = t.x;
+            n[i] = (i & 1) ? t.y : -t.y;
           }
         } else if (turned) {
-          const float2 c = s_turn[warp][low ? e0 + i : e0 + i - half];
-          cs[i] = c.x;
-          sn[i] = low ? -c.y : c.y;
+          const float2 t = s_turn[warp][low ? e0 + i : e0 + i - half];
+          c[i] = t.x;
+          n[i] = low ? -t.y : t.y;
         }
       }
-      y = static_cast<T*>(s.y) + at.b * s.y_stride_b + at.t * s.y_stride_t + e0;
-    }
-    {
-      const int64_t h = at.h + grp;
-      const bool row = held && h < h_hi;
-      copies_wait<kStages - 1>();
-      Raw8<T> rx, rp;
-      rx.zero();
-      if (row) rx.load(&s_ring[warp][slot][0][8 * lane]);
-      float v[8], sq = 0.f;
+      const float2* w = reinterpret_cast<const float2*>(&s_w[at.side][e0]);
+      const float2* wp = reinterpret_cast<const float2*>(&s_w[at.side][ep0]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = rx.at(i);
-        sq = fmaf(v[i], v[i], sq);
-      }
-      if (!BWD) {
-        const float r = rsqrtf(row_sum<LPR>(sq) * inv_e + a.eps);
-        float o[8];
-        if (INTER) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            o[i] = (v[i] * r * wt[i]) * cs[i] + (v[i ^ 1] * r * wt[i ^ 1]) * sn[i];
+      for (int i = 0; i < 4; ++i) {
+        cs[i] = make_float2(c[2 * i], c[2 * i + 1]);
+        sn[i] = make_float2(n[2 * i], n[2 * i + 1]);
+        if (!BWD) {
+          const float2 p = wp[i];
+          cs[i] = mul2(cs[i], w[i]);
+          sn[i] = mul2(sn[i], INTER ? make_float2(p.y, p.x) : p);
         } else {
-          rp.exchange(rx, src);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = (v[i] * r * wt[i]) * cs[i] + (rp.at(i) * r * wp[i]) * sn[i];
+          sn[i] = make_float2(-sn[i].x, -sn[i].y);      // the inverse turn
+          wt[i] = w[i];
         }
-        if (row) Raw8<T>::store(y + h * s.y_stride_h, o);
-      } else {
-        Raw8<T> rd;
-        rd.zero();
-        if (row) rd.load(&s_ring[warp][slot][1][8 * lane]);
-        float dz[8], dot = 0.f;
-        // the inverse turn: the sign of the sine flips
-        if (INTER) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) dz[i] = rd.at(i) * cs[i] - rd.at(i ^ 1) * sn[i];
-        } else {
-          rp.exchange(rd, src);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) dz[i] = rd.at(i) * cs[i] - rp.at(i) * sn[i];
+        if (BWD && a.joint && step > 0) {               // the other side's sums
+          const float2 d = dw[i];
+          dw[i] = dw_other[i];
+          dw_other[i] = d;
         }
+      }
+      y = static_cast<T*>(s.y) + at.b * s.y_stride_b + at.t * s.y_stride_t + (int64_t)(at.h + grp) * s.y_stride_h + e0;
+      y_hop = RPW * s.y_stride_h;
+    }
+    const bool row = held && at.h + grp < at.end;
+    copies_wait<kStages - 1>();
+    Raw8<T> rx, rd;
+    rx.zero();
+    if (row) rx.load(ring + slot * SLOT);
+    if (BWD) {
+      rd.zero();
+      if (row) rd.load(ring + slot * SLOT + 32 * 8);
+    }
+    float2 v[4], sq = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dot = fmaf(dz[i] * wt[i], v[i], dot);
-        const float r = rsqrtf(row_sum<LPR>(sq) * inv_e + a.eps);
-        const float c = row_sum<LPR>(dot) * r * r * inv_e;
-        float o[8];
+    for (int i = 0; i < 4; ++i) {
+      v[i] = rx.pair(i);
+      sq = fma2(v[i], v[i], sq);
+    }
+    // what is turned: x forward, dy backward; its partner is the other half, or the other entry of the pair
+    const Raw8<T>& raw = BWD ? rd : rx;
+    Raw8<T> rp;
+    if (!INTER) rp.exchange(raw, src);
+    float2 z[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float u = v[i] * r;
-          dw[i] = fmaf(dz[i], u, dw[i]);
-          o[i] = r * (dz[i] * wt[i] - v[i] * c);
-        }
-        if (row) Raw8<T>::store(y + h * s.y_stride_h, o);
+    for (int i = 0; i < 4; ++i) {
+      const float2 m = BWD ? raw.pair(i) : v[i];
+      const float2 p = INTER ? make_float2(m.y, m.x) : rp.pair(i);
+      z[i] = fma2(p, sn[i], mul2(m, cs[i]));
+    }
+    const float r = rsqrtf(row_sum<LPR>(sq.x + sq.y) * inv_e + a.eps);
+    const float2 r2 = make_float2(r, r);
+    float o[8];
+    if (!BWD) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 t = mul2(z[i], r2);
+        o[2 * i] = t.x;
+        o[2 * i + 1] = t.y;
+      }
+    } else {
+      float2 zw[4], dot = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        zw[i] = mul2(z[i], wt[i]);
+        dot = fma2(zw[i], v[i], dot);
+        dw[i] = fma2(z[i], mul2(v[i], r2), dw[i]);
+      }
+      const float c = -row_sum<LPR>(dot.x + dot.y) * r * r * inv_e;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 t = mul2(r2, fma2(v[i], make_float2(c, c), zw[i]));
+        o[2 * i] = t.x;
+        o[2 * i + 1] = t.y;
       }
     }
+    if (row) Raw8<T>::store(y, o);
+    y += y_hop;
+    fresh = advance(at);
   }
   if (BWD && a.partial) {
-    // lane groups, then warps, in a fixed order
+    // Lane groups, then warps, in a fixed order.  A joint warp has ended with the second side in `dw` (one without
+    // tokens has zeros in both).
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
 #pragma unroll
-      for (int o = LPR; o < 32; o <<= 1) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-      if (grp == 0) s_dw[warp][e0 + i] = dw[i];
+      for (int side = 0; side < 2; ++side) {
+        const float2 p = side == 0 ? dw[i / 2] : dw_other[i / 2];
+        float d = (i & 1) ? p.y : p.x;
+#pragma unroll
+        for (int o = LPR; o < 32; o <<= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        if (grp == 0) s_dw[warp][a.joint ? 1 - side : side][e0 + i] = d;
+      }
     }
     __syncthreads();
-    const int64_t block = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
-    for (int e = threadIdx.x; e < E; e += 32 * kWarps) {
-      float sum = 0.f;
-      for (int w = 0; w < kWarps; ++w) sum += s_dw[w][e];
-      a.partial[block * E + e] = sum;
+    for (int side = side_lo; side < side_hi; ++side) {
+      const int64_t block = ((int64_t)side * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+      for (int e = threadIdx.x; e < E; e += 32 * kWarps) {
+        float sum = 0.f;
+        for (int w = 0; w < kWarps; ++w) sum += s_dw[w][a.joint ? side : 0][e];
+        a.partial[block * E + e] = sum;
+      }
     }
   }
 }
@@ -425,14 +496,18 @@ bool side_is_vec(const SblNormRotarySide& s, bool bwd) {
 
 // Blocks over tokens and over heads.  Heads are split only while there are too few tokens to give every SM 16 warps
 // (a handful of decoded tokens: one step of rows per warp instead of a loop).
-void plan(const SblNormRotary& p, int rpw, bool bwd, unsigned* gx, unsigned* gy) {
+// Over tokens no more blocks than an SM holds at once (registers), so that all of them end together.
+void plan(const SblNormRotary& p, int rpw, bool bwd, unsigned* gx, unsigned* gy, bool* joint) {
   const int64_t tokens = (int64_t)p.B * (p.side[0].T > p.side[1].T ? p.side[0].T : p.side[1].T);
   const int H = p.side[0].H > p.side[1].H ? p.side[0].H : p.side[1].H;
   const int64_t steps = div_up(H, rpw);
   int64_t parts = 1;
   while (parts * 2 <= steps && tokens * parts * 2 <= 148 * 16) parts *= 2;
   int64_t bx = tokens > 0 ? div_up(tokens, kWarps) : 1;
-  const int64_t most = bwd ? 148 * 4 : 148 * 8;   // per side: the backward's blocks each leave a row of partials
+  const SblNormRotarySide &q = p.side[0], &k = p.side[1];
+  *joint = parts == 1 && q.T == k.T && q.positions == k.positions && q.pos0 == k.pos0 &&
+           (!q.positions || (q.pos_stride_b == k.pos_stride_b && q.pos_stride_t == k.pos_stride_t));
+  const int64_t most = 148 * (bwd ? 4 : 6) / (*joint ? 1 : 2);
   if (bx > most) bx = most;
   *gx = (unsigned)bx;
   *gy = (unsigned)parts;
@@ -444,10 +519,12 @@ cudaError_t launch(const SblNormRotary& p, RotaryArgs& a, cudaStream_t st) {
   const bool vec = p.E % 8 == 0 && p.E <= 256 && (inter || p.rotary % 16 == 0) && side_is_vec(p.side[0], BWD) &&
                    side_is_vec(p.side[1], BWD);
   unsigned gx, gy;
+  bool joint;
   if (vec) {
     const int lpr = p.E <= 32 ? 4 : p.E <= 64 ? 8 : p.E <= 128 ? 16 : 32;
-    plan(p, 32 / lpr, BWD, &gx, &gy);
-    const dim3 grid(gx, gy, 2);
+    plan(p, 32 / lpr, BWD, &gx, &gy, &joint);
+    a.joint = joint;
+    const dim3 grid(gx, gy, a.joint ? 1 : 2);
 #define SBL_VEC(L)                                                                                  \
   (inter ? vec_kernel<T, L, BWD, true><<<grid, 32 * kWarps, 0, st>>>(a)                             \
          : vec_kernel<T, L, BWD, false><<<grid, 32 * kWarps, 0, st>>>(a))
@@ -457,7 +534,7 @@ cudaError_t launch(const SblNormRotary& p, RotaryArgs& a, cudaStream_t st) {
     else SBL_VEC(32);
 #undef SBL_VEC
   } else {
-    plan(p, 1, BWD, &gx, &gy);
+    plan(p, 1, BWD, &gx, &gy, &joint);
     const dim3 grid(gx, gy, 2);
     if (p.E <= 128) scalar_kernel<T, 4, BWD><<<grid, 32 * kWarps, 0, st>>>(a, inter);
     else scalar_kernel<T, 16, BWD><<<grid, 32 * kWarps, 0, st>>>(a, inter);
@@ -475,8 +552,9 @@ cudaError_t launch(const SblNormRotary& p, RotaryArgs& a, cudaStream_t st) {
 size_t norm_rotary_partial_bytes(const SblNormRotary& p) {
   // an upper bound of what plan() may ask for: blocks over tokens x parts of the heads, two sides
   unsigned gx, gy, best = 0;
+  bool joint;
   for (int rpw = 1; rpw <= 8; rpw *= 2) {
-    plan(p, rpw, true, &gx, &gy);
+    plan(p, rpw, true, &gx, &gy, &joint);
     if (gx * gy > best) best = gx * gy;
   }
   return (size_t)best * 2 * p.E * sizeof(float);

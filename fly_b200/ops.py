@@ -3,6 +3,7 @@ launches on the current CUDA stream.  PyTorch is used only for device memory
 and streams; all arithmetic happens in libsblocal_b200.so.
 """
 import collections
+import contextlib
 import ctypes
 import math
 import threading
@@ -68,6 +69,14 @@ class _StatusWatch:
 status_watch = _StatusWatch()
 
 
+def _on(device):
+    """`torch.cuda.device(device)`, or nothing where the device is the current one already (some microseconds of a
+    small call)."""
+    if device.index is not None and device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
 class Problem:
     """One SBLocal problem: parameter block plus the tensors it borrows (kept
     alive for as long as the block is used)."""
@@ -105,23 +114,14 @@ class Problem:
             if key_lengths.shape != (B,):
                 raise ValueError(f'key lengths must have shape ({B},)')
         tau = float(softmax_temp) if softmax_temp else 1.0 / math.sqrt(E)
-        p = _cabi.SblParams()
-        p.dtype = _DTYPES[query.dtype]
-        p.B, p.H, p.T, p.S, p.E, p.D = B, H, T, S, E, D
-        p.r, p.w = W.shape[0], int(local_context)
-        p.softmax_temp, p.softmax_eps = tau, float(softmax_eps)
-        p.q, p.q_stride_b, p.q_stride_t, p.q_stride_h = (query.data_ptr(), query.stride(0), query.stride(1),
-                                                         query.stride(2))
-        p.k, p.k_stride_b, p.k_stride_s, p.k_stride_h = key.data_ptr(), key.stride(0), key.stride(1), key.stride(2)
-        p.v, p.v_stride_b, p.v_stride_s, p.v_stride_h = (value.data_ptr(), value.stride(0), value.stride(1),
-                                                         value.stride(2))
-        p.out, p.o_stride_b, p.o_stride_t, p.o_stride_h = out.data_ptr(), out.stride(0), out.stride(1), out.stride(2)
-        p.W = W32.data_ptr()
-        p.key_lengths = key_lengths.data_ptr() if key_lengths is not None else None
-        p.q_pos0, p.k_pos0 = int(q_pos0), int(k_pos0)
-        p.S_total = int(S_total) if S_total is not None else S
-        p.sum_lo, p.sum_hi = sum_range if sum_range is not None else (0, S)
-        p.flags = _cabi.SBL_FLAG_GENERIC_PATH if generic else 0
+        sum_lo, sum_hi = sum_range if sum_range is not None else (0, S)
+        # (in the order of the fields: one call, where assigning them one by one costs a small call some microseconds)
+        p = _cabi.SblParams(
+            _DTYPES[query.dtype], B, H, T, S, E, D, W.shape[0], int(local_context), tau, float(softmax_eps),
+            query.data_ptr(), *query.stride()[:3], key.data_ptr(), *key.stride()[:3],
+            value.data_ptr(), *value.stride()[:3], out.data_ptr(), *out.stride()[:3], W32.data_ptr(),
+            key_lengths.data_ptr() if key_lengths is not None else None, int(q_pos0), int(k_pos0),
+            int(S_total) if S_total is not None else S, sum_lo, sum_hi, _cabi.SBL_FLAG_GENERIC_PATH if generic else 0)
         self.params = p
         self.device = dev
         self.out = out
@@ -148,7 +148,7 @@ class Problem:
 
     def _call(self, fn, *extra, workspace=None):
         ws = workspace if workspace is not None else self.workspace()
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             stream = torch.cuda.current_stream(self.device).cuda_stream
             rc = fn(ctypes.byref(self.params), ws.data_ptr(), ws.numel(), *extra, stream)
         _cabi.check(rc)
@@ -159,7 +159,7 @@ class Problem:
         """watch: queue a non-blocking copy of the kernels' status words (see `status_watch`)."""
         ws = self._call(_cabi.load().sbl_forward, workspace=workspace)
         if watch and self.status_offset is not None:
-            with torch.cuda.device(self.device):
+            with _on(self.device):
                 status_watch.post(ws, self.status_offset, self.device)
         return self.out
 
@@ -191,13 +191,10 @@ class Problem:
         dq, dk, dv = (torch.empty(x.shape, device=self.device, dtype=x.dtype) for x in (query, key, value))
         # of this call alone: a backward pass may run on another stream or be captured while another one is alive
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        g = _cabi.SblGrads()
-        g.dout, g.do_stride_b, g.do_stride_t, g.do_stride_h = grad_out.data_ptr(), *grad_out.stride()[:3]
-        g.row_stats = row_stats.data_ptr()
-        g.dq, g.dq_stride_b, g.dq_stride_t, g.dq_stride_h = dq.data_ptr(), *dq.stride()[:3]
-        g.dk, g.dk_stride_b, g.dk_stride_s, g.dk_stride_h = dk.data_ptr(), *dk.stride()[:3]
-        g.dv, g.dv_stride_b, g.dv_stride_s, g.dv_stride_h = dv.data_ptr(), *dv.stride()[:3]
-        with torch.cuda.device(self.device):
+        g = _cabi.SblGrads(grad_out.data_ptr(), *grad_out.stride()[:3], row_stats.data_ptr(),
+                           dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3],
+                           dv.data_ptr(), *dv.stride()[:3])
+        with _on(self.device):
             stream = torch.cuda.current_stream(self.device).cuda_stream
             rc = _cabi.load().sbl_backward(ctypes.byref(self.params), ctypes.byref(g), ws.data_ptr(), nbytes, stream)
             _cabi.check(rc)
@@ -290,7 +287,7 @@ class _SBLocal(torch.autograd.Function):
         ws = torch.empty(prob.workspace_bytes, dtype=torch.uint8, device=prob.device)
         out, stats = prob.forward_train(ws)
         if watch and prob.status_offset is not None and not torch.cuda.is_current_stream_capturing():
-            with torch.cuda.device(prob.device):
+            with _on(prob.device):
                 status_watch.post(ws, prob.status_offset, prob.device)
         ctx.stats = True
         ctx.save_for_backward(query, key, value, W, key_lengths, out, stats)
@@ -319,36 +316,29 @@ def sblocal_attention(query, key, value, W, local_context, softmax_temp=None, so
 
 # ---- norm and rotation of query and key heads -------------------------------------------------------------------
 
-def _norm_rotary_params(xs, weights, positions, pos0, rotary_dim, theta, interleaved, eps):
-    """SblNormRotary of the inputs; the tensors it points to must stay alive."""
-    p = _cabi.SblNormRotary()
-    B, _, _, E = xs[0].shape
-    p.dtype = _DTYPES[xs[0].dtype]
+def _norm_rotary_params(xs, ys, weights, positions, pos0, rotary_dim, theta, interleaved, eps, dys=(None, None),
+                        dws=(None, None)):
+    """SblNormRotary of the tensors; those it points to must stay alive."""
+    sides = []
+    for x, y, dy, w, dw, pos in zip(xs, ys, dys, weights, dws, positions):
+        sides.append(_cabi.SblNormRotarySide(
+            x.shape[1], x.shape[2], x.data_ptr(), *x.stride()[:3], y.data_ptr(), *y.stride()[:3],
+            *((dy.data_ptr(), *dy.stride()[:3]) if dy is not None else (None, 0, 0, 0)),
+            w.data_ptr() if w is not None else None, dw.data_ptr() if dw is not None else None,
+            *((pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0, pos.stride(-1)) if pos is not None
+              else (None, 0, 0)), pos0))
     w = weights[0] if weights[0] is not None else weights[1]
-    p.weight_dtype = _DTYPES[w.dtype] if w is not None else _cabi.SBL_DTYPE_F32
-    p.B, p.E, p.rotary, p.interleaved = B, E, rotary_dim, 1 if interleaved else 0
-    p.eps, p.theta = eps, theta
-    for i in range(2):
-        s, x = p.side[i], xs[i]
-        s.T, s.H = x.shape[1], x.shape[2]
-        s.x, s.x_stride_b, s.x_stride_t, s.x_stride_h = x.data_ptr(), *x.stride()[:3]
-        if weights[i] is not None:
-            s.weight = weights[i].data_ptr()
-        if positions[i] is not None:
-            s.positions = positions[i].data_ptr()
-            s.pos_stride_t = positions[i].stride(-1)
-            s.pos_stride_b = positions[i].stride(0) if positions[i].dim() == 2 else 0
-        s.pos0 = pos0
-    return p
+    B, _, _, E = xs[0].shape
+    return _cabi.SblNormRotary(_DTYPES[xs[0].dtype], _DTYPES[w.dtype] if w is not None else _cabi.SBL_DTYPE_F32, B, E,
+                               rotary_dim, 1 if interleaved else 0, eps, theta,
+                               (_cabi.SblNormRotarySide * 2)(*sides))
 
 
-def _norm_rotary_forward(xs, weights, *args):
-    p = _norm_rotary_params(xs, weights, *args)
+def _norm_rotary_forward(xs, weights, positions, *args):
     dev = xs[0].device
     ys = tuple(torch.empty(x.shape, dtype=x.dtype, device=dev) for x in xs)
-    for s, y in zip(p.side, ys):
-        s.y, s.y_stride_b, s.y_stride_t, s.y_stride_h = y.data_ptr(), *y.stride()[:3]
-    with torch.cuda.device(dev):
+    p = _norm_rotary_params(xs, ys, weights, positions, *args)
+    with _on(dev):
         rc = _cabi.load().sbl_norm_rotary_forward(ctypes.byref(p), torch.cuda.current_stream(dev).cuda_stream)
     _cabi.check(rc)
     return ys
@@ -368,17 +358,12 @@ class _NormRotary(torch.autograd.Function):
     def backward(ctx, dq_out, dk_out):
         query, key, query_weight, key_weight, positions, key_positions = ctx.saved_tensors
         weights = (query_weight, key_weight)
-        p = _norm_rotary_params((query, key), weights, (positions, key_positions), *ctx.args)
         dev = query.device
         dys = [dy if dy.stride(-1) == 1 else dy.contiguous() for dy in (dq_out, dk_out)]
         dxs = [torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (query, key)]
         dws = [torch.empty_like(w) if w is not None and ctx.needs_input_grad[2 + i] else None
                for i, w in enumerate(weights)]
-        for s, dy, dx, dw in zip(p.side, dys, dxs, dws):
-            s.dy, s.dy_stride_b, s.dy_stride_t, s.dy_stride_h = dy.data_ptr(), *dy.stride()[:3]
-            s.y, s.y_stride_b, s.y_stride_t, s.y_stride_h = dx.data_ptr(), *dx.stride()[:3]
-            if dw is not None:
-                s.dweight = dw.data_ptr()
+        p = _norm_rotary_params((query, key), dxs, weights, (positions, key_positions), *ctx.args, dys, dws)
         lib = _cabi.load()
         ws, nbytes = None, 0
         if dws[0] is not None or dws[1] is not None:
@@ -386,7 +371,7 @@ class _NormRotary(torch.autograd.Function):
             _cabi.check(lib.sbl_norm_rotary_workspace_bytes(ctypes.byref(p), ctypes.byref(n)))
             nbytes = n.value
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
+        with _on(dev):
             rc = lib.sbl_norm_rotary_backward(ctypes.byref(p), ws.data_ptr() if ws is not None else None, nbytes,
                                               torch.cuda.current_stream(dev).cuda_stream)
         _cabi.check(rc)
