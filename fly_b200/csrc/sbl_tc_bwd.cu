@@ -125,6 +125,18 @@ __device__ __forceinline__ uint32_t seen(const Geom& g, const RowTile& t, int ro
 __device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
   return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~(uintptr_t)1023);
 }
+// Whether a phase is over, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // mbar_wait without the call.  A call makes the issuing warp rebuild every matrix descriptor behind it: about 130
 // cycles per group of four MMAs (256 cycles of work at N = 128), 30 with the loop in line.
 __device__ __forceinline__ void wait_inline(uint64_t* bar, uint32_t parity, int* status, int code) {
@@ -136,6 +148,13 @@ __device__ __forceinline__ void wait_inline(uint64_t* bar, uint32_t parity, int*
       break;
     }
   }
+}
+// The issuing lane asks for a barrier before it issues the products that come before the wait (`seen`), and waits only
+// where the answer was no.  A wait in front of a group of four products costs 30 cycles on an idle SM and 150 to 230
+// beside busy warps, in which the tensor core runs dry; asked ahead, by one lane that runs the whole loop, it costs
+// none (64.4 cycles per N = 128 product, its full rate; 72 to 124 with the wait in place).
+__device__ __forceinline__ void wait_unless(bool seen, uint64_t* bar, uint32_t parity, int* status, int code) {
+  if (!seen) wait_inline(bar, parity, status, code);
 }
 // untiled bulk copy to shared memory: both addresses and the size are multiples of 16 bytes
 __device__ __forceinline__ void bulk_load(void* smem, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -1414,40 +1433,40 @@ struct ValLoader {
   const ValArgs& a;
   uint8_t* smem;
   uint64_t* bars;
-  bool leader;
   int n = 0, loaded = 0;           // ring pieces, phi tiles
+  bool seen = true;                // the next piece's place is free
 
   __device__ uint8_t* piece() {
     const int slot = n % C::NS;
-    if (n >= C::NS) wait_inline(bars + C::R_FREE + slot, ((n / C::NS) - 1) & 1, a.status, 281);
-    if (leader) mbar_expect_tx(bars + C::R_FULL + slot, 16384);
+    wait_unless(seen, bars + C::R_FREE + slot, ((n / C::NS) - 1) & 1, a.status, 281);
+    mbar_expect_tx(bars + C::R_FULL + slot, 16384);
     return smem + C::OFF_RING + slot * 16384;
   }
-  __device__ uint64_t* full() { return bars + C::R_FULL + (n++ % C::NS); }
+  __device__ uint64_t* full() {
+    uint64_t* bar = bars + C::R_FULL + (n++ % C::NS);
+    seen = n < C::NS || mbar_test(bars + C::R_FREE + n % C::NS, ((n / C::NS) - 1) & 1);
+    return bar;
+  }
   __device__ void phi(const RowTile& t, int it) {
     const int buf = it % C::KBUF;
     if (it >= C::KBUF) wait_inline(bars + C::F_FREE + buf, ((it / C::KBUF) - 1) & 1, a.status, 282);
-    if (leader) {
-      mbar_expect_tx(bars + C::F_FULL + buf, C::FB);
-      for (int j = 0; j < C::M / 64; ++j)
-        tma_load_3d(smem + C::OFF_F + buf * C::FB + j * 16384, &a.tm_phi, bars + C::F_FULL + buf, 64 * j, t.r0, t.bh);
-    }
+    mbar_expect_tx(bars + C::F_FULL + buf, C::FB);
+    for (int j = 0; j < C::M / 64; ++j)
+      tma_load_3d(smem + C::OFF_F + buf * C::FB + j * 16384, &a.tm_phi, bars + C::F_FULL + buf, 64 * j, t.r0, t.bh);
     loaded = it + 1;
   }
   __device__ void score(const RowTile& t, int s, int ke, int) {
     if (s == 0) {
       const int buf = ke % C::KBUF;
       if (ke >= C::KBUF) wait_inline(bars + C::K_FREE + buf, ((ke / C::KBUF) - 1) & 1, a.status, 283);
-      if (leader) {
-        mbar_expect_tx(bars + C::K_FULL + buf, C::KB);
-        for (int j = 0; j < C::NB; ++j)
-          tma_load_4d(smem + C::OFF_K + buf * C::KB + j * 16384, &a.tm_k, bars + C::K_FULL + buf, 64 * j, t.r0, t.h, t.b);
-      }
+      mbar_expect_tx(bars + C::K_FULL + buf, C::KB);
+      for (int j = 0; j < C::NB; ++j)
+        tma_load_4d(smem + C::OFF_K + buf * C::KB + j * 16384, &a.tm_k, bars + C::K_FULL + buf, 64 * j, t.r0, t.h, t.b);
     }
     for (int j = 0; j < C::NB; ++j) {
       uint8_t* dst = piece();
       uint64_t* bar = full();
-      if (leader) tma_load_4d(dst, &a.tm_q, bar, 64 * j, t.c0 + 128 * s, t.h, t.b);
+      tma_load_4d(dst, &a.tm_q, bar, 64 * j, t.c0 + 128 * s, t.h, t.b);
     }
   }
   __device__ void begin(const RowTile& t, int it) {
@@ -1457,7 +1476,7 @@ struct ValLoader {
     for (int j = 0; j < C::M / 64; ++j) {
       uint8_t* dst = piece();
       uint64_t* bar = full();
-      if (leader) tma_load_3d(dst, &a.tm_psi, bar, 64 * j, t.c0 + 128 * s, t.bh);
+      tma_load_3d(dst, &a.tm_psi, bar, 64 * j, t.c0 + 128 * s, t.bh);
     }
     // two phi buffers: the next tile's features come in behind this tile's first step (the previous tile's last
     // product with its buffer was issued before this tile began)
@@ -1470,7 +1489,7 @@ struct ValLoader {
     for (int j = 0; j < C::NB; ++j) {
       uint8_t* dst = piece();
       uint64_t* bar = full();
-      if (leader) tma_load_4d(dst, &a.tm_do, bar, 64 * j, t.c0 + 128 * s, t.h, t.b);
+      tma_load_4d(dst, &a.tm_do, bar, 64 * j, t.c0 + 128 * s, t.h, t.b);
     }
   }
   __device__ void rank(const RowTile& t, int, bool, bool) {
@@ -1478,7 +1497,7 @@ struct ValLoader {
       for (int j = 0; j < C::NB; ++j) {
         uint8_t* dst = piece();
         uint64_t* bar = full();
-        if (leader) tma_load_3d(dst, &a.tm_sum, bar, 64 * j, 128 * f, t.bh);
+        tma_load_3d(dst, &a.tm_sum, bar, 64 * j, 128 * f, t.bh);
       }
   }
 };
@@ -1488,97 +1507,90 @@ struct ValIssuer {
   using C = ValCfg<D>;
   const ValArgs& a;
   uint64_t* bars;
-  bool leader;
   uint64_t dK, dF, dR, dRt;
-  int n = 0;
+  int n = 0, m = 0;                // ring pieces, differences
+  bool r_seen = false, e_seen = false, d_seen = false;
 
   __device__ int take() {          // the next ring piece, landed
     const int slot = n % C::NS;
-    wait_inline(bars + C::R_FULL + slot, (n / C::NS) & 1, a.status, 284);
+    wait_unless(r_seen, bars + C::R_FULL + slot, (n / C::NS) & 1, a.status, 284);
     ++n;
-    tc_fence_after_sync();
+    r_seen = mbar_test(bars + C::R_FULL + n % C::NS, (n / C::NS) & 1);
     return slot;
   }
   __device__ void score(const RowTile& t, int s, int ke, int g) {
     const int kb = ke % C::KBUF;
     if (s == 0) wait_inline(bars + C::K_FULL + kb, (ke / C::KBUF) & 1, a.status, 285);
     constexpr uint32_t id = idesc_bf16(128, 128, false, false);
+#pragma unroll
     for (int j = 0; j < C::NB; ++j) {
       const int slot = take();
-      if (leader) {
+      if (j == C::NB - 1) e_seen = mbar_test(bars + C::E_DONE + m % 3, (m / 3) & 1);
+      tc_fence_after_sync();
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mma_ss(128 * (g % 3), dK + (uint64_t)(kb * (C::KB >> 4) + j * 1024 + 2 * k), dR + (uint64_t)(slot * 1024 + 2 * k), id,
-                 j > 0 || k > 0);
-        mma_commit(bars + C::R_FREE + slot);
-      }
-      __syncwarp();
+      for (int k = 0; k < 4; ++k)
+        mma_ss(128 * (g % 3), dK + (uint64_t)(kb * (C::KB >> 4) + j * 1024 + 2 * k), dR + (uint64_t)(slot * 1024 + 2 * k), id,
+               j > 0 || k > 0);
+      mma_commit(bars + C::R_FREE + slot);
     }
-    if (leader) {
-      mma_commit(bars + C::S_FULL + g % 3);
-      if (s == t.n - 1) mma_commit(bars + C::K_FREE + kb);
-    }
-    __syncwarp();
+    mma_commit(bars + C::S_FULL + g % 3);
+    if (s == t.n - 1) mma_commit(bars + C::K_FREE + kb);
   }
   __device__ void begin(const RowTile&, int it) {
     wait_inline(bars + C::F_FULL + it % C::KBUF, (it / C::KBUF) & 1, a.status, 286);
   }
   __device__ void minus(const RowTile&, int it, int, int g) {
-    wait_inline(bars + C::E_DONE + g % 3, (g / 3) & 1, a.status, 287);
+    wait_unless(e_seen, bars + C::E_DONE + g % 3, (g / 3) & 1, a.status, 287);
+    m = g + 1;
+    e_seen = false;
     constexpr uint32_t id = idesc_bf16(128, 128, false, false) | (1u << 13);   // bit 13 negates A
     const int fb = it % C::KBUF;
+#pragma unroll
     for (int j = 0; j < C::M / 64; ++j) {
       const int slot = take();
-      if (leader) {
+      if (j == C::M / 64 - 1 && g > 0) d_seen = mbar_test(bars + C::D_DONE + (g - 1) % 3, ((g - 1) / 3) & 1);
+      tc_fence_after_sync();
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mma_ss(128 * (g % 3), dF + (uint64_t)(fb * (C::FB >> 4) + j * 1024 + 2 * k), dR + (uint64_t)(slot * 1024 + 2 * k), id,
-                 true);
-        mma_commit(bars + C::R_FREE + slot);
-      }
-      __syncwarp();
+      for (int k = 0; k < 4; ++k)
+        mma_ss(128 * (g % 3), dF + (uint64_t)(fb * (C::FB >> 4) + j * 1024 + 2 * k), dR + (uint64_t)(slot * 1024 + 2 * k), id,
+               true);
+      mma_commit(bars + C::R_FREE + slot);
     }
-    if (leader) mma_commit(bars + C::P_FULL + g % 3);
-    __syncwarp();
+    mma_commit(bars + C::P_FULL + g % 3);
   }
   __device__ void value(const RowTile&, int it, int, int g, bool first, bool last) {
-    wait_inline(bars + C::D_DONE + g % 3, (g / 3) & 1, a.status, 288);
+    wait_unless(d_seen, bars + C::D_DONE + g % 3, (g / 3) & 1, a.status, 288);
+    d_seen = false;
     if (first && it >= 1) wait_inline(bars + C::DV_FREE, (it - 1) & 1, a.status, 289);
     constexpr uint32_t id = idesc_bf16(128, 64, false, true);
+#pragma unroll
     for (int j = 0; j < C::NB; ++j) {
       const int slot = take();
-      if (leader) {
+      tc_fence_after_sync();
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          mma_ts(C::T_DV + 64 * j, 128 * (g % 3) + packed(k), dRt + (uint64_t)(slot * 1024 + k * 128), id, !first || k > 0);
-        mma_commit(bars + C::R_FREE + slot);
-      }
-      __syncwarp();
+      for (int k = 0; k < 8; ++k)
+        mma_ts(C::T_DV + 64 * j, 128 * (g % 3) + packed(k), dRt + (uint64_t)(slot * 1024 + k * 128), id, !first || k > 0);
+      mma_commit(bars + C::R_FREE + slot);
     }
-    if (leader && last) mma_commit(bars + C::DV_FULL);
-    __syncwarp();
+    if (last) mma_commit(bars + C::DV_FULL);
   }
   __device__ void rank(const RowTile&, int it, bool first, bool alone) {
     if (first && it >= 1) wait_inline(bars + C::DV_FREE, (it - 1) & 1, a.status, 290);
     constexpr uint32_t id = idesc_bf16(128, 64, false, true);
     const int fb = it % C::KBUF;
     for (int f = 0; f < C::M / 128; ++f)
+#pragma unroll
       for (int j = 0; j < C::NB; ++j) {
         const int slot = take();
-        if (leader) {
+        tc_fence_after_sync();
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            mma_ss(C::T_DV + 64 * j, dF + (uint64_t)(fb * (C::FB >> 4) + 2 * f * 1024) + kmajor(k, 16384),
-                   dRt + (uint64_t)(slot * 1024 + k * 128), id, !first || f > 0 || k > 0);
-          mma_commit(bars + C::R_FREE + slot);
-        }
-        __syncwarp();
+        for (int k = 0; k < 8; ++k)
+          mma_ss(C::T_DV + 64 * j, dF + (uint64_t)(fb * (C::FB >> 4) + 2 * f * 1024) + kmajor(k, 16384),
+                 dRt + (uint64_t)(slot * 1024 + k * 128), id, !first || f > 0 || k > 0);
+        mma_commit(bars + C::R_FREE + slot);
       }
-    if (leader) {
-      mma_commit(bars + C::F_FREE + fb);
-      if (alone) mma_commit(bars + C::DV_FULL);
-    }
-    __syncwarp();
+    mma_commit(bars + C::F_FREE + fb);
+    if (alone) mma_commit(bars + C::DV_FULL);
   }
 };
 
@@ -1607,15 +1619,19 @@ __global__ void __launch_bounds__(576, 1) bwd_value_kernel(const __grid_constant
   const int step = gridDim.x;
 
   if (warp == C::W_LOAD) {
-    ValLoader<D> v{a, smem, bars, elect_one()};
-    walk_values(a.g, v);
+    if (elect_one()) {
+      ValLoader<D> v{a, smem, bars};
+      walk_values(a.g, v);
+    }
     __syncwarp();
   } else if (warp == C::W_MMA) {
-    ValIssuer<D> v{a, bars, elect_one(), smem_desc_sw128(smem_u32(smem + C::OFF_K), 16, 1024),
-                   smem_desc_sw128(smem_u32(smem + C::OFF_F), 16, 1024),
-                   smem_desc_sw128(smem_u32(smem + C::OFF_RING), 16, 1024),
-                   smem_desc_sw128(smem_u32(smem + C::OFF_RING), 16384, 1024)};
-    walk_values(a.g, v);
+    if (elect_one()) {
+      ValIssuer<D> v{a, bars, smem_desc_sw128(smem_u32(smem + C::OFF_K), 16, 1024),
+                     smem_desc_sw128(smem_u32(smem + C::OFF_F), 16, 1024),
+                     smem_desc_sw128(smem_u32(smem + C::OFF_RING), 16, 1024),
+                     smem_desc_sw128(smem_u32(smem + C::OFF_RING), 16384, 1024)};
+      walk_values(a.g, v);
+    }
     __syncwarp();
   } else {
     // exponential group (warps 0-7): S -> p in place; packing group (warps 8-15): p - a -> bf16, epilogue.
