@@ -238,13 +238,18 @@ struct FeatCfg {
   static constexpr uint32_t OFF_W = 0, OFF_X = 2 * WB, OFF_Y = OFF_X + XD * XB, OFF_A = OFF_Y + 2 * YB;
   static constexpr uint32_t OFF_BAR = OFF_A + 2 * 32768;
   static constexpr uint32_t SMEM = OFF_BAR + 256 + 1024;
-  static constexpr int NFEAT = 256, NTHR = NFEAT + 64;
+  // Groups of eight warps that take the tiles in turn.  Head dim 64: two (110 and 94 us for queries and keys, with one 127
+  // and 100: B2 H16 N16384).  128 has room for one X tile only and waits for that: 169 and 163 us with one, 171 and 170
+  // with two (B1 H8 N32768).
+  static constexpr int GROUPS = D == 64 ? 2 : 1;
+  static constexpr int NFEAT = 256 * GROUPS, NTHR = NFEAT + 64, W_LOAD = NFEAT / 32, W_MMA = W_LOAD + 1;
   static constexpr uint32_t T_U = 0, T_SUM = 128;        // 2 x 64 | D + 16
+  static_assert(GROUPS <= XD, "a group sees every phase of the X slots it reads");
   static_assert(SMEM <= 232448, "dynamic shared memory of one CTA");
 };
 
 template <int SIDE, int D>
-__global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant__ FeatArgs a) {
+__global__ void __launch_bounds__(FeatCfg<D>::NTHR, 1) bwd_feat_kernel(const __grid_constant__ FeatArgs a) {
   using C = FeatCfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
@@ -274,7 +279,7 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
     }
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == C::W_LOAD) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -289,7 +294,7 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
   constexpr uint32_t tb = 0;   // the CTA owns all 512 tensor-memory columns of its SM
   if (tid == 0 && *tmem_slot != 0) atomicCAS(a.status, 0, 241);
 
-  if (warp == 8) {
+  if (warp == C::W_LOAD) {
     const bool leader = elect_one();
     if (leader) {
       mbar_expect_tx(bar_w, 2 * C::WB);
@@ -320,7 +325,7 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == C::W_MMA) {
     const bool leader = elect_one();
     constexpr uint32_t id_u = idesc_bf16(128, 64, false, false);
     constexpr uint32_t id_s = idesc_bf16(128, D + 16, true, true);
@@ -376,7 +381,8 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
     }
     __syncwarp();
   } else {
-    const int qd = warp & 3, cq = warp >> 2;
+    // a thread owns a row and 32 of the block's 64 projections
+    const int grp = warp >> 3, qd = warp & 3, cq = (warp >> 2) & 1;
     const int row = qd * 32 + lane;
     const uint32_t lane_base = tb + ((uint32_t)(qd * 32) << 16);
     const float beta = a.beta[bh];
@@ -385,9 +391,12 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
       const int64_t l = a.lengths[b];
       len = l < 0 ? 0 : (l < a.rows ? (int)l : a.rows);
     }
-    for (int i = 0; i < nt; ++i) {
+    const float2* nd = a.nd + (int64_t)bh * a.Tp;
+    for (int i = grp; i < nt; i += C::GROUPS) {
       const int s = i & 1, xs = i % C::XD;
       const int r = (t_lo + i) * TR + row;
+      float2 own = make_float2(0.f, 0.f);
+      if (SIDE == QUERIES) own = __ldg(nd + r);   // r < Tp: the row arrays are padded to whole tiles
       mbar_wait(x_full + xs, (i / C::XD) & 1, a.status, 208);
       float sq = 0.f;
 #pragma unroll
@@ -398,10 +407,8 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
       if (SIDE == KEYS) {
         off = (-g - a.half_log_m - beta) * kLog2e;
       } else {
-        // r < Tp: the row arrays are padded to whole tiles
-        const float2 nd = __ldg(a.nd + (int64_t)bh * a.Tp + r);
-        off = (-g - a.half_log_m + beta) * kLog2e - nd.x;
-        dl = nd.y;
+        off = (-g - a.half_log_m + beta) * kLog2e - own.x;
+        dl = own.y;
       }
       if (fb == 0 && cq == 0) a.off[((int64_t)bh * ntiles + t_lo + i) * TR + row] = live ? off : -INFINITY;
       mbar_wait(u_full + s, (i >> 1) & 1, a.status, 209);   // U computed: the X tile has been read too
@@ -444,9 +451,9 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
     tc_fence_after_sync();
     float* prow = a.partial + (((int64_t)bh * a.nsplit + split) * C::M + 128 * fb + row) * (D + 4);
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
+    for (int j = 0; j < D / (32 * C::GROUPS); ++j) {
       uint32_t r[16];
-      const int c = (D / 2) * cq + 16 * j;
+      const int c = (D / (2 * C::GROUPS)) * (2 * grp + cq) + 16 * j;
       tmem_ld16(lane_base + C::T_SUM + c, r);
       tmem_ld_wait();
 #pragma unroll
@@ -457,11 +464,11 @@ __global__ void __launch_bounds__(320, 1) bwd_feat_kernel(const __grid_constant_
     uint32_t r[16];
     tmem_ld16(lane_base + C::T_SUM + D, r);
     tmem_ld_wait();
-    if (cq == 0) prow[D] = nt == 0 ? 0.f : __uint_as_float(r[0]) + (SIDE == QUERIES ? __uint_as_float(r[1]) : 0.f);
+    if (cq == 0 && grp == 0) prow[D] = nt == 0 ? 0.f : __uint_as_float(r[0]) + (SIDE == QUERIES ? __uint_as_float(r[1]) : 0.f);
   }
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == C::W_LOAD) {
     __syncwarp();
     tmem_dealloc(tb, 512);
   }
