@@ -172,47 +172,60 @@ __device__ __forceinline__ uint32_t packed(int k) { return 32u * (uint32_t)(k >>
 // ---------------------------------------------------------------------------
 // Per query row: (log-normaliser * log2(e), delta = dout . out), (BH, Tp); zero in the padding rows.  Head dim 128:
 // delta once more by itself.
-// D / 8 lanes per row, four rows per group of lanes with all their loads in flight.
+// A block owns 32 positions of up to 16 heads: it reads them heads innermost, as they lie in memory, D / 8 lanes per row
+// and four rows per group of lanes with all their loads in flight, and writes the results by head through shared
+// memory, 256 bytes at a time.  (Written one by one, a plane apart: 46 us where this takes 30, B2 H16 N16384.)
+constexpr int kRowHeads = 16, kRowSpan = 32;
 template <int D>
 __global__ void __launch_bounds__(256) bwd_rows_kernel(const __nv_bfloat16* out, int64_t ob, int64_t ot, int64_t oh,
                                                        const __nv_bfloat16* dout, int64_t db, int64_t dt, int64_t dh,
                                                        const float* stats, int B, int H, int T, int Tp, float2* nd,
                                                        float* delta) {
   constexpr int LPR = D / 8, RPB = 256 / LPR;
-  const int sub = threadIdx.x % LPR;
-  const int64_t total = (int64_t)B * H * Tp, rows = (int64_t)B * H * T;
-  uint4 x[4], y[4];
-  int h[4], t[4], b[4];
+  __shared__ float s_delta[kRowHeads][kRowSpan + 1];
+  const int sub = threadIdx.x % LPR, slot = threadIdx.x / LPR;
+  const int t0 = blockIdx.x * kRowSpan, h0 = blockIdx.y * kRowHeads, b = blockIdx.z;
+  const int nh = min(kRowHeads, H - h0), n = nh * kRowSpan;
+  out += b * ob;
+  dout += b * db;
+  for (int base = 0; base < n; base += 4 * RPB) {
+    uint4 x[4], y[4];
+    int h[4], t[4];
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int64_t i = ((int64_t)blockIdx.x * 4 + u) * RPB + threadIdx.x / LPR;   // (b, t, h), heads innermost
-    h[u] = (int)(i % H);
-    t[u] = (int)((i / H) % Tp);
-    b[u] = i < total ? (int)(i / ((int64_t)H * Tp)) : -1;
-    x[u] = y[u] = make_uint4(0, 0, 0, 0);
-    if (b[u] >= 0 && t[u] < T) {
-      x[u] = __ldg(reinterpret_cast<const uint4*>(out + b[u] * ob + t[u] * ot + h[u] * oh) + sub);
-      y[u] = __ldg(reinterpret_cast<const uint4*>(dout + b[u] * db + t[u] * dt + h[u] * dh) + sub);
+    for (int u = 0; u < 4; ++u) {
+      const int i = base + u * RPB + slot;
+      t[u] = i / nh;
+      h[u] = i - t[u] * nh;
+      x[u] = y[u] = make_uint4(0, 0, 0, 0);
+      if (i < n && t0 + t[u] < T) {
+        x[u] = __ldg(reinterpret_cast<const uint4*>(out + (t0 + t[u]) * ot + (h0 + h[u]) * oh) + sub);
+        y[u] = __ldg(reinterpret_cast<const uint4*>(dout + (t0 + t[u]) * dt + (h0 + h[u]) * dh) + sub);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, yw[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s = fmaf(bf16_lo(xw[j]), bf16_lo(yw[j]), s);
+        s = fmaf(bf16_hi(xw[j]), bf16_hi(yw[j]), s);
+      }
+#pragma unroll
+      for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (sub == 0 && base + u * RPB + slot < n) s_delta[h[u]][t[u]] = s;
     }
   }
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, yw[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s = fmaf(bf16_lo(xw[j]), bf16_lo(yw[j]), s);
-      s = fmaf(bf16_hi(xw[j]), bf16_hi(yw[j]), s);
-    }
-#pragma unroll
-    for (int o = 1; o < LPR; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (b[u] >= 0 && sub == 0) {
-      const int64_t bh = (int64_t)b[u] * H + h[u];
-      float n = 0.f;
-      if (t[u] < T) n = stats[bh * T + t[u]] * kLog2e + log2f(stats[rows + bh * T + t[u]]);
-      nd[bh * Tp + t[u]] = make_float2(n, s);
-      if (D == 128) delta[bh * Tp + t[u]] = s;
-    }
+  __syncthreads();
+  const int64_t rows = (int64_t)B * H * T;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int h = i / kRowSpan, t = t0 + i % kRowSpan;      // (t < Tp, a multiple of kRowSpan)
+    const int64_t bh = (int64_t)b * H + h0 + h;
+    const float s = s_delta[h][i % kRowSpan];
+    float m = 0.f;
+    if (t < T) m = stats[bh * T + t] * kLog2e + log2f(stats[rows + bh * T + t]);
+    nd[bh * Tp + t] = make_float2(m, s);
+    if (D == 128) delta[bh * Tp + t] = s;
   }
 }
 
@@ -1883,8 +1896,7 @@ cudaError_t backward(const Host& h) {
   if ((e = tc_prepare_projection(p, h.ws.fwd, h.base, h.st, true, beta, h.at<__nv_bfloat16>(h.ws.wlo))) != cudaSuccess)
     return e;
   if ((e = tc_key_logscale_bound(p, h.ws.fwd, h.base, beta, h.st, true)) != cudaSuccess) return e;
-  const int64_t lanes = (int64_t)BH * h.ws.Tp * (D / 8);
-  bwd_rows_kernel<D><<<(unsigned)div_up(lanes, 1024), 256, 0, h.st>>>(
+  bwd_rows_kernel<D><<<dim3((unsigned)(h.ws.Tp / kRowSpan), (unsigned)div_up(p.H, kRowHeads), (unsigned)p.B), 256, 0, h.st>>>(
       static_cast<const __nv_bfloat16*>(p.out), p.o_stride_b, p.o_stride_t, p.o_stride_h,
       static_cast<const __nv_bfloat16*>(g.dout), g.do_stride_b, g.do_stride_t, g.do_stride_h, g.row_stats, p.B, p.H, p.T,
       h.ws.Tp, h.at<float2>(h.ws.nd), h.at<float>(h.ws.delta));
