@@ -16,19 +16,24 @@
 //             memory), df += Y summary^T; U = X Wt^T, du = (f df)_+ - (f df)_-, dx += du Wt; writes dq or dk.
 //             Head dim 64: the exact part too (S beside G, dx += (p g) X'); 128: adds the window kernel's
 //
+// Measured, us: B2 H16 N16384 d64 w256 | B1 H8 N32768 d128 w512
+//   rows 30 | 26   feat, queries and keys 103 + 93 | 168 + 163   combine 2 x 3.5 | 2 x 8   window - | 182 + 190
+//   dvalue 226 | 325   grad, queries and keys 293 + 325 | 395 + 405
+// The tensor core is busy for a third of that or less; what bounds each kernel stands beside it.
+//
 // Numerics.  Products take bf16 operands and accumulate in fp32.  Rounded to bf16
 // (half a step, 2^-9 on average): phi and psi as operands, g, p g, p - a.  Carried
 // as two bf16 terms (16 bits): the projection, the summaries and du -- each alone
 // would add as much to the error of dq and dk as the features do.  The own
 // features of a row are formed again in fp32 for du instead of being read back.
 //
-// Where a tile's columns are few (`complement`), df is summed over the columns
+// Where a tile's columns are few (`whole`), df is summed over the columns
 // OUTSIDE the window directly instead of all - inside: a short sequence lies
 // inside its windows almost entirely, and the difference of two sums of bf16
 // products would leave their rounding where the exact value is next to nothing.
 //
 // Feature order: block of 128 = "+" features of 64 projections, then their "-".
-// All waits are bounded (mbar_wait): a wait that runs out sets the first word of
+// All waits are bounded (mbar_wait, wait_inline): a wait that runs out sets the first word of
 // the workspace and the kernel runs to its end.
 #include "sbl_common.cuh"
 #include "sbl_tc_dev.cuh"
@@ -530,7 +535,8 @@ struct WinArgs {
 
 template <int D>
 struct WinCfg {
-  static constexpr int NB = D / 64, NS = D == 64 ? 6 : 3;
+  static_assert(D == 128, "head dim 64 has its exact part in the gradient kernel");
+  static constexpr int NB = D / 64, NS = 3;
   static constexpr uint32_t TB = NB * 16384, SLOT = 2 * NB * 8192;
   static constexpr uint32_t OFF_X = 0, OFF_Y = 2 * TB, OFF_RING = 4 * TB, OFF_BAR = OFF_RING + NS * SLOT;
   static constexpr uint32_t SMEM = OFF_BAR + 512 + 1024;
@@ -541,6 +547,8 @@ struct WinCfg {
   static_assert(SMEM <= 232448 && COUNT <= 60, "shared memory of one CTA");
 };
 
+// Bound: the chain of a step (S and G -> p g -> dx) over two buffers, 2.4 k cycles per step with 1.1 k of products; the
+// 32 KB that a step brings in take 0.8 k.
 template <int SIDE, int D>
 __global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constant__ WinArgs a) {
   using C = WinCfg<D>;
@@ -724,15 +732,7 @@ __global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constan
         const int db = ne & 1;
         mbar_wait(bars + C::DX_FULL + db, (ne >> 1) & 1, a.status, 228);
         tc_fence_after_sync();
-        if constexpr (NC == 32) {
-          tmem_ld32(lane_base + C::T_DX + D * db + c, v);
-        } else {
-          uint32_t w[16];
-          tmem_ld16(lane_base + C::T_DX + D * db + c, w);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = w[j];
-        }
+        tmem_ld32(lane_base + C::T_DX + D * db + c, v);
         tmem_ld_wait();
         tc_fence_before_sync();
         warp_arrive(bars + C::DX_FREE + db, lane);
@@ -782,9 +782,11 @@ struct GradArgs {
 // G on.  Every compute warp loads its U before it waits for df, so that the next tile's first G and S form meanwhile;
 // the group whose turn it is packs that step before it finishes the tile.
 //
-// Bound: the chain of a tile (last step -> df -> du -> dx -> stored) beside the stream into shared memory.  A step's
-// 64 columns are 32 KB of features and 16 KB of X' and Y'; with the summary and the own rows 368 KB per tile and
-// side, 8.8 k cycles at the 41.7 B/clk one SM's TMA loads sustain.
+// Bound: two chains beside the stream into shared memory.  A step's (G and S -> read -> packed -> df, dx) takes 1.4 k
+// cycles, because there is no room for a second G and S beside df; a tile's (last step -> df -> du -> dx -> stored)
+// 5 k.  With six steps 20 k cycles a tile at head dim 64 and w = 256, of which products take 8.7 k.  A step's 64
+// columns are 32 KB of features and 16 KB of X' and Y'; with the summary and the own rows 368 KB per tile, 8.8 k
+// cycles at the 41.7 B/clk that one SM's TMA loads sustain.
 template <int D>
 struct GradCfg {
   static constexpr bool FUSE = D == 64;
@@ -1387,6 +1389,15 @@ struct ValCfg {
   static_assert(SMEM <= 232448 && COUNT <= 60, "shared memory of one CTA");
 };
 
+// S = K Q^T -> p (exponential group, in place) -> p - phi psi^T (accumulated onto p) -> bf16 (packing group, in place)
+// -> dv += (p - a) dO; then dv += phi summary.
+//
+// Bound: one lane issues and one loads, in 16-KB pieces of four or eight products: 25 pieces and 17 k cycles a tile at
+// head dim 64 and w = 256, of which the products take 5.4 k and the stream into shared memory 10.4 k.  Two issuing
+// warps with a ring and a loader of their own each take 264 us for 226, because that leaves room for one phi tile
+// instead of two (head dim 128: 395 for 325); log-normalisers through shared memory instead of __ldg cost a fifth:
+// its whole bandwidth goes to products with both operands there (8 KB in 64 cycles at N = 128).
+//
 // The order in which the tensor core consumes what the producer loads; both walk it.  Column steps (128 queries) are
 // numbered g = 0, 1, .. over the CTA's tiles and use buffer g % 3.  The visitor's calls:
 //   score(tile t, first, ke, g)   S of step g; t is where it belongs, ke the number of that tile among those with steps
