@@ -251,7 +251,7 @@ static int forward(const SblParams* p, void* workspace, size_t workspace_bytes, 
   if (rc != SBL_OK) return rc;
   char* base = static_cast<char*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
-  float* beta = reinterpret_cast<float*>(base + ws.beta);
+  float* beta = row_stats ? row_stats + 2 * (int64_t)p->B * p->H * p->T : reinterpret_cast<float*>(base + ws.beta);
   float* kv = reinterpret_cast<float*>(base + ws.kv);
   float* ksum = reinterpret_cast<float*>(base + ws.ksum);
   cudaError_t e;

@@ -707,7 +707,6 @@ void f32_plan_backward(const SblParams& p, BwdWorkspace* ws) {
   f.tensor = false;
   f.wt = take((size_t)p.r * p.E * 4);
   f.phik = take(BH * S * m * 4);
-  f.beta = take(BH * 4);
   ws->lognorm = take(BH * T * 4);
   ws->scale = take(BH * T * 4);
   ws->delta = take(BH * T * 4);
@@ -732,7 +731,7 @@ void f32_plan_backward(const SblParams& p, BwdWorkspace* ws) {
 }
 
 cudaError_t f32_backward(const SblParams& p, const SblGrads& g, const BwdWorkspace& ws, char* base, cudaStream_t st) {
-  float* beta = reinterpret_cast<float*>(base + ws.fwd.beta);
+  const float* beta = g.row_stats + 2 * (int64_t)p.B * p.H * p.T;
   float* phi = reinterpret_cast<float*>(base + ws.fwd.phik);
   float* lognorm = reinterpret_cast<float*>(base + ws.lognorm);
   float* scale = reinterpret_cast<float*>(base + ws.scale);
@@ -740,7 +739,6 @@ cudaError_t f32_backward(const SblParams& p, const SblGrads& g, const BwdWorkspa
   float* psi = reinterpret_cast<float*>(base + ws.psi);
   cudaError_t e;
   if ((e = f32_prepare_projection(p, ws.fwd, base, st)) != cudaSuccess) return e;
-  if ((e = f32_key_logscale(p, ws.fwd, base, beta, st)) != cudaSuccess) return e;
   if ((e = f32_key_features(p, ws.fwd, base, beta, phi, st)) != cudaSuccess) return e;
   const unsigned blocks = (unsigned)div_up((int64_t)p.B * p.H * p.T, 8);
   if (p.dtype == SBL_DTYPE_F32) row_kernel<float><<<blocks, 256, 0, st>>>(p, g, beta, lognorm, scale, delta);

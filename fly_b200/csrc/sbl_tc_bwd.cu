@@ -1827,7 +1827,7 @@ cudaError_t launch_feat(const Host& h) {
       !map_w(&a.tm_lo, h.at<void>(h.ws.wlo), D, 64) || !map_rows(&a.tm_f, h.at<void>(h.ws.feat[SIDE]), C::M, rows, BH, 128))
     return cudaErrorInvalidValue;
   a.lengths = h.p.key_lengths;
-  a.beta = h.at<float>(h.ws.fwd.beta);
+  a.beta = h.g.row_stats + 2 * (int64_t)BH * h.p.T;
   a.nd = h.at<float2>(h.ws.nd);
   a.off = h.at<float>(h.ws.off[SIDE]);
   a.partial = h.at<float>(h.ws.partial);
@@ -1903,10 +1903,8 @@ cudaError_t backward(const Host& h) {
   const SblGrads& g = h.g;
   const int BH = p.B * p.H;
   cudaError_t e;
-  float* beta = h.at<float>(h.ws.fwd.beta);
-  if ((e = tc_prepare_projection(p, h.ws.fwd, h.base, h.st, true, beta, h.at<__nv_bfloat16>(h.ws.wlo))) != cudaSuccess)
+  if ((e = tc_prepare_projection(p, h.ws.fwd, h.base, h.st, true, nullptr, h.at<__nv_bfloat16>(h.ws.wlo))) != cudaSuccess)
     return e;
-  if ((e = tc_key_logscale_bound(p, h.ws.fwd, h.base, beta, h.st, true)) != cudaSuccess) return e;
   bwd_rows_kernel<D><<<dim3((unsigned)(h.ws.Tp / kRowSpan), (unsigned)div_up(p.H, kRowHeads), (unsigned)p.B), 256, 0, h.st>>>(
       static_cast<const __nv_bfloat16*>(p.out), p.o_stride_b, p.o_stride_t, p.o_stride_h,
       static_cast<const __nv_bfloat16*>(g.dout), g.do_stride_b, g.do_stride_t, g.do_stride_h, g.row_stats, p.B, p.H, p.T,
@@ -1967,7 +1965,6 @@ void tc_plan_backward(const SblParams& p, TcBwdWorkspace* ws) {
   f.wt = take((size_t)p.r * p.E * 4);
   f.phiq = take((size_t)p.r * p.E * 2);      // the projection's first bf16 term
   ws->wlo = take((size_t)p.r * p.E * 2);     // ... and its second
-  f.beta = take(BH * 4);
   ws->Tp = (int)(div_up(p.T, TR) * TR);
   ws->nd = take(BH * ws->Tp * 8);
   ws->delta = p.E == 128 ? take(BH * ws->Tp * 4) : off;

@@ -164,9 +164,9 @@ class Problem:
         return self.out
 
     def forward_train(self, workspace):
-        """Forward that also returns what `backward` needs of it: row statistics (2,B,H,T) fp32."""
+        """Forward that also returns what `backward` needs of it: two fp32 per query row and one per head."""
         B, H, T = self.shape[:3]
-        stats = torch.empty(2, B, H, T, device=self.device, dtype=torch.float32)
+        stats = torch.empty(2 * B * H * T + B * H, device=self.device, dtype=torch.float32)
         self._call(_cabi.load().sbl_forward_train, stats.data_ptr(), workspace=workspace)
         return self.out, stats
 

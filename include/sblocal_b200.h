@@ -226,11 +226,11 @@ const char* sbl_static_last_error(void);
 /* ------------------------------------------------------------------ training */
 
 /*
- * sbl_forward that also leaves what the gradients need: row_stats (2,B,H,T) fp32
- * device, [0] a log-scale and [1] a positive normaliser per query row, so that
- * row_stats[0] + ln(row_stats[1]) is the row's log_normalization
+ * sbl_forward that also leaves what the gradients need, in row_stats: 2*B*H*T +
+ * B*H fp32 on the device.  First (2,B,H,T), [0] a log-scale and [1] a positive
+ * normaliser per query row, so that [0] + ln([1]) is the row's log_normalization
  * (sblocal_attention.py:115): inside the window a key weighs
- * exp(tau q.k - log_normalization).  `out` is the same as sbl_forward's.  Rows
+ * exp(tau q.k - log_normalization); then (B,H), the key log-scale.  `out` is the same as sbl_forward's.  Rows
  * without any real key get an output of zero.  Sequence shards and
  * softmax_eps != 0: SBL_ERR_UNSUPPORTED.
  */
@@ -246,7 +246,7 @@ int sbl_forward_train(const SblParams* p, void* workspace, size_t workspace_byte
  */
 typedef struct SblGrads {
   const void* dout; int64_t do_stride_b, do_stride_t, do_stride_h;
-  const float* row_stats;     /* (2,B,H,T) from sbl_forward_train                          */
+  const float* row_stats;     /* from sbl_forward_train                                    */
   void* dq; int64_t dq_stride_b, dq_stride_t, dq_stride_h;
   void* dk; int64_t dk_stride_b, dk_stride_s, dk_stride_h;
   void* dv; int64_t dv_stride_b, dv_stride_s, dv_stride_h;
