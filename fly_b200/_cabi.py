@@ -6,6 +6,7 @@ is raised.
 """
 import ctypes
 import os
+import struct
 import threading
 
 from . import build as _build
@@ -101,6 +102,39 @@ class SblNormRotary(ctypes.Structure):
         ('side', SblNormRotarySide * 2),
         ('reserved', ctypes.c_int32 * 4),
     ]
+
+
+def _packer(cls):
+    """Fields in order -> an instance of the structure.  Native packing has C's alignment; for forty fields it takes a
+    tenth of the time that ctypes takes to convert them one by one."""
+    codes = {ctypes.c_int32: 'i', ctypes.c_int64: 'q', ctypes.c_float: 'f', ctypes.c_double: 'd', ctypes.c_void_p: 'P'}
+
+    def fields(c):
+        for _, t in c._fields_:
+            if t in codes:
+                yield codes[t]
+            elif issubclass(t, ctypes.Array) and t._type_ in codes:
+                yield codes[t._type_] * t._length_
+            elif issubclass(t, ctypes.Array):
+                yield from (code for _ in range(t._length_) for code in fields(t._type_))
+            else:
+                raise TypeError(t)
+
+    layout = struct.Struct('@' + ''.join(fields(cls)) + '0q')
+    assert layout.size == ctypes.sizeof(cls)
+
+    def pack(*values):
+        try:
+            return cls.from_buffer_copy(layout.pack(*values))
+        except (struct.error, OverflowError) as e:
+            raise ValueError(f'sblocal_b200: a size, stride or number does not fit its field of {cls.__name__}: {e}') from e
+
+    return pack
+
+
+pack_params = _packer(SblParams)
+pack_grads = _packer(SblGrads)
+pack_norm_rotary = _packer(SblNormRotary)
 
 
 class SblError(RuntimeError):

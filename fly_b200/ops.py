@@ -77,6 +77,16 @@ def _on(device):
     return torch.cuda.device(device)
 
 
+# (the current stream's handle without a Stream object around it, where this torch has the call)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+
+
+def _stream(device):
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
+    return torch.cuda.current_stream(device).cuda_stream
+
+
 class Problem:
     """One SBLocal problem: parameter block plus the tensors it borrows (kept
     alive for as long as the block is used)."""
@@ -104,7 +114,9 @@ class Problem:
         query = query if query.stride(-1) == 1 else query.contiguous()
         key = key if key.stride(-1) == 1 else key.contiguous()
         value = value if value.stride(-1) == 1 else value.contiguous()
-        W32 = W.detach().to(device=dev, dtype=torch.float32).contiguous()
+        W32 = W.detach()
+        if W32.device != dev or W32.dtype != torch.float32 or not W32.is_contiguous():
+            W32 = W32.to(device=dev, dtype=torch.float32).contiguous()
         if out is None:
             out = torch.empty(B, T, H, D, device=dev, dtype=query.dtype)
         elif out.shape != (B, T, H, D) or out.dtype != query.dtype or out.stride(-1) != 1:
@@ -115,13 +127,13 @@ class Problem:
                 raise ValueError(f'key lengths must have shape ({B},)')
         tau = float(softmax_temp) if softmax_temp else 1.0 / math.sqrt(E)
         sum_lo, sum_hi = sum_range if sum_range is not None else (0, S)
-        # (in the order of the fields: one call, where assigning them one by one costs a small call some microseconds)
-        p = _cabi.SblParams(
+        p = _cabi.pack_params(   # in the order of the fields
             _DTYPES[query.dtype], B, H, T, S, E, D, W.shape[0], int(local_context), tau, float(softmax_eps),
             query.data_ptr(), *query.stride()[:3], key.data_ptr(), *key.stride()[:3],
             value.data_ptr(), *value.stride()[:3], out.data_ptr(), *out.stride()[:3], W32.data_ptr(),
-            key_lengths.data_ptr() if key_lengths is not None else None, int(q_pos0), int(k_pos0),
-            int(S_total) if S_total is not None else S, sum_lo, sum_hi, _cabi.SBL_FLAG_GENERIC_PATH if generic else 0)
+            key_lengths.data_ptr() if key_lengths is not None else 0, int(q_pos0), int(k_pos0),
+            int(S_total) if S_total is not None else S, sum_lo, sum_hi, _cabi.SBL_FLAG_GENERIC_PATH if generic else 0,
+            0, 0, 0)
         self.params = p
         self.device = dev
         self.out = out
@@ -149,7 +161,7 @@ class Problem:
     def _call(self, fn, *extra, workspace=None):
         ws = workspace if workspace is not None else self.workspace()
         with _on(self.device):
-            stream = torch.cuda.current_stream(self.device).cuda_stream
+            stream = _stream(self.device)
             rc = fn(ctypes.byref(self.params), ws.data_ptr(), ws.numel(), *extra, stream)
         _cabi.check(rc)
         return ws
@@ -191,11 +203,11 @@ class Problem:
         dq, dk, dv = (torch.empty(x.shape, device=self.device, dtype=x.dtype) for x in (query, key, value))
         # of this call alone: a backward pass may run on another stream or be captured while another one is alive
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        g = _cabi.SblGrads(grad_out.data_ptr(), *grad_out.stride()[:3], row_stats.data_ptr(),
-                           dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3],
-                           dv.data_ptr(), *dv.stride()[:3])
+        g = _cabi.pack_grads(grad_out.data_ptr(), *grad_out.stride()[:3], row_stats.data_ptr(),
+                             dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3],
+                             dv.data_ptr(), *dv.stride()[:3], 0, 0, 0, 0)
         with _on(self.device):
-            stream = torch.cuda.current_stream(self.device).cuda_stream
+            stream = _stream(self.device)
             rc = _cabi.load().sbl_backward(ctypes.byref(self.params), ctypes.byref(g), ws.data_ptr(), nbytes, stream)
             _cabi.check(rc)
             if tensor and watch and not torch.cuda.is_current_stream_capturing():
@@ -319,19 +331,18 @@ def sblocal_attention(query, key, value, W, local_context, softmax_temp=None, so
 def _norm_rotary_params(xs, ys, weights, positions, pos0, rotary_dim, theta, interleaved, eps, dys=(None, None),
                         dws=(None, None)):
     """SblNormRotary of the tensors; those it points to must stay alive."""
-    sides = []
-    for x, y, dy, w, dw, pos in zip(xs, ys, dys, weights, dws, positions):
-        sides.append(_cabi.SblNormRotarySide(
-            x.shape[1], x.shape[2], x.data_ptr(), *x.stride()[:3], y.data_ptr(), *y.stride()[:3],
-            *((dy.data_ptr(), *dy.stride()[:3]) if dy is not None else (None, 0, 0, 0)),
-            w.data_ptr() if w is not None else None, dw.data_ptr() if dw is not None else None,
-            *((pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0, pos.stride(-1)) if pos is not None
-              else (None, 0, 0)), pos0))
     w = weights[0] if weights[0] is not None else weights[1]
     B, _, _, E = xs[0].shape
-    return _cabi.SblNormRotary(_DTYPES[xs[0].dtype], _DTYPES[w.dtype] if w is not None else _cabi.SBL_DTYPE_F32, B, E,
-                               rotary_dim, 1 if interleaved else 0, eps, theta,
-                               (_cabi.SblNormRotarySide * 2)(*sides))
+    fields = [_DTYPES[xs[0].dtype], _DTYPES[w.dtype] if w is not None else _cabi.SBL_DTYPE_F32, B, E, rotary_dim,
+              1 if interleaved else 0, eps, theta]
+    for x, y, dy, w, dw, pos in zip(xs, ys, dys, weights, dws, positions):
+        fields += [x.shape[1], x.shape[2], x.data_ptr(), *x.stride()[:3], y.data_ptr(), *y.stride()[:3]]
+        fields += [dy.data_ptr(), *dy.stride()[:3]] if dy is not None else [0, 0, 0, 0]
+        fields += [w.data_ptr() if w is not None else 0, dw.data_ptr() if dw is not None else 0]
+        fields += ([pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0, pos.stride(-1)] if pos is not None
+                   else [0, 0, 0])
+        fields.append(pos0)
+    return _cabi.pack_norm_rotary(*fields, 0, 0, 0, 0)
 
 
 def _norm_rotary_forward(xs, weights, positions, *args):
@@ -339,7 +350,7 @@ def _norm_rotary_forward(xs, weights, positions, *args):
     ys = tuple(torch.empty(x.shape, dtype=x.dtype, device=dev) for x in xs)
     p = _norm_rotary_params(xs, ys, weights, positions, *args)
     with _on(dev):
-        rc = _cabi.load().sbl_norm_rotary_forward(ctypes.byref(p), torch.cuda.current_stream(dev).cuda_stream)
+        rc = _cabi.load().sbl_norm_rotary_forward(ctypes.byref(p), _stream(dev))
     _cabi.check(rc)
     return ys
 
@@ -373,7 +384,7 @@ class _NormRotary(torch.autograd.Function):
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         with _on(dev):
             rc = lib.sbl_norm_rotary_backward(ctypes.byref(p), ws.data_ptr() if ws is not None else None, nbytes,
-                                              torch.cuda.current_stream(dev).cuda_stream)
+                                              _stream(dev))
         _cabi.check(rc)
         return (*dxs, *dws, *([None] * (2 + len(ctx.args))))
 
