@@ -146,6 +146,7 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 // cycles per group of four MMAs (256 cycles of work at N = 128), 30 with the loop in line.
 __device__ __forceinline__ void wait_inline(uint64_t* bar, uint32_t parity, int* status, int code) {
   uint32_t n = 0;
+#pragma unroll 1
   while (!mbar_try_wait(bar, parity)) {
     ++n;
     if (n >= kWaitLimit || ((n & 255u) == 255u && *reinterpret_cast<volatile int*>(status) != 0)) {
