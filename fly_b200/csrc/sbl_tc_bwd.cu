@@ -930,21 +930,20 @@ __global__ void __launch_bounds__(640, 1) bwd_grad_kernel(const __grid_constant_
         }
         if (C::FUSE) load_x();
       }
-      // column tiles run one step ahead of the features; the summary's terms behind steps 0 and 1, Wt behind step 2
-      if (t.n > 0) load_c(0);
+      // Column tiles run one step ahead of the features; the summary's terms behind steps 0 and 1, Wt behind step 2.
+      // (Each load has one place in the code: see `wait_inline` on its size.)
       int sums = whole ? 2 : 0;
       bool w = false;
-      for (int s = 0; s < t.n; ++s) {
+#pragma unroll 1
+      for (int s = -1; s < t.n || !w; ++s) {
         if (s + 1 < t.n) load_c(s + 1);
-        load_f(s);
-        if (sums < 2) load_sum(sums++);
-        if (s == 2) {
+        if (s >= 0 && s < t.n) load_f(s);
+        if (s >= 0 && sums < 2) load_sum(sums++);
+        if (!w && (s == 2 || (s >= t.n - 1 && sums == 2))) {
           load_w();
           w = true;
         }
       }
-      while (sums < 2) load_sum(sums++);
-      if (!w) load_w();
       if (!C::FUSE && pass == 0) load_x();
     }
     __syncwarp();
@@ -999,7 +998,7 @@ __global__ void __launch_bounds__(640, 1) bwd_grad_kernel(const __grid_constant_
       tc_fence_after_sync();
       if (leader) {
         if (pass == C::PASS - 1) mma_commit(bars + C::Y_FREE);
-#pragma unroll
+#pragma unroll 1
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
@@ -1055,39 +1054,41 @@ __global__ void __launch_bounds__(640, 1) bwd_grad_kernel(const __grid_constant_
         if (!dx_seen) wait_inline(bars + C::DX_FREE, (it - 1) & 1, a.status, 298);
         dx_seen = true;
       };
-      for (int s = 0; s < n; ++s) {
+#pragma unroll 1
+      for (int s = 0; s < n || sums < 2; ++s) {
         const int gg = g0 + s, slot = gg % C::NF;
-        wait_inline(bars + C::F_FULL + slot, (gg / C::NF) & 1, a.status, 294);
-        wait_inline(bars + C::G_DONE + (gg & 1), (gg >> 1) & 1, a.status, 278);
-        tc_fence_after_sync();
-        if (leader) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_ts(tb + C::T_DF, tb + C::T_P + (C::FUSE ? 0 : 32 * (gg & 1)) + 8 * k, dF + (uint64_t)(slot * 2048 + k * 128),
-                   id_df, !fresh || k > 0);
-          mma_commit(bars + C::F_FREE + slot);
-        }
-        __syncwarp();
-        fresh = false;
-        if (C::FUSE && s == 0) {
-          if (sums < 2) issue_sum();
-          dx_ready();
+        if (s < n) {
+          wait_inline(bars + C::F_FULL + slot, (gg / C::NF) & 1, a.status, 294);
+          wait_inline(bars + C::G_DONE + (gg & 1), (gg >> 1) & 1, a.status, 278);
           tc_fence_after_sync();
+          if (leader) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_ts(tb + C::T_DF, tb + C::T_P + (C::FUSE ? 0 : 32 * (gg & 1)) + 8 * k, dF + (uint64_t)(slot * 2048 + k * 128),
+                     id_df, !fresh || k > 0);
+            mma_commit(bars + C::F_FREE + slot);
+            if (!C::FUSE) mma_commit(bars + C::P_FREE + (gg & 1));
+          }
+          __syncwarp();
+          fresh = false;
         }
-        if (leader) {
-          if (C::FUSE) {
+        if (sums < 2) issue_sum();
+        if (C::FUSE && s < n) {
+          if (s == 0) {
+            dx_ready();
+            tc_fence_after_sync();
+          }
+          if (leader) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               mma_ts(tb + C::T_DX, tb + C::T_P + 32 + 8 * k, dCt + (uint64_t)((gg % C::NC) * (C::CSLOT >> 4) + k * 128),
                      id_dx | (1u << 13), s > 0 || k > 0);
             mma_commit(bars + C::C_FREE + gg % C::NC);
+            mma_commit(bars + C::P_FREE + (gg & 1));
           }
-          mma_commit(bars + C::P_FREE + (gg & 1));
+          __syncwarp();
         }
-        __syncwarp();
-        if (sums < 2 && !(C::FUSE && s == 0)) issue_sum();
       }
-      while (sums < 2) issue_sum();
       g0 += n;
       if (leader) {
         if (pass == C::PASS - 1) mma_commit(bars + C::Y_FREE);
@@ -1101,7 +1102,7 @@ __global__ void __launch_bounds__(640, 1) bwd_grad_kernel(const __grid_constant_
       tc_fence_after_sync();
       if (leader) {
         // du Wt: high x high, high x low, low x high; du's low term lies behind its high one
-#pragma unroll
+#pragma unroll 1
         for (int t = 0; t < 3; ++t)
 #pragma unroll
           for (int k = 0; k < 8; ++k)
@@ -1205,20 +1206,72 @@ __global__ void __launch_bounds__(640, 1) bwd_grad_kernel(const __grid_constant_
     };
     fetch_row();
     int gg = 0;                     // number of the unit's first step
-    float hs = 0.f;
-    bool early = false;             // the unit's first step has been packed already
-    for (int u = 0; u < n_u; ++u) {
-      const int it = u / C::PASS, pass = u % C::PASS;
-      const int tile = blockIdx.x + it * step;
-      float sum1 = 0.f;
-      if (tid < 256) sum1 = __ldg(a.sum1 + (int64_t)t.bh * C::M + 256 * pass + tid);
-      const bool none = whole && t.n == 0;
-      const bool last = pass == C::PASS - 1;
+    float hs = 0.f, hsum = 0.f;
+    // One unit more than there are: the last tile's dx.
 #pragma unroll 1
-      for (int s = early ? 1 : 0; s < t.n; ++s)
-        if (((gg + s) & 1) == grp) pack_step(s, gg + s);
-      early = false;
-      gg += t.n;
+    for (int u = 0; u <= n_u; ++u) {
+      const int it = u / C::PASS, pass = u % C::PASS;
+      const int n = u < n_u ? t.n : 0;
+      float sum1 = 0.f;
+      if (tid < 256 && u < n_u) sum1 = __ldg(a.sum1 + (int64_t)t.bh * C::M + 256 * pass + tid);
+      const bool none = whole && n == 0;
+      const bool last = pass == C::PASS - 1;
+      // This group's steps, and the previous tile's dx: behind step 0 in the group that packs it (its G and S are there
+      // as soon as U has been read), in front of the steps in the other.  One place in the code for each.
+      bool pend = pass == 0 && it > 0;
+      int s = (gg ^ grp) & 1;
+#pragma unroll 1
+      while (pend || s < n) {
+        if (s < n && (!pend || s == 0)) {
+          pack_step(s, gg + s);
+          s += 2;
+          continue;
+        }
+        pend = false;
+        const int pi = it - 1;
+        constexpr int NQ = D / 4;
+        const int c = NQ * (2 * grp + cq), buf = pi % C::XBUF;
+        uint8_t* xs = smem + C::OFF_X + buf * C::TB + (c >> 6) * 16384 + row * 128;
+        float4 e[C::FUSE ? 1 : NQ / 4];
+        if (!C::FUSE) {
+          const float4* part = reinterpret_cast<const float4*>(a.part) + ((int64_t)(blockIdx.x + pi * step) * (D / 4) + c / 4) * TR + row;
+#pragma unroll
+          for (int j = 0; j < NQ / 4; ++j) e[j] = __ldg(part + j * TR);
+        }
+        mbar_wait(bars + C::X_FULL + buf, (pi / C::XBUF) & 1, a.status, 288);
+        mbar_wait(bars + C::DX_FULL, pi & 1, a.status, 289);
+        tc_fence_after_sync();
+        uint32_t v[NQ / 16][16];
+#pragma unroll
+        for (int q = 0; q < NQ / 16; ++q) tmem_ld16(lane_base + C::T_DX + c + 16 * q, v[q]);
+        tmem_ld_wait();
+        tc_fence_before_sync();
+        warp_arrive(bars + C::DX_FREE, lane);
+#pragma unroll
+        for (int j = 0; j < NQ / 8; ++j) {
+          // eight entries: 16 bytes of the row's swizzled line, dx over x
+          uint4* at = reinterpret_cast<uint4*>(xs + ((((c & 63) >> 3) + j) ^ (row & 7)) * 16);
+          const uint4 xv = *at;
+          const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+          float z[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) z[k] = __uint_as_float(v[j >> 1][8 * (j & 1) + k]);
+          if (!C::FUSE) {
+            const float4 e0 = e[2 * j], e1 = e[2 * j + 1];
+            z[0] += e0.x; z[1] += e0.y; z[2] += e0.z; z[3] += e0.w;
+            z[4] += e1.x; z[5] += e1.y; z[6] += e1.z; z[7] += e1.w;
+          }
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] = pack_bf16(fmaf(-hsum, bf16_lo(xw[k]), z[2 * k]), fmaf(-hsum, bf16_hi(xw[k]), z[2 * k + 1]));
+          *at = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        fence_async_smem();
+        warp_arrive(bars + C::STAGED, lane);
+      }
+      if (u == n_u) break;
+      gg += n;
       if (tid < 256) {
         // (every reader of the unit before is through; head dim 64: a tile has one unit, and its dx was waited for)
         if (!C::FUSE && u >= 1) mbar_wait(bars + C::DU_DONE, (u - 1) & 1, a.status, 283);
@@ -1240,7 +1293,7 @@ __global__ void __launch_bounds__(640, 1) bwd_grad_kernel(const __grid_constant_
       warp_arrive(bars + C::U_READ, lane);
       // the next tile's row, on its way while df is waited for
       if (last && it + 1 < n_it) {
-        t = row_tile<SIDE, 64>(a.g, tile + step, whole);
+        t = row_tile<SIDE, 64>(a.g, blockIdx.x + (it + 1) * step, whole);
         fetch_row();
       }
       mbar_wait(bars + C::DF_FULL, u & 1, a.status, 287);
@@ -1307,54 +1360,7 @@ __global__ void __launch_bounds__(640, 1) bwd_grad_kernel(const __grid_constant_
       tmem_ld_wait();
       tc_fence_before_sync();
       warp_arrive(bars + C::H_READ, lane);
-      const float hsum = a.tau * ((__uint_as_float(h0) + __uint_as_float(h1)) + (__uint_as_float(h2) + __uint_as_float(h3)));
-      // the next tile's first step, before this tile's dx: G and S are there as soon as U has been read
-      if (it + 1 < n_it && t.n > 0 && (gg & 1) == grp) {
-        pack_step(0, gg);
-        early = true;
-      } else if (it + 1 < n_it && t.n > 0) {
-        early = true;               // (the other group's)
-      }
-      constexpr int NQ = D / 4;
-      const int c = NQ * (2 * grp + cq), buf = it % C::XBUF;
-      uint8_t* xs = smem + C::OFF_X + buf * C::TB + (c >> 6) * 16384 + row * 128;
-      float4 e[C::FUSE ? 1 : NQ / 4];
-      if (!C::FUSE) {
-        const float4* part = reinterpret_cast<const float4*>(a.part) + ((int64_t)tile * (D / 4) + c / 4) * TR + row;
-#pragma unroll
-        for (int j = 0; j < NQ / 4; ++j) e[j] = __ldg(part + j * TR);
-      }
-      mbar_wait(bars + C::X_FULL + buf, (it / C::XBUF) & 1, a.status, 288);
-      mbar_wait(bars + C::DX_FULL, it & 1, a.status, 289);
-      tc_fence_after_sync();
-      uint32_t v[NQ / 16][16];
-#pragma unroll
-      for (int q = 0; q < NQ / 16; ++q) tmem_ld16(lane_base + C::T_DX + c + 16 * q, v[q]);
-      tmem_ld_wait();
-      tc_fence_before_sync();
-      warp_arrive(bars + C::DX_FREE, lane);
-#pragma unroll
-      for (int j = 0; j < NQ / 8; ++j) {
-        // eight entries: 16 bytes of the row's swizzled line, dx over x
-        uint4* at = reinterpret_cast<uint4*>(xs + ((((c & 63) >> 3) + j) ^ (row & 7)) * 16);
-        const uint4 xv = *at;
-        const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
-        float z[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) z[k] = __uint_as_float(v[j >> 1][8 * (j & 1) + k]);
-        if (!C::FUSE) {
-          const float4 e0 = e[2 * j], e1 = e[2 * j + 1];
-          z[0] += e0.x; z[1] += e0.y; z[2] += e0.z; z[3] += e0.w;
-          z[4] += e1.x; z[5] += e1.y; z[6] += e1.z; z[7] += e1.w;
-        }
-        uint32_t w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          w[k] = pack_bf16(fmaf(-hsum, bf16_lo(xw[k]), z[2 * k]), fmaf(-hsum, bf16_hi(xw[k]), z[2 * k + 1]));
-        *at = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      fence_async_smem();
-      warp_arrive(bars + C::STAGED, lane);
+      hsum = a.tau * ((__uint_as_float(h0) + __uint_as_float(h1)) + (__uint_as_float(h2) + __uint_as_float(h3)));
     }
   }
   tc_fence_before_sync();
