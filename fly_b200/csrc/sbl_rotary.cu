@@ -13,12 +13,13 @@
 // bytes per pair of shared memory; with equal positions once for queries and
 // keys.  Arithmetic goes in packed fp32 pairs.
 //
-// B2 N16384 H16 E64 bf16: forward 58 us, backward 85 us, 4.6 and 4.7 TB/s (70 %
-// of a plain copy); B1 N32768 H8 E128: 70 and 91 us.  Steps that led there, at
+// B2 N16384 H16 E64 bf16: forward 55 us, backward 82 us, 4.9 TB/s both (74 % of
+// a plain copy); B1 N32768 H8 E128: 67 and 87 us.  Steps that led there, at
 // the first size: 97 / 134 us with plain loads in front of their use; 71 / 91
 // with the ring; 64 / 86 with packed arithmetic and the weights folded into the
-// angles; 58 / 85 with the angles shared by both sides.  Eight stages in the
-// ring instead of four, alone: no difference.
+// angles; 58 / 85 with the angles shared by both sides; 55 / 82 without the
+// divisions of every token.  Eight stages in the ring instead of four, alone:
+// no difference.
 //
 // Two layouts.  `vec`: a row is held by LPR lanes with 8 consecutive entries
 // each (16-byte copies of bf16, two of fp32), several rows per warp; pairs of
@@ -166,10 +167,13 @@ __global__ void __launch_bounds__(32 * kWarps, BWD ? 4 : 6) vec_kernel(const __g
   const uint32_t T_ = (uint32_t)a.side[side_lo].T, hop = gridDim.x * kWarps, first = blockIdx.x * kWarps + warp;
   const uint32_t hop_b = T_ ? hop / T_ : 0, hop_t = T_ ? hop % T_ : 0;
   struct Cursor { uint32_t b, t; int side, h, end; };
-  auto heads = [&](Cursor& c) {                         // this block's part of the side's heads
-    const int H = a.side[c.side].H, per = (H + gridDim.y - 1) / gridDim.y;
-    c.h = blockIdx.y * per;
-    c.end = min(H, c.h + per);
+  // this block's part of either side's heads
+  const int per0 = (a.side[0].H + gridDim.y - 1) / gridDim.y, per1 = (a.side[1].H + gridDim.y - 1) / gridDim.y;
+  const int lo0 = blockIdx.y * per0, lo1 = blockIdx.y * per1;
+  const int hi0 = min(a.side[0].H, lo0 + per0), hi1 = min(a.side[1].H, lo1 + per1);
+  auto heads = [&](Cursor& c) {
+    c.h = c.side ? lo1 : lo0;
+    c.end = c.side ? hi1 : hi0;
   };
   Cursor at = {T_ ? first / T_ : 0, T_ ? first % T_ : 0, side_lo, 0, 0};
   heads(at);

@@ -17,9 +17,9 @@
 //             Head dim 64: the exact part too (S beside G, dx += (p g) X'); 128: adds the window kernel's
 //
 // Measured, us: B2 H16 N16384 d64 w256 | B1 H8 N32768 d128 w512
-//   rows 30 | 26   feat, queries and keys 103 + 93 | 168 + 163   combine 2 x 3.5 | 2 x 8   window - | 182 + 190
-//   dvalue 226 | 325   grad, queries and keys 293 + 325 | 395 + 405
-// The tensor core is busy for a third of that or less; what bounds each kernel stands beside it.
+//   rows 30 | 26   feat, queries and keys 101 + 94 | 169 + 163   combine 2 x 3.5 | 2 x 8   window - | 179 + 189
+//   dvalue 215 | 307   grad, queries and keys 268 + 300 | 371 + 390
+// The tensor core is busy for 20 (feat) to 43 % (grad) of that; what bounds each kernel stands beside it.
 //
 // Numerics.  Products take bf16 operands and accumulate in fp32.  Rounded to bf16
 // (half a step, 2^-9 on average): phi and psi as operands, g, p g, p - a.  Carried
@@ -143,7 +143,9 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 // mbar_wait without the call.  A call makes the issuing warp rebuild every matrix descriptor behind it: about 130
-// cycles per group of four MMAs (256 cycles of work at N = 128), 30 with the loop in line.
+// cycles per group of four MMAs (256 cycles of work at N = 128), 30 with the loop in line.  The loop stays a loop: the
+// compiler unrolls it by four at some forty waits of a kernel, a sixth of the code, and what does not fit the
+// instruction cache is paid for in every tile (grad 293 + 325 -> 273 + 300 us, dvalue 226 -> 215).
 __device__ __forceinline__ void wait_inline(uint64_t* bar, uint32_t parity, int* status, int code) {
   uint32_t n = 0;
 #pragma unroll 1
@@ -548,7 +550,7 @@ struct WinCfg {
   static_assert(SMEM <= 232448 && COUNT <= 60, "shared memory of one CTA");
 };
 
-// Bound: the chain of a step (S and G -> p g -> dx) over two buffers, 2.4 k cycles per step with 1.1 k of products; the
+// Bound: the chain of a step (S and G -> p g -> dx) over two buffers, 2.3 k cycles per step with 1.1 k of products; the
 // 32 KB that a step brings in take 0.8 k.
 template <int SIDE, int D>
 __global__ void __launch_bounds__(576, 1) bwd_window_kernel(const __grid_constant__ WinArgs a) {
@@ -785,7 +787,7 @@ struct GradArgs {
 //
 // Bound: two chains beside the stream into shared memory.  A step's (G and S -> read -> packed -> df, dx) takes 1.4 k
 // cycles, because there is no room for a second G and S beside df; a tile's (last step -> df -> du -> dx -> stored)
-// 5 k.  With six steps 20 k cycles a tile at head dim 64 and w = 256, of which products take 8.7 k.  A step's 64
+// 5 k.  With six steps 18 to 20 k cycles a tile at head dim 64 and w = 256, of which products take 8.7 k.  A step's 64
 // columns are 32 KB of features and 16 KB of X' and Y'; with the summary and the own rows 368 KB per tile, 8.8 k
 // cycles at the 41.7 B/clk that one SM's TMA loads sustain.
 template <int D>
@@ -1399,9 +1401,9 @@ struct ValCfg {
 // S = K Q^T -> p (exponential group, in place) -> p - phi psi^T (accumulated onto p) -> bf16 (packing group, in place)
 // -> dv += (p - a) dO; then dv += phi summary.
 //
-// Bound: one lane issues and one loads, in 16-KB pieces of four or eight products: 25 pieces and 17 k cycles a tile at
-// head dim 64 and w = 256, of which the products take 5.4 k and the stream into shared memory 10.4 k.  Two issuing
-// warps with a ring and a loader of their own each take 264 us for 226, because that leaves room for one phi tile
+// Bound: one lane issues and one loads, in 16-KB pieces of four or eight products: 25 pieces and 14.5 k cycles a tile
+// at head dim 64 and w = 256, of which the products take 5.4 k and the stream into shared memory 10.4 k.  Two issuing
+// warps with a ring and a loader of their own each took 264 us for 226, because that leaves room for one phi tile
 // instead of two (head dim 128: 395 for 325); log-normalisers through shared memory instead of __ldg cost a fifth:
 // its whole bandwidth goes to products with both operands there (8 KB in 64 cycles at N = 128).
 //
