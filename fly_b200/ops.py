@@ -320,7 +320,8 @@ def sblocal_attention(query, key, value, W, local_context, softmax_temp=None, so
                       watch=False):
     """`sblocal_forward` that autograd can differentiate in query, key and value (softmax_eps = 0; the projection W
     and the lengths are constants).  Rows of a batch without any real key give an output and gradients of zero, and
-    padded keys gradients of zero.  Padded keys and values must hold finite numbers."""
+    padded keys gradients of zero.  Padded keys and values must hold finite numbers.  A step may be captured into a CUDA
+    graph, lengths included, while no eager autograd graph of the same leaves is alive (torch ends the capture)."""
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
         return _SBLocal.apply(query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths, watch)
     return sblocal_forward(query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths, watch=watch)
