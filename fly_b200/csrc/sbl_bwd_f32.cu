@@ -325,7 +325,8 @@ __global__ void __launch_bounds__(256) row_kernel(SblParams p, SblGrads g, const
   if (lane == 0) {
     const float n = g.row_stats[i] + logf(g.row_stats[rows + i]);
     lognorm[i] = n;
-    scale[i] = n - beta[bh];
+    // (a batch without keys: no features over the floor of the normaliser, whose sums could leave the fp32 range)
+    scale[i] = p.key_lengths && p.key_lengths[b] <= 0 ? INFINITY : n - beta[bh];
     delta[i] = s;
   }
 }

@@ -332,10 +332,13 @@ __global__ void __launch_bounds__(FeatCfg<D>::NTHR, 1) bwd_feat_kernel(const __g
     const int row = qd * 32 + lane;
     const uint32_t lane_base = tb + ((uint32_t)(qd * 32) << 16);
     const float beta = a.beta[bh];
+    // Padded keys have no features.  Nor have the queries of a batch without keys: over the floor of their normaliser
+    // (1e-37) they would be so large that their sums leave the fp32 range, and zero weights do not hide that.
     int len = a.rows;
-    if (SIDE == KEYS && a.lengths) {
+    if (a.lengths) {
       const int64_t l = a.lengths[b];
-      len = l < 0 ? 0 : (l < a.rows ? (int)l : a.rows);
+      if (l <= 0) len = 0;
+      else if (SIDE == KEYS && l < a.rows) len = (int)l;
     }
     const float2* nd = a.nd + (int64_t)bh * a.Tp;
     for (int i = grp; i < nt; i += C::GROUPS) {
