@@ -198,7 +198,8 @@ class Problem:
         tensor = self.status_offset is not None
         if grad_out.stride(-1) != 1 or tensor and (grad_out.data_ptr() % 16 or grad_out.stride(1) < D or any(
                 n > 1 and (st <= 0 or st % 8) for n, st in zip(grad_out.shape[:3], grad_out.stride()))):
-            grad_out = grad_out.contiguous()
+            # (fresh storage: `contiguous` keeps a dense tensor where it is, and the stride of an axis of one as it is)
+            grad_out = torch.empty((B, T, H, D), device=self.device, dtype=query.dtype).copy_(grad_out)
         nbytes = self.backward_workspace_bytes()
         dq, dk, dv = (torch.empty(x.shape, device=self.device, dtype=x.dtype) for x in (query, key, value))
         # of this call alone: a backward pass may run on another stream or be captured while another one is alive
