@@ -104,7 +104,8 @@ bool map_bthe(CUtensorMap* m, const void* base, int B, int rows, int H, int E, i
               uint32_t box_rows) {
   const uint64_t dims[4] = {(uint64_t)E, (uint64_t)rows, (uint64_t)H, (uint64_t)B};
   // a size-1 axis may carry any stride in torch; give the encoder a legal one
-  const uint64_t str[3] = {(uint64_t)ss * 2, (uint64_t)(H > 1 ? sh : E) * 2, (uint64_t)(B > 1 ? sb : E) * 2};
+  const uint64_t str[3] = {(uint64_t)(rows > 1 ? ss : E) * 2, (uint64_t)(H > 1 ? sh : E) * 2,
+                           (uint64_t)(B > 1 ? sb : E) * 2};
   const uint32_t box[4] = {64, box_rows, 1, 1};
   return cached_tmap(m, base, 4, dims, str, box);
 }

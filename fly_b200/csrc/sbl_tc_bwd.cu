@@ -1613,17 +1613,17 @@ cudaError_t backward(const Host& h) {
 }  // namespace
 
 const char* tc_backward_strides(const SblGrads& g, const SblParams& p) {
-  struct { const char* name; const void* ptr; int64_t b, r, h; } t[] = {
-      {"dout", g.dout, g.do_stride_b, g.do_stride_t, g.do_stride_h},
-      {"dq", g.dq, g.dq_stride_b, g.dq_stride_t, g.dq_stride_h},
-      {"dk", g.dk, g.dk_stride_b, g.dk_stride_s, g.dk_stride_h},
-      {"dv", g.dv, g.dv_stride_b, g.dv_stride_s, g.dv_stride_h}};
+  struct { const char* name; const void* ptr; int rows; int64_t b, r, h; } t[] = {
+      {"dout", g.dout, p.T, g.do_stride_b, g.do_stride_t, g.do_stride_h},
+      {"dq", g.dq, p.T, g.dq_stride_b, g.dq_stride_t, g.dq_stride_h},
+      {"dk", g.dk, p.S, g.dk_stride_b, g.dk_stride_s, g.dk_stride_h},
+      {"dv", g.dv, p.S, g.dv_stride_b, g.dv_stride_s, g.dv_stride_h}};
   for (const auto& x : t) {
     if (!aligned16(x.ptr)) return x.name;
     // a size-1 axis may carry any stride
-    for (int64_t s : {p.B > 1 ? x.b : 8, x.r, p.H > 1 ? x.h : 8})
+    for (int64_t s : {p.B > 1 ? x.b : 8, x.rows > 1 ? x.r : 8, p.H > 1 ? x.h : 8})
       if (s % 8 != 0 || s <= 0) return x.name;
-    if (x.r < p.E) return x.name;
+    if (x.rows > 1 && x.r < p.E) return x.name;
   }
   return nullptr;
 }

@@ -196,7 +196,7 @@ class Problem:
             raise ValueError('grad_out must be (B,T,H,D) in the input dtype on the problem device')
         # (the tensor-core kernels read it through tensor maps: no broadcast axes, 16-byte steps)
         tensor = self.status_offset is not None
-        if grad_out.stride(-1) != 1 or tensor and (grad_out.data_ptr() % 16 or grad_out.stride(1) < D or any(
+        if grad_out.stride(-1) != 1 or tensor and (grad_out.data_ptr() % 16 or T > 1 and grad_out.stride(1) < D or any(
                 n > 1 and (st <= 0 or st % 8) for n, st in zip(grad_out.shape[:3], grad_out.stride()))):
             # (fresh storage: `contiguous` keeps a dense tensor where it is, and the stride of an axis of one as it is)
             grad_out = torch.empty((B, T, H, D), device=self.device, dtype=query.dtype).copy_(grad_out)

@@ -242,7 +242,8 @@ int sbl_forward_train(const SblParams* p, void* workspace, size_t workspace_byte
  * like q, dk like k, dv like v, same dtype, last axis contiguous, element
  * strides for the others (a stride of 0 is allowed in dout only).  Where the
  * tensor-core kernels run (sbl_status_words succeeds), all four are 16-byte
- * aligned with positive strides that are multiples of 8.
+ * aligned with positive strides that are multiples of 8 (an axis of one may
+ * have any).
  */
 typedef struct SblGrads {
   const void* dout; int64_t do_stride_b, do_stride_t, do_stride_h;

@@ -42,3 +42,35 @@ def test_gradient_of_one_row(B, H, d, sbl_lib):
     for stride in (1, 4):
         odd = dout.as_strided(dout.shape, (H * d, stride, d, 1))
         same(torch.autograd.grad(ops.sblocal_attention(*xs, W, 16), xs, odd), want)
+
+
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('T,S', [(1, 70), (70, 1), (1, 1)])
+def test_single_rows_with_any_stride(T, S, d, sbl_lib):
+    """At the C entry, dout, dq, dk and dv of one row with row strides that a tensor map cannot have."""
+    import ctypes
+
+    from fly_b200 import _cabi, ops
+    B, H = 2, 3
+    q, k, v, dout, W = inputs(B, T, S, H, d, d, 2 * d, torch.bfloat16)
+    prob = ops.Problem(q, k, v, W, 16)
+    _, stats = prob.forward_train(torch.empty(prob.workspace_bytes, dtype=torch.uint8, device='cuda'))
+    want = prob.backward(dout, stats)
+    got = [torch.full_like(x, 7.0) for x in want]
+    for stride in (1, 0, d + 4, -8):
+        g = _cabi.SblGrads()
+        for name, x, axis in (('dout', dout, 't'), ('dq', got[0], 't'), ('dk', got[1], 's'), ('dv', got[2], 's')):
+            setattr(g, name, x.data_ptr())
+            pre = 'do' if name == 'dout' else name
+            sb, sr, sh = x.stride()[:3]
+            setattr(g, f'{pre}_stride_b', sb)
+            setattr(g, f'{pre}_stride_{axis}', stride if x.shape[1] == 1 else sr)
+            setattr(g, f'{pre}_stride_h', sh)
+        g.row_stats = stats.data_ptr()
+        n = prob.backward_workspace_bytes()
+        ws = torch.empty(n, dtype=torch.uint8, device='cuda')
+        _cabi.check(sbl_lib.sbl_backward(ctypes.byref(prob.params), ctypes.byref(g), ws.data_ptr(), n,
+                                         torch.cuda.current_stream().cuda_stream))
+        same(got, want)
+        for x in got:
+            x.fill_(7.0)
