@@ -8,14 +8,31 @@ Differentiable in query, key and value (softmax_eps = 0): the backward pass
 recomputes the weights from two saved floats per row.  There is no CPU path:
 CPU tensors raise.  Not built (raise NotImplementedError): causal=True (the
 reference marks it unchecked, :61), an attn_mask that masks anything (the
-reference's own assert at :106 rejects it), dropout in training mode,
-gradients with softmax_eps != 0 or through need_weights.
+reference's own assert at :106 rejects it), dropout in training mode, and, in
+the backward pass, gradients with softmax_eps != 0 or through need_weights.
 """
 import torch
 import torch.nn as nn
 
 from . import ops
 from .feature_maps_sb import SBPerformerFeatures
+
+
+class _DenseWeights(torch.autograd.Function):
+    """Output and dense weights (`need_weights`).  Part of the autograd graph, so that a backward pass through them
+    raises instead of leaving these gradients out of a sum."""
+
+    @staticmethod
+    def forward(ctx, unnormalized, *args):
+        prob = ops.Problem(*args, generic=True)
+        ws = prob.workspace()
+        out = prob.forward(workspace=ws)
+        attn = prob.attention_weights(unnormalized=unnormalized, workspace=ws)
+        return (out, *attn) if unnormalized else (out, attn)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError('sblocal_b200: gradients through need_weights are not built')
 
 
 class SBLocalAttention(nn.Module):
@@ -76,11 +93,8 @@ class SBLocalAttention(nn.Module):
         if need_weights:
             # dense (B,H,T,S) matrices, fp32 (sblocal_attention.py:124-136): the generic kernels keep phi(Q) and
             # phi(K) in the workspace for this; meant for tests and inspection, O(T*S) memory
-            prob = ops.Problem(*args, generic=True)
-            ws = prob.workspace()
-            out = prob.forward(workspace=ws)
-            attn = prob.attention_weights(unnormalized=return_attn_unnormalized, workspace=ws)
-            return out, attn
+            out, *attn = _DenseWeights.apply(return_attn_unnormalized, *args)
+            return out, tuple(attn) if return_attn_unnormalized else attn[0]
         out = ops.sblocal_attention(*args, watch=True)
         if out_dtype is not None:
             out = out.to(out_dtype)
