@@ -9,6 +9,7 @@ import math
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _cabi
 
@@ -284,6 +285,14 @@ def sblocal_forward(query, key, value, W, local_context, softmax_temp=None, soft
                    out).forward(watch=watch)
 
 
+def _refuse_tangents(*tensors):
+    """Forward-mode differentiation is not built: without this a call would drop the tangents.  (Outside a dual level,
+    where this torch says so, there are none to look for.)"""
+    if getattr(forward_ad, '_current_level', 0) >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError('sblocal_b200: forward-mode differentiation is not built')
+
+
 class _SBLocal(torch.autograd.Function):
     """Differentiable SBLocal attention: saves the inputs, the output and two floats per query row; the gradients
     recompute the weights (sbl_backward)."""
@@ -323,6 +332,7 @@ def sblocal_attention(query, key, value, W, local_context, softmax_temp=None, so
     and the lengths are constants).  Rows of a batch without any real key give an output and gradients of zero, and
     padded keys gradients of zero.  Padded keys and values must hold finite numbers.  A step may be captured into a CUDA
     graph, lengths included, while no eager autograd graph of the same leaves is alive (torch ends the capture)."""
+    _refuse_tangents(query, key, value)
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
         return _SBLocal.apply(query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths, watch)
     return sblocal_forward(query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths, watch=watch)
@@ -402,6 +412,7 @@ def qk_norm_rotary(query, key, query_weight=None, key_weight=None, positions=Non
     same over S, by default `positions` (which then has to fit both).  Without positions row t has position
     pos0 + t.  rotary_dim: even, by default all of an even E; pair i turns by position * theta^(-2i / rotary_dim); pairs are
     (i, i + rotary_dim / 2), or (2i, 2i + 1) with `interleaved`.  Returns new contiguous (query, key)."""
+    _refuse_tangents(query, key, query_weight, key_weight)
     if not (query.is_cuda and key.is_cuda):
         raise ValueError('sblocal_b200 runs on CUDA tensors only (there is no CPU path)')
     if query.dim() != 4 or key.dim() != 4 or query.shape[0] != key.shape[0] or query.shape[3] != key.shape[3]:
