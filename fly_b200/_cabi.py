@@ -29,7 +29,7 @@ EXPORTS = ('sbl_version', 'sbl_last_error', 'sbl_has_tensor_path', 'sbl_workspac
            'sbl_key_features', 'sbl_attention_weights', 'sbl_check_status', 'sbl_selftest_wait_timeout',
            'sbl_key_logscale_static', 'sbl_static_last_error', 'sbl_status_words', 'sbl_forward_train',
            'sbl_backward_workspace_bytes', 'sbl_backward', 'sbl_norm_rotary_forward',
-           'sbl_norm_rotary_workspace_bytes', 'sbl_norm_rotary_backward')
+           'sbl_norm_rotary_workspace_bytes', 'sbl_norm_rotary_backward', 'sbl_collect_status')
 
 
 class SblParams(ctypes.Structure):
@@ -195,6 +195,8 @@ def load():
         lib.sbl_check_status.argtypes = [P, vp, sz, vp]
         lib.sbl_status_words.restype = ctypes.c_int
         lib.sbl_status_words.argtypes = [P, ctypes.POINTER(sz)]
+        lib.sbl_collect_status.restype = ctypes.c_int
+        lib.sbl_collect_status.argtypes = [vp, vp, vp]
         lib.sbl_selftest_wait_timeout.restype = ctypes.c_int
         lib.sbl_selftest_wait_timeout.argtypes = [vp, sz, vp]
         lib.sbl_key_logscale_static.restype = ctypes.c_int

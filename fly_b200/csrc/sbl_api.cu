@@ -420,6 +420,14 @@ int sbl_status_words(const SblParams* p, size_t* offset) {
   return SBL_OK;
 }
 
+int sbl_collect_status(const int32_t* words, int32_t* host, void* cuda_stream) {
+  if (!words || !host) return fail(SBL_ERR_INVALID_ARGUMENT, "words and host must be non-null");
+  if (((reinterpret_cast<uintptr_t>(words) | reinterpret_cast<uintptr_t>(host)) & 3) != 0)
+    return fail(SBL_ERR_INVALID_ARGUMENT, "words and host must be 4-byte aligned");
+  cudaError_t e = tc_collect_status(words, host, static_cast<cudaStream_t>(cuda_stream));
+  return e == cudaSuccess ? SBL_OK : cuda_fail(e, "collect status");
+}
+
 int sbl_selftest_wait_timeout(void* workspace, size_t workspace_bytes, void* cuda_stream) {
   if (!workspace || workspace_bytes < 256) return fail(SBL_ERR_INVALID_ARGUMENT, "self-test needs a 256-byte workspace");
   if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0)

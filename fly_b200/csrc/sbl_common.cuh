@@ -118,6 +118,8 @@ const char* tc_backward_strides(const SblGrads& g, const SblParams& p);
 cudaError_t tc_backward(const SblParams& p, const SblGrads& g, const TcBwdWorkspace& ws, char* base, cudaStream_t st);
 // runs a kernel whose only wait can never be satisfied; *host_status receives the recorded wait site (99)
 cudaError_t tc_wait_selftest(int* device_status, int* host_status, cudaStream_t st);
+// queues the collection of three status words into page-locked host memory
+cudaError_t tc_collect_status(const int32_t* words, int32_t* host, cudaStream_t st);
 // copies the three device status words (host_status[0]: wait site that ran out, host_status[1]: 1 if an
 // exponential left the fp32 range, host_status[2]: 1 if a row's low-rank estimate swamped its exact part) and
 // synchronises the stream

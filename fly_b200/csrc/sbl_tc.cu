@@ -1637,6 +1637,16 @@ cudaError_t tc_wait_selftest(int* device_status, int* host_status, cudaStream_t 
   return cudaStreamSynchronize(st);
 }
 
+__global__ void tc_collect_status_kernel(const int32_t* words, volatile int32_t* host) {
+  const int32_t v = threadIdx.x < 3 ? words[threadIdx.x] : 0;
+  if (v != 0) host[threadIdx.x] = v;
+}
+
+cudaError_t tc_collect_status(const int32_t* words, int32_t* host, cudaStream_t st) {
+  tc_collect_status_kernel<<<1, 32, 0, st>>>(words, host);
+  return cudaGetLastError();
+}
+
 cudaError_t tc_read_status(const Workspace& ws, char* base, int* host_status, cudaStream_t st) {
   cudaError_t e = cudaMemcpyAsync(host_status, base + ws.status, 3 * sizeof(int), cudaMemcpyDeviceToHost, st);
   if (e != cudaSuccess) return e;

@@ -2,7 +2,6 @@
 launches on the current CUDA stream.  PyTorch is used only for device memory
 and streams; all arithmetic happens in libsblocal_b200.so.
 """
-import collections
 import contextlib
 import ctypes
 import math
@@ -19,52 +18,62 @@ _workspaces = {}
 
 
 class _StatusWatch:
-    """Device status words of earlier forwards, looked at without ever blocking the host.
+    """Device status words of earlier calls, forward and backward, looked at without ever blocking the host.
 
     The tensor-core kernels leave three int32 words in the workspace (a bounded wait that ran out; an exponential
-    that left the fp32 range; a row whose low-rank estimate swamped its exact part).  `post` queues an asynchronous copy of them into pinned host memory behind a
-    forward; `poll` inspects the copies that have already landed and raises for the first bad one.  A module
-    calls `poll` at the start of every forward, so a bad result is reported by the next call at the latest
-    (or by `Problem.check_status`, which synchronises)."""
+    that left the fp32 range; a row whose low-rank estimate swamped its exact part).  `post` queues a kernel behind a
+    call that brings words other than zero into page-locked host memory, in a captured call with every replay; `poll`
+    looks there and raises.  The module and `sblocal_attention` call `poll` at the start of every forward, so a bad
+    result is reported by the next call at the latest.  `poll(wait=True)` waits for the devices first: for the end of
+    a program, and for graphs, whose replays call nothing that could look."""
 
     def __init__(self):
         self._lock = threading.Lock()
-        self._pending = collections.deque()
-        self._free = []
+        self._words = None             # three int32, page-locked
+        self._devices = set()          # that have written there
 
-    def post(self, workspace, offset, device):
-        with self._lock:
-            host = self._free.pop() if self._free else torch.empty(3, dtype=torch.int32).pin_memory()
-        words = workspace[offset:offset + 12].view(torch.int32)
-        host.copy_(words, non_blocking=True)
-        event = torch.cuda.Event()
-        event.record(torch.cuda.current_stream(device))
-        with self._lock:
-            self._pending.append((event, host))
-
-    def poll(self):
-        while True:
+    def post(self, words, device):
+        """words: address of the three status words that the current stream's work writes."""
+        if self._words is None:
+            if torch.cuda.is_current_stream_capturing():
+                return                 # (page-locked memory cannot be had in a capture that no call came before)
             with self._lock:
-                if not self._pending or not self._pending[0][0].query():
-                    return
-                _, host = self._pending.popleft()
-                wait_site, out_of_range, imprecise = host.tolist()
-                self._free.append(host)
-            if wait_site:
-                raise _cabi.SblError(_cabi.SBL_ERR_DEVICE_STATUS,
-                                     f'an earlier forward gave up on a bounded wait inside a kernel (wait site '
-                                     f'{wait_site}); its output is invalid')
-            if out_of_range:
-                raise _cabi.SblError(_cabi.SBL_ERR_DEVICE_STATUS,
-                                     'an earlier forward met logits beyond the range of the bf16 tensor-core kernels '
-                                     '(an exponential left the fp32 range); its output is invalid -- use fp32 inputs '
-                                     'or Problem(..., generic=True)')
-            if imprecise:
-                raise _cabi.SblError(_cabi.SBL_ERR_DEVICE_STATUS,
-                                     'an earlier forward met query rows whose in-window low-rank estimate is more than '
-                                     '16 times their exact softmax mass (logits 3-4 times the unit scale): the bf16 '
-                                     'tensor-core kernels lose accuracy there -- use fp32 inputs or '
-                                     'Problem(..., generic=True)')
+                if self._words is None:
+                    self._memory = torch.zeros(3, dtype=torch.int32).pin_memory()
+                    self._words = (ctypes.c_int32 * 3).from_address(self._memory.data_ptr())
+        self._devices.add(device.index)
+        _cabi.check(_cabi.load().sbl_collect_status(words, ctypes.addressof(self._words), _stream(device)))
+
+    def poll(self, wait=False):
+        if self._words is None:
+            return
+        if wait:
+            for index in tuple(self._devices):
+                torch.cuda.synchronize(index)
+        if any(self._words):
+            with self._lock:
+                words = list(self._words)
+                self._words[:] = [0, 0, 0]
+            self._report(words)
+
+    @staticmethod
+    def _report(words):
+        wait_site, out_of_range, imprecise = words
+        if wait_site:
+            raise _cabi.SblError(_cabi.SBL_ERR_DEVICE_STATUS,
+                                 f'an earlier call gave up on a bounded wait inside a kernel (wait site '
+                                 f'{wait_site}); its results are invalid')
+        if out_of_range:
+            raise _cabi.SblError(_cabi.SBL_ERR_DEVICE_STATUS,
+                                 'an earlier forward met logits beyond the range of the bf16 tensor-core kernels '
+                                 '(an exponential left the fp32 range); its output is invalid -- use fp32 inputs '
+                                 'or Problem(..., generic=True)')
+        if imprecise:
+            raise _cabi.SblError(_cabi.SBL_ERR_DEVICE_STATUS,
+                                 'an earlier forward met query rows whose in-window low-rank estimate is more than '
+                                 '16 times their exact softmax mass (logits 3-4 times the unit scale): the bf16 '
+                                 'tensor-core kernels lose accuracy there -- use fp32 inputs or '
+                                 'Problem(..., generic=True)')
 
 
 status_watch = _StatusWatch()
@@ -169,11 +178,11 @@ class Problem:
 
     # -- entry points -----------------------------------------------------
     def forward(self, workspace=None, watch=False):
-        """watch: queue a non-blocking copy of the kernels' status words (see `status_watch`)."""
+        """watch: queue the collection of the kernels' status words (see `status_watch`)."""
         ws = self._call(_cabi.load().sbl_forward, workspace=workspace)
         if watch and self.status_offset is not None:
             with _on(self.device):
-                status_watch.post(ws, self.status_offset, self.device)
+                status_watch.post(ws.data_ptr() + self.status_offset, self.device)
         return self.out
 
     def forward_train(self, workspace):
@@ -212,8 +221,8 @@ class Problem:
             stream = _stream(self.device)
             rc = _cabi.load().sbl_backward(ctypes.byref(self.params), ctypes.byref(g), ws.data_ptr(), nbytes, stream)
             _cabi.check(rc)
-            if tensor and watch and not torch.cuda.is_current_stream_capturing():
-                status_watch.post(ws, 0, self.device)
+            if tensor and watch:
+                status_watch.post(ws.data_ptr(), self.device)
         return dq, dk, dv
 
     def check_status(self, workspace=None):
@@ -308,9 +317,9 @@ class _SBLocal(torch.autograd.Function):
         # a workspace of this call alone, for the reason given in Problem.backward
         ws = torch.empty(prob.workspace_bytes, dtype=torch.uint8, device=prob.device)
         out, stats = prob.forward_train(ws)
-        if watch and prob.status_offset is not None and not torch.cuda.is_current_stream_capturing():
+        if watch and prob.status_offset is not None:
             with _on(prob.device):
-                status_watch.post(ws, prob.status_offset, prob.device)
+                status_watch.post(ws.data_ptr() + prob.status_offset, prob.device)
         ctx.stats = True
         ctx.save_for_backward(query, key, value, W, key_lengths, out, stats)
         return out
@@ -327,11 +336,15 @@ class _SBLocal(torch.autograd.Function):
 
 
 def sblocal_attention(query, key, value, W, local_context, softmax_temp=None, softmax_eps=0.0, key_lengths=None,
-                      watch=False):
+                      watch=True):
     """`sblocal_forward` that autograd can differentiate in query, key and value (softmax_eps = 0; the projection W
     and the lengths are constants).  Rows of a batch without any real key give an output and gradients of zero, and
     padded keys gradients of zero.  Padded keys and values must hold finite numbers.  A step may be captured into a CUDA
-    graph, lengths included, while no eager autograd graph of the same leaves is alive (torch ends the capture)."""
+    graph, lengths included, while no eager autograd graph of the same leaves is alive (torch ends the capture).
+    watch: report what the kernels of this call, or of its gradients, found wrong to a later call (`status_watch`); a
+    replayed step's reports are read by `status_watch.poll(wait=True)`."""
+    if watch:
+        status_watch.poll()
     _refuse_tangents(query, key, value)
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
         return _SBLocal.apply(query, key, value, W, local_context, softmax_temp, softmax_eps, key_lengths, watch)

@@ -168,13 +168,22 @@ int sbl_check_status(const SblParams* p, void* workspace, size_t workspace_bytes
  * kernels write (word 0: site of a bounded wait that ran out, word 1: 1 if an
  * exponential left the fp32 range because the logits are far above unit
  * scale, word 2: 1 if a row's low-rank estimate swamped its exact part, see
- * sbl_check_status; all 0 = fine).  A caller may copy them out asynchronously behind a
+ * sbl_check_status; all 0 = fine).  A caller may collect them behind a
  * forward and look at them later; sbl_check_status reads the same words with
  * a synchronisation.  Returns SBL_ERR_UNSUPPORTED for problems that run the
  * generic kernels (they keep no status words).  No counterpart in the
  * reference.
  */
 int sbl_status_words(const SblParams* p, size_t* offset);
+
+/*
+ * Queues, behind the work of the stream, the collection of three status words
+ * (device) into `host` (three int32 in page-locked host memory that the device
+ * can write): words that are not 0 overwrite those there, zeros leave them.  So
+ * one place serves many calls, replays of captured ones too; its owner looks at
+ * it when it likes and clears what it has seen.  No counterpart in the reference.
+ */
+int sbl_collect_status(const int32_t* words, int32_t* host, void* cuda_stream);
 
 /*
  * Self-test of that mechanism: launches one warp that waits on a barrier
