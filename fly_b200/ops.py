@@ -105,6 +105,8 @@ class Problem:
                  key_lengths=None, out=None, q_pos0=0, k_pos0=0, S_total=None, sum_range=None, generic=False):
         if not (query.is_cuda and key.is_cuda and value.is_cuda):
             raise ValueError('sblocal_b200 runs on CUDA tensors only (there is no CPU path)')
+        if key.device != query.device or value.device != query.device:
+            raise ValueError('query, key and value must be on one device')
         if query.dim() != 4 or key.dim() != 4 or value.dim() != 4:
             raise ValueError('query/key/value must be (B,T,H,E), (B,S,H,E), (B,S,H,D)')
         if query.dtype not in _DTYPES:
@@ -129,8 +131,9 @@ class Problem:
             W32 = W32.to(device=dev, dtype=torch.float32).contiguous()
         if out is None:
             out = torch.empty(B, T, H, D, device=dev, dtype=query.dtype)
-        elif out.shape != (B, T, H, D) or out.dtype != query.dtype or out.stride(-1) != 1:
-            raise ValueError('out must be (B,T,H,D) in the input dtype with a contiguous last axis')
+        elif (out.shape != (B, T, H, D) or out.dtype != query.dtype or out.stride(-1) != 1 or out.device != dev):
+            raise ValueError('out must be (B,T,H,D) in the input dtype with a contiguous last axis, on the device of the '
+                             'inputs')
         if key_lengths is not None:
             key_lengths = key_lengths.to(device=dev, dtype=torch.int64).contiguous()
             if key_lengths.shape != (B,):
@@ -170,6 +173,8 @@ class Problem:
 
     def _call(self, fn, *extra, workspace=None):
         ws = workspace if workspace is not None else self.workspace()
+        if ws.device != self.device or not ws.is_contiguous():
+            raise ValueError('the workspace must be a contiguous tensor on the problem device')
         with _on(self.device):
             stream = _stream(self.device)
             rc = fn(ctypes.byref(self.params), ws.data_ptr(), ws.numel(), *extra, stream)
@@ -204,6 +209,9 @@ class Problem:
         B, H, T, S, E, D = self.shape
         if grad_out.shape != (B, T, H, D) or grad_out.dtype != query.dtype or grad_out.device != self.device:
             raise ValueError('grad_out must be (B,T,H,D) in the input dtype on the problem device')
+        if (row_stats.shape != (2 * B * H * T + B * H,) or row_stats.dtype != torch.float32
+                or row_stats.device != self.device or not row_stats.is_contiguous()):
+            raise ValueError('row_stats must be what forward_train of this problem returned')
         # (the tensor-core kernels read it through tensor maps: no broadcast axes, 16-byte steps)
         tensor = self.status_offset is not None
         if grad_out.stride(-1) != 1 or tensor and (grad_out.data_ptr() % 16 or T > 1 and grad_out.stride(1) < D or any(
