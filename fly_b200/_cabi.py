@@ -14,6 +14,7 @@ from . import build as _build
 SBL_DTYPE_F32 = 0
 SBL_DTYPE_BF16 = 1
 SBL_FLAG_GENERIC_PATH = 1
+SBL_SKIP = (1, 2, 4)   # SBL_SKIP_DQ, SBL_SKIP_DK, SBL_SKIP_DV
 
 SBL_OK = 0
 SBL_ERR_INVALID_ARGUMENT = -1
@@ -72,7 +73,8 @@ class SblGrads(ctypes.Structure):
         ('dk_stride_h', ctypes.c_int64),
         ('dv', ctypes.c_void_p), ('dv_stride_b', ctypes.c_int64), ('dv_stride_s', ctypes.c_int64),
         ('dv_stride_h', ctypes.c_int64),
-        ('reserved', ctypes.c_int32 * 4),
+        ('skip', ctypes.c_int32),
+        ('reserved', ctypes.c_int32 * 3),
     ]
 
 

@@ -310,10 +310,13 @@ int sbl_backward(const SblParams* p, const SblGrads* g, void* workspace, size_t 
   int rc = validate_training(p);
   if (rc != SBL_OK) return rc;
   if (!g) return fail(SBL_ERR_INVALID_ARGUMENT, "grads is null");
-  if (!g->dout || !g->row_stats || !g->dq || !g->dk || !g->dv)
-    return fail(SBL_ERR_INVALID_ARGUMENT, "dout, row_stats, dq, dk and dv must be non-null device pointers");
+  const int all = SBL_SKIP_DQ | SBL_SKIP_DK | SBL_SKIP_DV;
+  if (g->skip & ~all) return fail(SBL_ERR_INVALID_ARGUMENT, "unknown skip bits 0x%x", g->skip);
   for (int r : g->reserved)
     if (r != 0) return fail(SBL_ERR_INVALID_ARGUMENT, "reserved fields must be 0");
+  if (!g->dout || !g->row_stats || (!g->dq && !(g->skip & SBL_SKIP_DQ)) || (!g->dk && !(g->skip & SBL_SKIP_DK)) ||
+      (!g->dv && !(g->skip & SBL_SKIP_DV)))
+    return fail(SBL_ERR_INVALID_ARGUMENT, "dout, row_stats, and dq, dk and dv unless skipped, must be non-null device pointers");
   cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
   if (tensor_path(*p)) {
     if (const char* name = tc_backward_strides(*g, *p))

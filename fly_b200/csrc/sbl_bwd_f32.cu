@@ -666,14 +666,18 @@ template <typename T>
 cudaError_t grads(const SblParams& p, const SblGrads& g, GradArgs a, const BwdWorkspace& ws, char* base, cudaStream_t st) {
   const unsigned bh = (unsigned)(p.B * p.H);
   cudaError_t e;
-  if ((e = summary<T, KEYS>(p, a, ws, base, st)) != cudaSuccess) return e;
-  if ((e = summary<T, QUERIES>(p, a, ws, base, st)) != cudaSuccess) return e;
-  a.dx = g.dv; a.dxb = g.dv_stride_b; a.dxr = g.dv_stride_s; a.dxh = g.dv_stride_h;
-  const dim3 grid((unsigned)div_up(p.S, 64), 1, bh);
-  e = p.D <= 64 ? run(dv_kernel<T, 1>, grid, 192 * LK, a, st) : run(dv_kernel<T, 2>, grid, 128 * LK + 64 * LW, a, st);
-  if (e != cudaSuccess) return e;
+  const bool dq = !(g.skip & SBL_SKIP_DQ), dk = !(g.skip & SBL_SKIP_DK), dv = !(g.skip & SBL_SKIP_DV);
+  if (dq && (e = summary<T, KEYS>(p, a, ws, base, st)) != cudaSuccess) return e;
+  if ((dk || dv) && (e = summary<T, QUERIES>(p, a, ws, base, st)) != cudaSuccess) return e;
+  if (dv) {
+    a.dx = g.dv; a.dxb = g.dv_stride_b; a.dxr = g.dv_stride_s; a.dxh = g.dv_stride_h;
+    const dim3 grid((unsigned)div_up(p.S, 64), 1, bh);
+    e = p.D <= 64 ? run(dv_kernel<T, 1>, grid, 192 * LK, a, st) : run(dv_kernel<T, 2>, grid, 128 * LK + 64 * LW, a, st);
+    if (e != cudaSuccess) return e;
+  }
   a.dx = g.dq; a.dxb = g.dq_stride_b; a.dxr = g.dq_stride_t; a.dxh = g.dq_stride_h;
-  if ((e = side_grads<T, QUERIES>(p, a, st)) != cudaSuccess) return e;
+  if (dq && (e = side_grads<T, QUERIES>(p, a, st)) != cudaSuccess) return e;
+  if (!dk) return cudaSuccess;
   a.dx = g.dk; a.dxb = g.dk_stride_b; a.dxr = g.dk_stride_s; a.dxh = g.dk_stride_h;
   return side_grads<T, KEYS>(p, a, st);
 }

@@ -1575,21 +1575,12 @@ cudaError_t launch_side(const Host& h, void* dx, int64_t ob, int64_t orow, int64
 }
 
 template <int D>
-cudaError_t backward(const Host& h) {
+cudaError_t launch_value(const Host& h) {
   using C = ValCfg<D>;
   const SblParams& p = h.p;
   const SblGrads& g = h.g;
   const int BH = p.B * p.H;
   cudaError_t e;
-  if ((e = tc_prepare_projection(p, h.ws.fwd, h.base, h.st, true, nullptr, h.at<__nv_bfloat16>(h.ws.wlo))) != cudaSuccess)
-    return e;
-  bwd_rows_kernel<D><<<dim3((unsigned)(h.ws.Tp / kRowSpan), (unsigned)div_up(p.H, kRowHeads), (unsigned)p.B), 256, 0, h.st>>>(
-      static_cast<const __nv_bfloat16*>(p.out), p.o_stride_b, p.o_stride_t, p.o_stride_h,
-      static_cast<const __nv_bfloat16*>(g.dout), g.do_stride_b, g.do_stride_t, g.do_stride_h, g.row_stats, p.B, p.H, p.T,
-      h.ws.Tp, h.at<float2>(h.ws.nd), h.at<float>(h.ws.delta));
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  if ((e = launch_feat<KEYS, D>(h)) != cudaSuccess) return e;
-  if ((e = launch_feat<QUERIES, D>(h)) != cudaSuccess) return e;
   ValArgs a{};
   if (!h.map_x(&a.tm_k, KEYS, 128) || !h.map_x(&a.tm_q, QUERIES, 128) || !h.map_y(&a.tm_do, QUERIES, 128) ||
       !map_rows(&a.tm_phi, h.at<void>(h.ws.feat[KEYS]), C::M, p.S, BH, 128) ||
@@ -1605,20 +1596,41 @@ cudaError_t backward(const Host& h) {
   a.tau = p.softmax_temp;
   if ((e = allow_smem(bwd_value_kernel<D>, C::SMEM, &h.dev->attr_bwd[D == 128][3][0])) != cudaSuccess) return e;
   bwd_value_kernel<D><<<(unsigned)(a.g.ntiles < h.dev->sms ? a.g.ntiles : h.dev->sms), C::NTHR, C::SMEM, h.st>>>(a);
+  return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t backward(const Host& h) {
+  const SblParams& p = h.p;
+  const SblGrads& g = h.g;
+  cudaError_t e;
+  if ((e = tc_prepare_projection(p, h.ws.fwd, h.base, h.st, true, nullptr, h.at<__nv_bfloat16>(h.ws.wlo))) != cudaSuccess)
+    return e;
+  bwd_rows_kernel<D><<<dim3((unsigned)(h.ws.Tp / kRowSpan), (unsigned)div_up(p.H, kRowHeads), (unsigned)p.B), 256, 0, h.st>>>(
+      static_cast<const __nv_bfloat16*>(p.out), p.o_stride_b, p.o_stride_t, p.o_stride_h,
+      static_cast<const __nv_bfloat16*>(g.dout), g.do_stride_b, g.do_stride_t, g.do_stride_h, g.row_stats, p.B, p.H, p.T,
+      h.ws.Tp, h.at<float2>(h.ws.nd), h.at<float>(h.ws.delta));
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  if ((e = launch_side<QUERIES, D>(h, g.dq, g.dq_stride_b, g.dq_stride_t, g.dq_stride_h)) != cudaSuccess) return e;
+  if ((e = launch_feat<KEYS, D>(h)) != cudaSuccess) return e;
+  if ((e = launch_feat<QUERIES, D>(h)) != cudaSuccess) return e;
+  if (!(g.skip & SBL_SKIP_DV) && (e = launch_value<D>(h)) != cudaSuccess) return e;
+  if (!(g.skip & SBL_SKIP_DQ) &&
+      (e = launch_side<QUERIES, D>(h, g.dq, g.dq_stride_b, g.dq_stride_t, g.dq_stride_h)) != cudaSuccess)
+    return e;
+  if (g.skip & SBL_SKIP_DK) return cudaSuccess;
   return launch_side<KEYS, D>(h, g.dk, g.dk_stride_b, g.dk_stride_s, g.dk_stride_h);
 }
 
 }  // namespace
 
 const char* tc_backward_strides(const SblGrads& g, const SblParams& p) {
-  struct { const char* name; const void* ptr; int rows; int64_t b, r, h; } t[] = {
-      {"dout", g.dout, p.T, g.do_stride_b, g.do_stride_t, g.do_stride_h},
-      {"dq", g.dq, p.T, g.dq_stride_b, g.dq_stride_t, g.dq_stride_h},
-      {"dk", g.dk, p.S, g.dk_stride_b, g.dk_stride_s, g.dk_stride_h},
-      {"dv", g.dv, p.S, g.dv_stride_b, g.dv_stride_s, g.dv_stride_h}};
+  struct { const char* name; const void* ptr; int skip, rows; int64_t b, r, h; } t[] = {
+      {"dout", g.dout, 0, p.T, g.do_stride_b, g.do_stride_t, g.do_stride_h},
+      {"dq", g.dq, SBL_SKIP_DQ, p.T, g.dq_stride_b, g.dq_stride_t, g.dq_stride_h},
+      {"dk", g.dk, SBL_SKIP_DK, p.S, g.dk_stride_b, g.dk_stride_s, g.dk_stride_h},
+      {"dv", g.dv, SBL_SKIP_DV, p.S, g.dv_stride_b, g.dv_stride_s, g.dv_stride_h}};
   for (const auto& x : t) {
+    if (g.skip & x.skip) continue;
     if (!aligned16(x.ptr)) return x.name;
     // a size-1 axis may carry any stride
     for (int64_t s : {p.B > 1 ? x.b : 8, x.rows > 1 ? x.r : 8, p.H > 1 ? x.h : 8})

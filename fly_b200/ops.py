@@ -202,9 +202,9 @@ class Problem:
         _cabi.check(_cabi.load().sbl_backward_workspace_bytes(ctypes.byref(self.params), ctypes.byref(n)))
         return n.value
 
-    def backward(self, grad_out, row_stats, watch=False):
+    def backward(self, grad_out, row_stats, watch=False, needs=(True, True, True)):
         """(dq, dk, dv) of sum(grad_out * out); the problem's `out` must hold the output of `forward_train`.
-        watch: as in `forward`."""
+        watch: as in `forward`.  needs: which of the three to form, None in the place of the others."""
         query, key, value = self._keep[:3]
         B, H, T, S, E, D = self.shape
         if grad_out.shape != (B, T, H, D) or grad_out.dtype != query.dtype or grad_out.device != self.device:
@@ -219,19 +219,20 @@ class Problem:
             # (fresh storage: `contiguous` keeps a dense tensor where it is, and the stride of an axis of one as it is)
             grad_out = torch.empty((B, T, H, D), device=self.device, dtype=query.dtype).copy_(grad_out)
         nbytes = self.backward_workspace_bytes()
-        dq, dk, dv = (torch.empty(x.shape, device=self.device, dtype=x.dtype) for x in (query, key, value))
+        grads = [torch.empty(x.shape, device=self.device, dtype=x.dtype) if need else None
+                 for x, need in zip((query, key, value), needs)]
         # of this call alone: a backward pass may run on another stream or be captured while another one is alive
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        g = _cabi.pack_grads(grad_out.data_ptr(), *grad_out.stride()[:3], row_stats.data_ptr(),
-                             dq.data_ptr(), *dq.stride()[:3], dk.data_ptr(), *dk.stride()[:3],
-                             dv.data_ptr(), *dv.stride()[:3], 0, 0, 0, 0)
+        places = [n for x in grads for n in ((x.data_ptr(), *x.stride()[:3]) if x is not None else (0, 0, 0, 0))]
+        skip = sum(bit for bit, need in zip(_cabi.SBL_SKIP, needs) if not need)
+        g = _cabi.pack_grads(grad_out.data_ptr(), *grad_out.stride()[:3], row_stats.data_ptr(), *places, skip, 0, 0, 0)
         with _on(self.device):
             stream = _stream(self.device)
             rc = _cabi.load().sbl_backward(ctypes.byref(self.params), ctypes.byref(g), ws.data_ptr(), nbytes, stream)
             _cabi.check(rc)
             if tensor and watch:
                 status_watch.post(ws.data_ptr(), self.device)
-        return dq, dk, dv
+        return tuple(grads)
 
     def check_status(self, workspace=None):
         """Synchronises the stream; raises if a kernel gave up on a bounded wait."""
@@ -339,8 +340,8 @@ class _SBLocal(torch.autograd.Function):
             raise NotImplementedError('sblocal_b200: gradients are built for softmax_eps = 0 only')
         query, key, value, W, key_lengths, out, stats = ctx.saved_tensors
         prob = Problem(query, key, value, W, *ctx.args, key_lengths, out=out)
-        dq, dk, dv = prob.backward(grad_out, stats, watch=ctx.watch)
-        return dq, dk, dv, None, None, None, None, None, None
+        grads = prob.backward(grad_out, stats, watch=ctx.watch, needs=ctx.needs_input_grad[:3])
+        return *grads, None, None, None, None, None, None
 
 
 def sblocal_attention(query, key, value, W, local_context, softmax_temp=None, softmax_eps=0.0, key_lengths=None,

@@ -260,8 +260,13 @@ typedef struct SblGrads {
   void* dq; int64_t dq_stride_b, dq_stride_t, dq_stride_h;
   void* dk; int64_t dk_stride_b, dk_stride_s, dk_stride_h;
   void* dv; int64_t dv_stride_b, dv_stride_s, dv_stride_h;
-  int32_t reserved[4];        /* must be 0                                                 */
+  int32_t skip;               /* SBL_SKIP_* bits: gradients nobody needs (their pointers may be null) */
+  int32_t reserved[3];        /* must be 0                                                 */
 } SblGrads;
+
+#define SBL_SKIP_DQ 1
+#define SBL_SKIP_DK 2
+#define SBL_SKIP_DV 4
 
 /*
  * Bytes of workspace sbl_backward needs (256-byte aligned base); nothing of a forward's workspace is reused.  The
