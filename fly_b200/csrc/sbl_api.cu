@@ -103,7 +103,7 @@ int validate_norm_rotary(const SblNormRotary* p, bool backward) {
     if (r != 0) return fail(SBL_ERR_INVALID_ARGUMENT, "reserved fields must be 0");
   for (const SblNormRotarySide& s : p->side) {
     if (s.T < 0 || s.H <= 0) return fail(SBL_ERR_INVALID_ARGUMENT, "T must be >= 0 and H positive (got %d, %d)", s.T, s.H);
-    if (s.T == 0 || p->B == 0) continue;
+    if (s.T == 0 || p->B == 0 || (backward && !s.y && !s.dweight)) continue;
     if (!s.x || !s.y) return fail(SBL_ERR_INVALID_ARGUMENT, "x and y must be non-null device pointers");
     if (backward && !s.dy) return fail(SBL_ERR_INVALID_ARGUMENT, "dy must be a non-null device pointer");
   }

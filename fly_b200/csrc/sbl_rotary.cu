@@ -44,6 +44,7 @@ struct RotaryArgs {
   SblNormRotarySide side[2];
   int B, E, rotary, wbf16;
   int joint;                                            // vec: both sides in one warp
+  int side0;                                            // otherwise the side of blockIdx.z = 0
   float eps;
   float* partial;                                       // backward: (2, blocks, E), null = no weight gradients
   double rate[kMaxPairs];                               // turns per position of pair i
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(32 * kWarps, BWD ? 4 : 6) vec_kernel(const __g
   const int sub = lane % LPR, grp = lane / LPR;
   const int e0 = 8 * sub, E = a.E, half = a.rotary / 2;
   const bool held = e0 < E;
-  const int side_lo = a.joint ? 0 : blockIdx.z, side_hi = a.joint ? 2 : blockIdx.z + 1;
+  const int side_lo = a.joint ? 0 : a.side0 + blockIdx.z, side_hi = a.joint ? 2 : side_lo + 1;
   for (int i = threadIdx.x; i < half; i += 32 * kWarps) s_rate[i] = a.rate[i];
   for (int i = threadIdx.x; i < 2 * EP; i += 32 * kWarps)
     s_w[i / EP][i % EP] = i % EP < E ? weight_at(a.side[i / EP].weight, a.wbf16, i % EP) : 0.f;
@@ -377,7 +378,8 @@ __device__ __forceinline__ void st1(__nv_bfloat16* p, float v) { *p = __float2bf
 template <typename T, int NJ, bool BWD>
 __global__ void __launch_bounds__(32 * kWarps) scalar_kernel(const __grid_constant__ RotaryArgs a, int interleaved) {
   __shared__ float s_dw[BWD ? kWarps : 1][BWD ? 32 * NJ : 1];
-  const SblNormRotarySide& s = a.side[blockIdx.z];
+  const int side = a.side0 + blockIdx.z;
+  const SblNormRotarySide& s = a.side[side];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int E = a.E, half = a.rotary / 2;
   float wt[NJ], wp[NJ], dw[NJ];
@@ -458,7 +460,7 @@ __global__ void __launch_bounds__(32 * kWarps) scalar_kernel(const __grid_consta
 #pragma unroll
     for (int j = 0; j < NJ; ++j) s_dw[warp][lane + 32 * j] = dw[j];
     __syncthreads();
-    const int64_t block = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+    const int64_t block = ((int64_t)side * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
     for (int e = threadIdx.x; e < E; e += 32 * kWarps) {
       float sum = 0.f;
       for (int w = 0; w < kWarps; ++w) sum += s_dw[w][e];
@@ -522,13 +524,19 @@ cudaError_t launch(const SblNormRotary& p, RotaryArgs& a, cudaStream_t st) {
   const bool inter = p.interleaved != 0;
   const bool vec = p.E % 8 == 0 && p.E <= 256 && (inter || p.rotary % 16 == 0) && side_is_vec(p.side[0], BWD) &&
                    side_is_vec(p.side[1], BWD);
+  // A side whose gradients nobody needs has no blocks.  The plan is that of both, so that the other side's sums keep
+  // their order.
+  const bool skip0 = BWD && !p.side[0].y && !p.side[0].dweight, skip1 = BWD && !p.side[1].y && !p.side[1].dweight;
+  if (skip0 && skip1) return cudaSuccess;
+  a.side0 = skip0;
+  const unsigned sides = skip0 || skip1 ? 1 : 2;
   unsigned gx, gy;
   bool joint;
   if (vec) {
     const int lpr = p.E <= 32 ? 4 : p.E <= 64 ? 8 : p.E <= 128 ? 16 : 32;
     plan(p, 32 / lpr, BWD, &gx, &gy, &joint);
-    a.joint = joint;
-    const dim3 grid(gx, gy, a.joint ? 1 : 2);
+    a.joint = joint && sides == 2;
+    const dim3 grid(gx, gy, a.joint ? 1 : sides);
 #define SBL_VEC(L)                                                                                  \
   (inter ? vec_kernel<T, L, BWD, true><<<grid, 32 * kWarps, 0, st>>>(a)                             \
          : vec_kernel<T, L, BWD, false><<<grid, 32 * kWarps, 0, st>>>(a))
@@ -539,7 +547,7 @@ cudaError_t launch(const SblNormRotary& p, RotaryArgs& a, cudaStream_t st) {
 #undef SBL_VEC
   } else {
     plan(p, 1, BWD, &gx, &gy, &joint);
-    const dim3 grid(gx, gy, 2);
+    const dim3 grid(gx, gy, sides);
     if (p.E <= 128) scalar_kernel<T, 4, BWD><<<grid, 32 * kWarps, 0, st>>>(a, inter);
     else scalar_kernel<T, 16, BWD><<<grid, 32 * kWarps, 0, st>>>(a, inter);
   }

@@ -370,7 +370,8 @@ def _norm_rotary_params(xs, ys, weights, positions, pos0, rotary_dim, theta, int
     fields = [_DTYPES[xs[0].dtype], _DTYPES[w.dtype] if w is not None else _cabi.SBL_DTYPE_F32, B, E, rotary_dim,
               1 if interleaved else 0, eps, theta]
     for x, y, dy, w, dw, pos in zip(xs, ys, dys, weights, dws, positions):
-        fields += [x.shape[1], x.shape[2], x.data_ptr(), *x.stride()[:3], y.data_ptr(), *y.stride()[:3]]
+        fields += [x.shape[1], x.shape[2], x.data_ptr(), *x.stride()[:3]]
+        fields += [y.data_ptr(), *y.stride()[:3]] if y is not None else [0, 0, 0, 0]
         fields += [dy.data_ptr(), *dy.stride()[:3]] if dy is not None else [0, 0, 0, 0]
         fields += [w.data_ptr() if w is not None else 0, dw.data_ptr() if dw is not None else 0]
         fields += ([pos.data_ptr(), pos.stride(0) if pos.dim() == 2 else 0, pos.stride(-1)] if pos is not None
@@ -405,9 +406,11 @@ class _NormRotary(torch.autograd.Function):
         weights = (query_weight, key_weight)
         dev = query.device
         dys = [dy if dy.stride(-1) == 1 else dy.contiguous() for dy in (dq_out, dk_out)]
-        dxs = [torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (query, key)]
         dws = [torch.empty_like(w) if w is not None and ctx.needs_input_grad[2 + i] else None
                for i, w in enumerate(weights)]
+        # (a side of which nothing is needed is left out; one whose weight alone is needed has the place of its dx)
+        dxs = [torch.empty(x.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[i] or dws[i] is not None else None
+               for i, x in enumerate((query, key))]
         p = _norm_rotary_params((query, key), dxs, weights, (positions, key_positions), *ctx.args, dys, dws)
         lib = _cabi.load()
         ws, nbytes = None, 0
@@ -420,7 +423,8 @@ class _NormRotary(torch.autograd.Function):
             rc = lib.sbl_norm_rotary_backward(ctypes.byref(p), ws.data_ptr() if ws is not None else None, nbytes,
                                               _stream(dev))
         _cabi.check(rc)
-        return (*dxs, *dws, *([None] * (2 + len(ctx.args))))
+        return (*(dx if need else None for dx, need in zip(dxs, ctx.needs_input_grad)), *dws,
+                *([None] * (2 + len(ctx.args))))
 
 
 def qk_norm_rotary(query, key, query_weight=None, key_weight=None, positions=None, key_positions=None, pos0=0,

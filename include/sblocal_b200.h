@@ -290,7 +290,8 @@ int sbl_backward(const SblParams* p, const SblGrads* g, void* workspace, size_t 
  * position * theta^(-2i/rotary); the entries behind them stay.  side[0] is the
  * query, side[1] the key; they may differ in length and heads.  Angles are
  * reduced in fp64, so far positions keep their accuracy; sums are fp32.  y must
- * not overlap x or dy.  No counterpart in the reference.
+ * not overlap x or dy.  Backward, a side without y and dweight is left out.  No
+ * counterpart in the reference.
  */
 typedef struct SblNormRotarySide {
   int32_t T, H;               /* rows and heads; a side without rows may have null pointers */

@@ -54,3 +54,39 @@ def test_any_part_of_the_gradients(d, r, dtype, sbl_lib):
     for needs in NEEDS:
         got = prob.backward(dout, stats, needs=needs)
         assert all(torch.equal(a, b) if n else a is None for a, b, n in zip(got, every, needs))
+
+
+def test_rotation_side_without_a_place_is_left_out(sbl_lib):
+    from test_training_host import _rotary
+    p, n = _rotary(), ctypes.c_size_t(0)
+    p.side[0].y = None
+    p.side[1].dweight = 4096
+    assert sbl_lib.sbl_norm_rotary_forward(ctypes.byref(p), None) == -1
+    # (-3: behind the checks of the sides, the workspace is missing)
+    assert sbl_lib.sbl_norm_rotary_backward(ctypes.byref(p), None, 0, None) == -3
+    assert sbl_lib.sbl_norm_rotary_workspace_bytes(ctypes.byref(p), ctypes.byref(n)) == 0 and n.value > 0
+    p.side[0].dweight = 4096
+    assert sbl_lib.sbl_norm_rotary_backward(ctypes.byref(p), None, 0, None) == -1
+    p.side[0].dweight = p.side[1].dweight = p.side[1].y = None
+    assert sbl_lib.sbl_norm_rotary_backward(ctypes.byref(p), None, 0, None) == 0      # nothing to do
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('interleaved', [False, True])
+@pytest.mark.parametrize('B,T,S,Hq,Hk,E,dtype', [
+    (2, 1300, 1300, 5, 2, 64, torch.bfloat16), (3, 7, 7, 16, 4, 128, torch.bfloat16), (2, 40, 90, 3, 3, 64, torch.float32),
+    (2, 300, 300, 3, 2, 21, torch.float32), (2, 300, 0, 3, 2, 64, torch.float32)])
+def test_any_part_of_the_rotation(B, T, S, Hq, Hk, E, dtype, interleaved, sbl_lib):
+    from fly_b200 import ops
+    from tests.test_norm_rotary_gpu import make
+    q, k, wq, wk, dq, dk = make(B, T, S, Hq, Hk, E, dtype, seed=3)
+    xs = (q, k, wq, wk)
+    whole = [x.clone().requires_grad_() for x in xs]
+    want = torch.autograd.grad(ops.qk_norm_rotary(*whole, interleaved=interleaved), whole, (dq, dk))
+    for needs in itertools.product((False, True), repeat=4):
+        if not any(needs):
+            continue
+        leaves = [x.clone().requires_grad_(n) for x, n in zip(xs, needs)]
+        torch.autograd.backward(ops.qk_norm_rotary(*leaves, interleaved=interleaved), (dq, dk))
+        for x, need, y in zip(leaves, needs, want):
+            assert (x.grad is not None) == need and (not need or torch.equal(x.grad, y))
