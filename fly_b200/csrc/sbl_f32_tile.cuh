@@ -1,6 +1,7 @@
-// Block-tile helpers of the generic fp32 kernels, forward (sbl_f32.cu) and
-// backward (sbl_bwd_f32.cu): 64x64 register-tiled products fed from shared
-// memory in K-slices of 16 with the next slice prefetched into registers.
+// Helpers of the generic fp32 kernels: the loads and stores of either storage
+// type, which forward (sbl_f32.cu) and backward (sbl_bwd_f32.cu) share, and the
+// forward's 64x64 register-tiled products, fed from shared memory in K-slices of
+// 16 with the next slice prefetched into registers.
 #pragma once
 
 #include "sbl_common.cuh"

@@ -68,7 +68,7 @@ class SBLocalAttention(nn.Module):
         objects (fly_b200.masking or the reference's).  Returns
         (out (B,T,H,D), None)."""
         # A device-side problem of an earlier forward (a wait that ran out, logits beyond the bf16 kernels' range)
-        # surfaces here, without a host synchronisation: only status copies that have already landed are read.
+        # surfaces here, without a host synchronisation: only what has already arrived in host memory is read.
         ops.status_watch.poll()
         if self.causal:
             raise NotImplementedError('causal SBLocal attention is not built')
