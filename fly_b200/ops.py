@@ -53,7 +53,9 @@ class _StatusWatch:
         if any(self._words):
             with self._lock:
                 words = list(self._words)
-                self._words[:] = [0, 0, 0]
+                for i, word in enumerate(words):
+                    if word:               # (one that arrives meanwhile is left for the next look)
+                        self._words[i] = 0
             self._report(words)
 
     @staticmethod

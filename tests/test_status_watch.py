@@ -110,6 +110,26 @@ def test_the_gradients_words_are_watched(watch, sbl_lib, monkeypatch):
         watch.poll(wait=True)
 
 
+def test_a_word_that_arrives_during_a_report_is_kept(watch):
+    from fly_b200 import _cabi
+
+    class Words(list):
+        reads = 0
+
+        def __iter__(self):
+            seen = [self[i] for i in range(3)]
+            self.reads += 1
+            if self.reads == 2:            # a kernel of another stream, while the words are taken down
+                self[2] = 1
+            return iter(seen)
+
+    watch._words = Words([0, 1, 0])
+    with pytest.raises(_cabi.SblError, match='range'):
+        watch.poll()
+    with pytest.raises(_cabi.SblError, match='16 times'):
+        watch.poll()
+
+
 @pytest.mark.gpu
 def test_zeros_leave_what_was_collected(sbl_lib):
     from fly_b200 import _cabi
